@@ -281,6 +281,122 @@ RTA_API rta_status rta_gated_delta_step(const float* x, const float* attn_norm, 
 RTA_API rta_status rta_workspace_error(const void* workspace, size_t workspace_bytes, void* stream, uint32_t* error_word);
 
 
+/* ------------------------------------------------------- 1c. paged K/V cache
+ *
+ * A cache of many sequences whose histories live in pages of one pool, next to
+ * the model handle's one ring per sequence: attention over the pages for one
+ * new token per sequence and for ragged batches of new tokens, the writes of
+ * new rows, and the bookkeeping of pages.  No reference counterpart: the
+ * reference keeps one sequence per process (optical_resident.cpp:964-971); its
+ * shared 16-position history blocks (shared_history_cache.hpp:5-142) are the
+ * nearest relative.
+ *
+ * rta_page_pool: K and V of every layer, format RTA_F16 or RTA_BF16.  Element
+ * (layer, page, kv head, position in the page, dim) of K is
+ *   k + layer * layer_stride + page * page_stride + head * head_stride
+ *     + position * position_stride + dim            (strides in elements),
+ * of V the same from v: both [page][head][position][dim] and
+ * [page][position][head][dim] pools, and pools that interleave K and V, are
+ * described so.  head_dim is 64, 128 or 256; strides are multiples of 8
+ * elements, k and v 16-byte aligned; page_size is 1 .. 65536.
+ *
+ * rta_page_map: device arrays.  lengths[slot] positions of slot's sequence are
+ * held; position p lives in page table[slot * width + p / page_size]; unused
+ * table entries are -1; refs[page] counts the table entries that name the page
+ * (0: free).  width * page_size must stay below 2^31.
+ *
+ * Every call takes a workspace of rta_paged_workspace_bytes() bytes, 16-byte
+ * aligned, that the caller zeroes ONCE before its first use (the attention
+ * calls leave their counters zeroed).  Calls that share a workspace, or a map
+ * that one of them writes, must be ordered on one stream.  Device-side checks
+ * accumulate in the workspace's first word, read by rta_workspace_error and
+ * cleared by zeroing that word: 4 = the map names a page outside the pool or
+ * one without references, 8 = not enough free pages, 16 = a bad slot or count;
+ * 1 = a bounded device-side wait expired (then zero the whole workspace).
+ * `slots` (device, `batch` entries) names the sequences of a call; NULL means
+ * slots 0 .. batch - 1. */
+typedef struct rta_page_pool {
+  void *k, *v;
+  int32_t format;
+  uint32_t layers, pages, page_size, kv_heads, head_dim;
+  uint64_t layer_stride, page_stride, head_stride, position_stride;
+} rta_page_pool;
+typedef struct rta_page_map {
+  int32_t *refs, *table, *lengths;
+  uint32_t slots, width;
+} rta_page_map;
+RTA_API size_t rta_paged_workspace_bytes(const rta_page_pool* pool, const rta_page_map* map);
+
+/* Attention of one new token per sequence (already written to the pages and
+ * counted in lengths): the token at position t = lengths[slot] - 1 sees the
+ * positions p <= t with p > t - window or p < sinks (window 0: all p <= t).
+ *   out[b][h] = sum_p softmax_p(scale q[b][h] . k_p) v_p, K/V head
+ *   h / (heads / kv_heads);  lse[b][h] = log sum_p exp(scale q . k_p)
+ * q: element (b, h, d) at q + b * q_row_stride + h * q_head_stride + d, 16-byte
+ * aligned rows, q_format the pool's format, or RTA_F32 with an RTA_F16 pool;
+ * out [batch][heads][head_dim] contiguous in q's format; lse [batch][heads]
+ * fp32 or NULL.  A sequence of length 0 gives zeros and lse -inf.  heads is a
+ * multiple of kv_heads, at most 128 query heads per K/V head. */
+RTA_API rta_status rta_paged_decode(const rta_page_pool* pool, const rta_page_map* map, uint32_t layer,
+                                    const int32_t* slots, uint32_t batch, const void* q, int q_format, uint32_t heads,
+                                    uint64_t q_row_stride, uint64_t q_head_stride, float scale, uint32_t window,
+                                    uint32_t sinks, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                                    void* stream);
+
+/* The same attention for `rows` new tokens: sequence b of the call owns rows
+ * starts[b] .. starts[b + 1] - 1 (device, batch + 1 entries, ascending from 0
+ * to rows), already written to the pages and counted in lengths; row i of m
+ * sits at position t = lengths[slot] - m + i.  q_format is the pool's format;
+ * out [rows][heads][head_dim], lse [rows][heads].  A row before position 0
+ * (more new rows than the sequence is long) gives zeros and lse -inf.  What a
+ * row does not see never reaches it, non-finite values included. */
+RTA_API rta_status rta_paged_prefill(const rta_page_pool* pool, const rta_page_map* map, uint32_t layer,
+                                     const int32_t* slots, uint32_t batch, const int32_t* starts, uint32_t rows,
+                                     const void* q, int q_format, uint32_t heads, uint64_t q_row_stride,
+                                     uint64_t q_head_stride, float scale, uint32_t window, uint32_t sinks, void* out,
+                                     float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Write the K and V rows of new tokens (element (row, head, d) at
+ * row * row_stride + head * head_stride + d, 16-byte aligned rows, format the
+ * pool's or RTA_F32, rounded once) to their positions, `starts` and positions
+ * as in rta_paged_prefill (rta_pages_reserve has grown the sequences). */
+RTA_API rta_status rta_paged_append(const rta_page_pool* pool, const rta_page_map* map, uint32_t layer,
+                                    const int32_t* slots, uint32_t batch, const int32_t* starts, uint32_t rows,
+                                    const void* k, const void* v, int format, uint64_t row_stride,
+                                    uint64_t head_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bookkeeping.  Each call reads `map` and leaves the result in `out`, which is
+ * `map` itself or a map of the same slots and width with arrays of its own.
+ * A call whose check fails on the device changes nothing (out = map).
+ *
+ * reserve: slots[i]'s sequence grows by counts[i] >= 0 positions; the pages it
+ * lacks are the lowest free ones, taken in the order of the call.  Slots are
+ * distinct. */
+RTA_API rta_status rta_pages_reserve(const rta_page_pool* pool, const rta_page_map* map, const rta_page_map* out,
+                                     const int32_t* slots, const int32_t* counts, uint32_t batch, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+/* fork: the empty slot dst[i] becomes a copy of src[i]: full pages are shared
+ * (refs + 1), the positions of a partly filled last page are copied, in every
+ * layer, to the lowest free page.  dst are distinct and none of them a src. */
+RTA_API rta_status rta_pages_fork(const rta_page_pool* pool, const rta_page_map* map, const rta_page_map* out,
+                                  const int32_t* src, const int32_t* dst, uint32_t count, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+/* free: refs - 1 for every page of the slots, their table entries -1, their
+ * lengths 0.  (A page without references is flagged and left at 0.) */
+RTA_API rta_status rta_pages_free(const rta_page_pool* pool, const rta_page_map* map, const rta_page_map* out,
+                                  const int32_t* slots, uint32_t count, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+/* compact: with L pages in use, the k-th free page below L takes the data (of
+ * every layer), references and table entries of the k-th page in use from L
+ * on; afterwards pages 0 .. L - 1 are the ones in use.  live (device, may be
+ * NULL) receives L. */
+RTA_API rta_status rta_pages_compact(const rta_page_pool* pool, const rta_page_map* map, const rta_page_map* out,
+                                     uint32_t* live, void* workspace, size_t workspace_bytes, void* stream);
+/* copy: page dst[i] takes the data of page src[i] in every layer (device
+ * arrays, at most `pages` of them; no dst is a src, and dst are distinct). */
+RTA_API rta_status rta_pages_copy(const rta_page_pool* pool, const int32_t* src, const int32_t* dst, uint32_t count,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------ 2. resident model */
 
 /* Model geometry: the fields of the compiler's ModelSpec

@@ -1,0 +1,465 @@
+// pages.cu -- writes of new K/V rows into a paged cache, and the bookkeeping
+// of its pages: reserve, fork, free, compact, copy.
+//
+// Everything is decided on the device (no call waits for the host): one block
+// plans -- it ranks free pages, holes and movers with block-wide sums, so the
+// choice is the lowest page first, whatever the order of threads -- and a
+// launch over the whole device moves the data.  The moves of a plan have
+// disjoint sources and destinations, so they run in any order.
+#include "paged_device.cuh"
+
+namespace rta {
+namespace paged {
+namespace {
+
+// ------------------------------------------------------------------ append
+// One warp per (new row, K/V head): K and V rows of head_dim elements, 16
+// bytes written per lane and step.
+template <typename T, typename X>
+__device__ __forceinline__ uint4 convert8(const X* src);
+template <>
+__device__ __forceinline__ uint4 convert8<__half, __half>(const __half* src) {
+  return *reinterpret_cast<const uint4*>(src);
+}
+template <>
+__device__ __forceinline__ uint4 convert8<__nv_bfloat16, __nv_bfloat16>(const __nv_bfloat16* src) {
+  return *reinterpret_cast<const uint4*>(src);
+}
+template <typename T>
+__device__ __forceinline__ uint4 round8(const float* src) {
+  const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+  return make_uint4(Num<T>::pack(a.x, a.y), Num<T>::pack(a.z, a.w), Num<T>::pack(b.x, b.y), Num<T>::pack(b.z, b.w));
+}
+template <>
+__device__ __forceinline__ uint4 convert8<__half, float>(const float* src) { return round8<__half>(src); }
+template <>
+__device__ __forceinline__ uint4 convert8<__nv_bfloat16, float>(const float* src) { return round8<__nv_bfloat16>(src); }
+
+template <typename T, typename X>
+__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
+  const uint32_t lane = threadIdx.x & 31u;
+  const uint64_t item = static_cast<uint64_t>(blockIdx.x) * 8u + (threadIdx.x >> 5);
+  if (item >= static_cast<uint64_t>(p.rows) * p.c.kv_heads) return;
+  const uint32_t row = static_cast<uint32_t>(item / p.c.kv_heads), kv = static_cast<uint32_t>(item % p.c.kv_heads);
+  // the sequence: how many of starts[1 .. batch] are <= row
+  uint32_t b = 0;
+  for (uint32_t i = 0; i < p.c.batch; i += 32u)
+    b += __popc(__ballot_sync(0xffffffffu, i + lane < p.c.batch && static_cast<uint32_t>(p.starts[i + lane + 1u]) <= row));
+  if (b >= p.c.batch) {
+    if (lane == 0u) atomicOr(p.err, RTA_DEVERR_SLOT);
+    return;
+  }
+  const Sequence s = sequence(p.c, b, lane == 0u ? p.err : nullptr);
+  const uint32_t new_rows = static_cast<uint32_t>(p.starts[b + 1u] - p.starts[b]);
+  const int64_t at = static_cast<int64_t>(s.length) - new_rows + (row - static_cast<uint32_t>(p.starts[b]));
+  uint64_t off = 0;
+  const bool inside = at >= 0 && at < s.length;
+  if (!inside || !locate(p.c, s.slot, static_cast<uint32_t>(at), off)) {
+    if (lane == 0u) atomicOr(p.err, inside ? RTA_DEVERR_PAGE : RTA_DEVERR_SLOT);
+    return;
+  }
+  off += kv * p.c.head_bytes;
+  const X* ks = static_cast<const X*>(p.k) + row * p.row_stride + kv * p.head_stride;
+  const X* vs = static_cast<const X*>(p.v) + row * p.row_stride + kv * p.head_stride;
+  uint8_t* kd = const_cast<uint8_t*>(p.c.k) + off;
+  uint8_t* vd = const_cast<uint8_t*>(p.c.v) + off;
+  for (uint32_t d = lane * 8u; d < p.c.head_dim; d += 256u) {
+    const uint4 a = convert8<T, X>(ks + d), c = convert8<T, X>(vs + d);
+    *reinterpret_cast<uint4*>(kd + d * 2u) = a;
+    *reinterpret_cast<uint4*>(vd + d * 2u) = c;
+  }
+}
+
+// ------------------------------------------------------------------ plans
+// Scratch words of a plan: [0] moves, then per move source page, destination
+// page and positions, then the free-page list, or for compact the map of moved
+// pages.
+constexpr uint32_t kPlanHead = 8;
+struct Plan {
+  uint32_t *moves, *src, *dst, *held, *list;
+  __device__ __forceinline__ Plan(uint32_t* w, uint32_t pages, uint32_t slots) {
+    const uint32_t most = pages > slots ? pages : slots;
+    moves = w;
+    src = w + kPlanHead;
+    dst = src + most;
+    held = dst + most;
+    list = held + most;
+  }
+};
+
+constexpr uint32_t kPlanThreads = 1024;
+
+// The first `want` free pages, ascending, into list (at most `want` of them);
+// returns how many there are.
+__device__ uint32_t list_free(const int32_t* refs, uint32_t pages, uint32_t want, uint32_t* list, uint64_t* part) {
+  uint64_t found = 0;
+  for (uint32_t p0 = 0; p0 < pages && found < want; p0 += kPlanThreads * 4u) {
+    const uint32_t p = p0 + threadIdx.x * 4u;
+    uint32_t free_mask = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; ++k)
+      if (p + k < pages && refs[p + k] == 0) free_mask |= 1u << k;
+    uint64_t sum;
+    const uint32_t n = __popc(free_mask);
+    uint64_t at = found + block_scan(n, part, sum) - n;
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; ++k)
+      if (free_mask >> k & 1u) {
+        if (at < want) list[at] = p + k;
+        ++at;
+      }
+    found += sum;
+  }
+  __syncthreads();
+  return static_cast<uint32_t>(found < want ? found : want);
+}
+
+__global__ void map_copy_kernel(MapArrays from, MapArrays to, uint32_t pages, uint32_t slots, uint64_t cells) {
+  const uint64_t stride = static_cast<uint64_t>(gridDim.x) * blockDim.x;
+  const uint64_t t = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  for (uint64_t i = t; i < cells; i += stride) to.table[i] = from.table[i];
+  for (uint64_t i = t; i < pages; i += stride) to.refs[i] = from.refs[i];
+  for (uint64_t i = t; i < slots; i += stride) to.lengths[i] = from.lengths[i];
+}
+
+__global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const PagesParams p) {
+  __shared__ uint64_t part[32];
+  const Plan plan(p.plan, p.pages, p.slot_count);
+  uint64_t total = 0;
+  bool bad = false;
+  for (uint32_t i0 = 0; i0 < p.count; i0 += kPlanThreads) {
+    const uint32_t i = i0 + threadIdx.x;
+    uint64_t need = 0, sum;
+    if (i < p.count) {
+      const int32_t slot = p.a ? p.a[i] : static_cast<int32_t>(i), add = p.b[i];
+      if (slot < 0 || static_cast<uint32_t>(slot) >= p.slot_count || add < 0) {
+        bad = true;
+      } else {
+        const int64_t n = p.map.lengths[slot];
+        if (n < 0 || n + add > static_cast<int64_t>(p.width) * p.page_size)
+          bad = true;
+        else
+          need = (n + add + p.page_size - 1) / p.page_size - (n + p.page_size - 1) / p.page_size;
+      }
+    }
+    const uint64_t first = total + block_scan(need, part, sum) - need;
+    if (i < p.count) plan.src[i] = static_cast<uint32_t>(first);
+    total += sum;
+  }
+  if (__syncthreads_or(bad ? 1 : 0)) {
+    if (threadIdx.x == 0) atomicOr(p.err, RTA_DEVERR_SLOT);
+    return;
+  }
+  if (total > p.pages || list_free(p.map.refs, p.pages, static_cast<uint32_t>(total), plan.list, part) < total) {
+    if (threadIdx.x == 0) atomicOr(p.err, RTA_DEVERR_POOL);
+    return;
+  }
+  for (uint32_t k = threadIdx.x; k < total; k += kPlanThreads) p.map.refs[plan.list[k]] = 1;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  for (uint32_t i = warp; i < p.count; i += kPlanThreads / 32u) {
+    const uint32_t slot = p.a ? p.a[i] : i;
+    const uint32_t n = p.map.lengths[slot], grown = n + p.b[i];
+    const uint32_t have = (n + p.page_size - 1u) / p.page_size, need = (grown + p.page_size - 1u) / p.page_size;
+    for (uint32_t j = have + lane; j < need; j += 32u)
+      p.map.table[static_cast<size_t>(slot) * p.width + j] = static_cast<int32_t>(plan.list[plan.src[i] + j - have]);
+    __syncwarp();
+    if (lane == 0u) p.map.lengths[slot] = static_cast<int32_t>(grown);
+  }
+}
+
+// Claims the destinations, ranks the partly filled last pages, takes a page
+// for each; the launch after it shares the full pages and copies the rest.
+__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagesParams p) {
+  __shared__ uint64_t part[32];
+  __shared__ uint32_t fault;
+  const Plan plan(p.plan, p.pages, p.slot_count);
+  if (threadIdx.x == 0) {
+    *plan.moves = 0u;
+    fault = 0u;
+  }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < p.count; i += kPlanThreads) {
+    const int32_t dst = p.b[i];
+    if (dst < 0 || static_cast<uint32_t>(dst) >= p.slot_count ||
+        atomicCAS(&p.map.lengths[dst], 0, -1 - static_cast<int32_t>(i)) != 0)
+      atomicOr(&fault, RTA_DEVERR_SLOT);
+  }
+  __syncthreads();
+  uint64_t total = 0;
+  for (uint32_t i0 = 0; i0 < p.count; i0 += kPlanThreads) {
+    const uint32_t i = i0 + threadIdx.x;
+    uint64_t need = 0, sum;
+    if (i < p.count) {
+      const int32_t src = p.a[i];
+      const int32_t n = src >= 0 && static_cast<uint32_t>(src) < p.slot_count ? p.map.lengths[src] : -1;
+      if (n < 0 || static_cast<uint32_t>(n) > p.width * p.page_size) {
+        atomicOr(&fault, RTA_DEVERR_SLOT);
+      } else {
+        const uint32_t rest = static_cast<uint32_t>(n) % p.page_size;
+        if (rest) {
+          const int32_t page = p.map.table[static_cast<size_t>(src) * p.width + static_cast<uint32_t>(n) / p.page_size];
+          if (static_cast<uint32_t>(page) >= p.pages) atomicOr(&fault, RTA_DEVERR_PAGE);
+          plan.src[i] = static_cast<uint32_t>(page);
+          need = 1u;
+        }
+        plan.held[i] = rest;
+      }
+    }
+    const uint64_t first = total + block_scan(need, part, sum) - need;
+    if (i < p.count) plan.dst[i] = static_cast<uint32_t>(first);
+    total += sum;
+  }
+  __syncthreads();
+  uint32_t wrong = fault;
+  if (!wrong && (total > p.pages ||
+                 list_free(p.map.refs, p.pages, static_cast<uint32_t>(total), plan.list, part) < total))
+    wrong = RTA_DEVERR_POOL;
+  if (wrong) {  // give the claimed slots back
+    for (uint32_t i = threadIdx.x; i < p.count; i += kPlanThreads) {
+      const int32_t dst = p.b[i];
+      if (dst >= 0 && static_cast<uint32_t>(dst) < p.slot_count)
+        atomicCAS(&p.map.lengths[dst], -1 - static_cast<int32_t>(i), 0);
+    }
+    if (threadIdx.x == 0) atomicOr(p.err, wrong);
+    return;
+  }
+  for (uint32_t k = threadIdx.x; k < total; k += kPlanThreads) p.map.refs[plan.list[k]] = 1;
+  for (uint32_t i = threadIdx.x; i < p.count; i += kPlanThreads) {
+    plan.dst[i] = plan.held[i] ? plan.list[plan.dst[i]] : 0u;
+    p.map.lengths[p.b[i]] = p.map.lengths[p.a[i]];
+  }
+  if (threadIdx.x == 0) *plan.moves = p.count;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagesParams p) {
+  __shared__ uint64_t part[32];
+  const Plan plan(p.plan, p.pages, p.slot_count);
+  uint64_t mine = 0, live;
+  for (uint32_t i = threadIdx.x; i < p.pages; i += kPlanThreads) mine += p.map.refs[i] > 0 ? 1u : 0u;
+  block_scan(mine, part, live);
+  uint64_t holes = 0, movers = 0;
+  for (uint32_t p0 = 0; p0 < p.pages; p0 += kPlanThreads * 4u) {
+    const uint32_t i = p0 + threadIdx.x * 4u;
+    uint32_t hole = 0, mover = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; ++k)
+      if (i + k < p.pages) {
+        const bool used = p.map.refs[i + k] > 0;
+        if (!used && i + k < live) hole |= 1u << k;
+        if (used && i + k >= live) mover |= 1u << k;
+        if (!used && i + k >= live) plan.list[i + k] = 0xffffffffu;  // no table entry should name it
+      }
+    uint64_t sum;  // both ranks in one scan: holes in the low half, movers in the high half
+    const uint64_t n = __popc(hole) | static_cast<uint64_t>(__popc(mover)) << 32;
+    const uint64_t before = block_scan(n, part, sum) - n;
+    uint32_t h = static_cast<uint32_t>(holes + (before & 0xffffffffu)), m = static_cast<uint32_t>(movers + (before >> 32));
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; ++k) {
+      if (hole >> k & 1u) plan.dst[h++] = i + k;
+      if (mover >> k & 1u) plan.src[m++] = i + k;
+    }
+    holes += sum & 0xffffffffu;
+    movers += sum >> 32;
+  }
+  __syncthreads();  // holes == movers: both count the pages in use from `live` on
+  for (uint32_t k = threadIdx.x; k < movers; k += kPlanThreads) {
+    const uint32_t s = plan.src[k], d = plan.dst[k];
+    plan.list[s] = d;
+    plan.held[k] = p.page_size;
+    p.map.refs[d] = p.map.refs[s];
+    p.map.refs[s] = 0;
+  }
+  if (threadIdx.x == 0) {
+    plan.moves[0] = static_cast<uint32_t>(movers);
+    plan.moves[1] = static_cast<uint32_t>(live);
+    if (p.live) *p.live = static_cast<uint32_t>(live);
+  }
+}
+
+__global__ void __launch_bounds__(kPlanThreads) copy_plan_kernel(const PagesParams p) {
+  const Plan plan(p.plan, p.pages, p.slot_count);
+  for (uint32_t i = threadIdx.x; i < p.count; i += kPlanThreads) {
+    const uint32_t s = p.a[i], d = p.b[i];
+    const bool ok = s < p.pages && d < p.pages;
+    if (!ok) atomicOr(p.err, RTA_DEVERR_PAGE);
+    plan.src[i] = ok ? s : 0u;
+    plan.dst[i] = ok ? d : 0u;
+    plan.held[i] = ok ? p.page_size : 0u;
+  }
+  if (threadIdx.x == 0) *plan.moves = p.count;
+}
+
+// ------------------------------------------------------------------ moves
+enum { kMoveFork = 0, kMoveCompact = 1, kMoveCopy = 2 };
+constexpr uint32_t kPiece = 4096;  // bytes one warp moves per step: eight 16-byte loads in flight per lane
+
+template <int KIND>
+__global__ void __launch_bounds__(256) move_kernel(const PagesParams p) {
+  const Plan plan(p.plan, p.pages, p.slot_count);
+  const uint32_t lane = threadIdx.x & 31u;
+  const uint64_t warps = static_cast<uint64_t>(gridDim.x) * 8u;
+  const uint64_t me = static_cast<uint64_t>(blockIdx.x) * 8u + (threadIdx.x >> 5);
+  const uint32_t moves = *plan.moves;
+  if (KIND == kMoveFork) {
+    for (uint64_t i = me; i < moves; i += warps) {  // share the full pages, end the row
+      const uint32_t src = p.a[i], dst = p.b[i], rest = plan.held[i];
+      const uint32_t full = static_cast<uint32_t>(p.map.lengths[src]) / p.page_size;
+      const int32_t* from = p.map.table + static_cast<size_t>(src) * p.width;
+      int32_t* to = p.map.table + static_cast<size_t>(dst) * p.width;
+      for (uint32_t j = lane; j < p.width; j += 32u) {
+        int32_t page = -1;
+        if (j < full) {
+          page = from[j];
+          if (static_cast<uint32_t>(page) < p.pages)
+            atomicAdd(&p.map.refs[page], 1);
+          else
+            atomicOr(p.err, RTA_DEVERR_PAGE);
+        } else if (j == full && rest) {
+          page = static_cast<int32_t>(plan.dst[i]);
+        }
+        to[j] = page;
+      }
+    }
+  }
+  if (KIND == kMoveCompact) {
+    const uint32_t live = plan.moves[1];
+    const uint64_t cells = static_cast<uint64_t>(p.slot_count) * p.width;
+    for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < cells; i += warps * 32u) {
+      const int32_t page = p.map.table[i];
+      if (page >= 0 && static_cast<uint32_t>(page) >= live) {
+        const uint32_t to = static_cast<uint32_t>(page) < p.pages ? plan.list[page] : 0xffffffffu;
+        if (to != 0xffffffffu)
+          p.map.table[i] = static_cast<int32_t>(to);
+        else
+          atomicOr(p.err, RTA_DEVERR_PAGE);
+      }
+    }
+  }
+  // (move, layer, K or V, head, piece of the head's positions)
+  const uint32_t pieces = (p.page_size * p.row_bytes + kPiece - 1u) / kPiece;
+  const uint64_t items = static_cast<uint64_t>(moves) * p.layers * 2u * p.kv_heads * pieces;
+  const uint32_t per_row = p.row_bytes / 16u;
+  for (uint64_t it = me; it < items; it += warps) {
+    uint64_t x = it;
+    const uint32_t piece = static_cast<uint32_t>(x % pieces);
+    x /= pieces;
+    const uint32_t head = static_cast<uint32_t>(x % p.kv_heads);
+    x /= p.kv_heads;
+    const uint32_t is_v = static_cast<uint32_t>(x & 1u);
+    x >>= 1;
+    const uint32_t layer = static_cast<uint32_t>(x % p.layers), i = static_cast<uint32_t>(x / p.layers);
+    const uint32_t chunks = plan.held[i] * per_row, c0 = piece * (kPiece / 16u);
+    if (c0 >= chunks) continue;
+    uint8_t* const base = (is_v ? p.v : p.k) + layer * p.layer_bytes + head * p.head_bytes;
+    const uint8_t* const from = base + plan.src[i] * p.page_bytes;
+    uint8_t* const to = base + plan.dst[i] * p.page_bytes;
+    uint4 v[kPiece / 512u];
+#pragma unroll
+    for (uint32_t k = 0; k < kPiece / 512u; ++k) {
+      const uint32_t c = c0 + k * 32u + lane;
+      if (c < chunks) v[k] = __ldcs(reinterpret_cast<const uint4*>(from + c / per_row * p.pos_bytes + c % per_row * 16u));
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < kPiece / 512u; ++k) {
+      const uint32_t c = c0 + k * 32u + lane;
+      if (c < chunks) *reinterpret_cast<uint4*>(to + c / per_row * p.pos_bytes + c % per_row * 16u) = v[k];
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) free_kernel(const PagesParams p) {
+  __shared__ int32_t length;
+  const int32_t slot = p.a[blockIdx.x];
+  if (slot < 0 || static_cast<uint32_t>(slot) >= p.slot_count) {
+    if (threadIdx.x == 0) atomicOr(p.err, RTA_DEVERR_SLOT);
+    return;
+  }
+  if (threadIdx.x == 0) length = atomicExch(&p.map.lengths[slot], 0);  // a slot named twice is freed once
+  __syncthreads();
+  const int32_t n = length;
+  if (n <= 0) {
+    if (n < 0 && threadIdx.x == 0) atomicOr(p.err, RTA_DEVERR_SLOT);
+    return;
+  }
+  uint32_t held = (static_cast<uint32_t>(n) + p.page_size - 1u) / p.page_size;
+  if (held > p.width) held = p.width;
+  for (uint32_t j = threadIdx.x; j < held; j += blockDim.x) {
+    int32_t* cell = p.map.table + static_cast<size_t>(slot) * p.width + j;
+    const int32_t page = *cell;
+    *cell = -1;
+    if (static_cast<uint32_t>(page) >= p.pages) {
+      atomicOr(p.err, RTA_DEVERR_PAGE);
+    } else if (atomicSub(&p.map.refs[page], 1) <= 0) {
+      atomicAdd(&p.map.refs[page], 1);
+      atomicOr(p.err, RTA_DEVERR_PAGE);
+    }
+  }
+}
+
+constexpr uint32_t kMoveBlocks = 148 * 6;
+
+}  // namespace
+
+size_t plan_bytes(uint32_t pages, uint32_t slots) {
+  const size_t most = pages > slots ? pages : slots;
+  return (kPlanHead + 4u * most) * 4u;
+}
+
+cudaError_t launch_append(const AppendParams& p, int fmt, int in_fmt, cudaStream_t s) {
+  const uint64_t items = static_cast<uint64_t>(p.rows) * p.c.kv_heads;
+  if (items == 0u) return cudaSuccess;
+  const uint64_t blocks = (items + 7u) / 8u;
+  if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
+  const dim3 grid(static_cast<uint32_t>(blocks));
+  if (fmt == kF16 && in_fmt == kF32)
+    append_kernel<__half, float><<<grid, 256, 0, s>>>(p);
+  else if (fmt == kF16)
+    append_kernel<__half, __half><<<grid, 256, 0, s>>>(p);
+  else if (in_fmt == kF32)
+    append_kernel<__nv_bfloat16, float><<<grid, 256, 0, s>>>(p);
+  else
+    append_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, 256, 0, s>>>(p);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_map_copy(const MapArrays& from, const MapArrays& to, uint32_t pages, uint32_t slots,
+                            uint32_t width, cudaStream_t s) {
+  const uint64_t cells = static_cast<uint64_t>(slots) * width;
+  const uint64_t most = cells > pages ? cells : pages;
+  const uint64_t blocks = (most + 1023u) / 1024u;
+  map_copy_kernel<<<static_cast<uint32_t>(blocks < 592u ? (blocks ? blocks : 1u) : 592u), 256, 0, s>>>(from, to, pages, slots,
+                                                                                                  cells);
+  return cudaGetLastError();
+}
+cudaError_t launch_reserve(const PagesParams& p, cudaStream_t s) {
+  reserve_kernel<<<1, kPlanThreads, 0, s>>>(p);
+  return cudaGetLastError();
+}
+cudaError_t launch_fork(const PagesParams& p, cudaStream_t s) {
+  fork_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  move_kernel<kMoveFork><<<kMoveBlocks, 256, 0, s>>>(p);
+  return cudaGetLastError();
+}
+cudaError_t launch_free(const PagesParams& p, cudaStream_t s) {
+  free_kernel<<<p.count, 256, 0, s>>>(p);
+  return cudaGetLastError();
+}
+cudaError_t launch_compact(const PagesParams& p, cudaStream_t s) {
+  compact_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  move_kernel<kMoveCompact><<<kMoveBlocks, 256, 0, s>>>(p);
+  return cudaGetLastError();
+}
+cudaError_t launch_copy(const PagesParams& p, cudaStream_t s) {
+  copy_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  move_kernel<kMoveCopy><<<kMoveBlocks, 256, 0, s>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace paged
+}  // namespace rta

@@ -18,6 +18,9 @@
 // Device error bits (the host maps any non-zero word to RTA_E_DEVICE_CHECK).
 enum : uint32_t {
   RTA_DEVERR_TIMEOUT = 1u,        // an mbarrier / counter wait exceeded RTA_WAIT_NS
+  RTA_DEVERR_PAGE = 4u,           // paged cache: a table entry outside the pool, or a page without references
+  RTA_DEVERR_POOL = 8u,           // paged cache: not enough free pages
+  RTA_DEVERR_SLOT = 16u,          // paged cache: a bad slot, length or count
   RTA_DEVERR_NONFINITE = 256u,    // mirrors the reference's control[3] bit 256
   RTA_DEVERR_TOKEN = 2048u,       // argmax produced no valid vocabulary row
   RTA_DEVERR_DETECTOR = 65536u,   // mirrors the reference detector error bit

@@ -66,7 +66,31 @@ _SIGNATURES = {
                                                  c_p, c_p, c_u32, c_p, c_p]),
     "rta_gated_delta_step": (c_i32, [c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_u32, c_p, c_p, c_p, c_p, c_p, c_u32, c_u32,
                                      c_u32, c_u32, c_f, c_p, c_p]),
+    "rta_paged_workspace_bytes": (c_sz, [c_p, c_p]),
+    "rta_paged_decode": (c_i32, [c_p, c_p, c_u32, c_p, c_u32, c_p, c_i32, c_u32, c_u64, c_u64, c_f, c_u32, c_u32, c_p,
+                                 c_p, c_p, c_sz, c_p]),
+    "rta_paged_prefill": (c_i32, [c_p, c_p, c_u32, c_p, c_u32, c_p, c_u32, c_p, c_i32, c_u32, c_u64, c_u64, c_f, c_u32,
+                                  c_u32, c_p, c_p, c_p, c_sz, c_p]),
+    "rta_paged_append": (c_i32, [c_p, c_p, c_u32, c_p, c_u32, c_p, c_u32, c_p, c_p, c_i32, c_u64, c_u64, c_p, c_sz,
+                                 c_p]),
+    "rta_pages_reserve": (c_i32, [c_p, c_p, c_p, c_p, c_p, c_u32, c_p, c_sz, c_p]),
+    "rta_pages_fork": (c_i32, [c_p, c_p, c_p, c_p, c_p, c_u32, c_p, c_sz, c_p]),
+    "rta_pages_free": (c_i32, [c_p, c_p, c_p, c_p, c_u32, c_p, c_sz, c_p]),
+    "rta_pages_compact": (c_i32, [c_p, c_p, c_p, c_p, c_p, c_sz, c_p]),
+    "rta_pages_copy": (c_i32, [c_p, c_p, c_p, c_u32, c_p, c_sz, c_p]),
 }
+
+
+class PagePoolC(ctypes.Structure):
+    """rta_page_pool (include/rta.h)."""
+    _fields_ = [("k", c_p), ("v", c_p), ("format", ctypes.c_int32), ("layers", c_u32), ("pages", c_u32),
+                ("page_size", c_u32), ("kv_heads", c_u32), ("head_dim", c_u32), ("layer_stride", c_u64),
+                ("page_stride", c_u64), ("head_stride", c_u64), ("position_stride", c_u64)]
+
+
+class PageMapC(ctypes.Structure):
+    """rta_page_map (include/rta.h)."""
+    _fields_ = [("refs", c_p), ("table", c_p), ("lengths", c_p), ("slots", c_u32), ("width", c_u32)]
 
 
 def header_symbols() -> list[str]:
