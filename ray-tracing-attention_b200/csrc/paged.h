@@ -39,7 +39,7 @@ struct AttendParams {
   void* out;
   float* lse;
   uint32_t* err;
-  uint32_t* counters;  // [kMaxCtas], zero between calls
+  uint32_t* counters;  // [kMaxCtas][2], zero between calls
   float* records;
 };
 

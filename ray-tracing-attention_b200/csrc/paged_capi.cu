@@ -42,7 +42,7 @@ const char* bad_map(const rta_page_pool* p, const rta_page_map* m) {
 
 // Workspace: error word and padding, the counters of split units, then either
 // the split records of an attention call or the plan of a bookkeeping call.
-constexpr size_t kErr = 256, kCounters = (paged::kMaxCtas * 4u + 255u) / 256u * 256u, kBody = kErr + kCounters;
+constexpr size_t kErr = 256, kCounters = (paged::kMaxCtas * 8u + 255u) / 256u * 256u, kBody = kErr + kCounters;
 size_t workspace_bytes_of(const rta_page_pool* p, const rta_page_map* m) {
   size_t body = paged::decode_record_bytes();
   if (paged::prefill_record_bytes() > body) body = paged::prefill_record_bytes();

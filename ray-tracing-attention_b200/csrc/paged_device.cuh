@@ -81,6 +81,7 @@ struct Num<__half> {
   // exp2(score - max) is scaled by 2^10: fp16 weights far below the largest
   // stay clear of the subnormals, the sum carries the same factor.
   static constexpr float kShift = 10.f;
+  static constexpr bool kBf16 = false;
   static __device__ __forceinline__ __half from(float x) { return __float2half_rn(x); }
   static __device__ __forceinline__ float to(__half x) { return __half2float(x); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
@@ -101,6 +102,7 @@ struct Num<__half> {
 template <>
 struct Num<__nv_bfloat16> {
   static constexpr float kShift = 0.f;  // bf16 has fp32's exponents
+  static constexpr bool kBf16 = true;
   static __device__ __forceinline__ __nv_bfloat16 from(float x) { return __float2bfloat16_rn(x); }
   static __device__ __forceinline__ float to(__nv_bfloat16 x) { return __bfloat162float(x); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {

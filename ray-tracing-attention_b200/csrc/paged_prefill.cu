@@ -1,10 +1,35 @@
 // paged_prefill.cu -- attention of many new tokens per sequence over a paged
-// K/V cache, causal, with a window and first tokens that stay visible.
+// K/V cache, causal, with a window and first tokens that stay visible, on the
+// 5th-generation tensor cores.
 //
-// The query heads that share a K/V head are rows of one matrix: row R of a
-// sequence and K/V head is query R / group, head R % group, so a tile of rows
-// reads the K/V head once for all of them.  The positions a tile needs are the
-// first tokens, then a run of neighbours; they are numbered without the gap.
+// Rows.  The query heads that share a K/V head are rows of one matrix: row R
+// of a sequence and K/V head is query R / group, head R % group.  A lane is a
+// tile of 128 rows (the M of an MMA); a unit is the one (head_dim 256) or two
+// lanes that read the same K and V blocks of 128 positions.  The positions a
+// unit needs are the first tokens, then a run of neighbours up to its last
+// row's own; they are numbered without the gap, u < firsts ? u : u + skip.
+//
+// Mathematics.  One pass over the blocks with a running maximum and sum per
+// row, in base 2: S = Q K^T, w = 2^(scale_log2 S - m), O += w V, z += sum w.
+// m follows a block's maximum only when that exceeds it by 2^kSlack: the
+// weights then stay below 2^(kSlack + shift), O and z carry the same factor,
+// and O is seldom rescaled.  w enters the second product rounded to the cache's type
+// (its one rounding; the sum takes w itself).
+//
+// Work: the blocks of all units form one list, cut evenly over the CTAs (one
+// per SM) whatever the lengths are; a lane of a unit that is cut leaves a
+// record (m, z, O) per CTA and the CTA that arrives last joins them in order.
+//
+// Roles (all waits bounded):
+//   softmax    four warps per lane, a thread per row: load Q, take S from
+//              tensor memory, write w back over it, keep m and z, rescale O,
+//              write results or records
+//   MMA        one warp issues S = Q K^T (both operands in shared memory) and
+//              O += w V (w from tensor memory)
+//   producers  three warps copy K and V blocks into a ring of stages (128
+//              positions x up to 128 dimensions, 128-byte swizzle)
+// head_dim 256: one lane, two S buffers, so that S of the next block is
+// computed under this block's softmax; 64 and 128: two lanes take turns.
 #include <atomic>
 #include <mutex>
 
@@ -14,184 +39,823 @@ namespace rta {
 namespace paged {
 namespace {
 
-constexpr uint32_t kRows = 64;  // rows per CTA, sixteen per warp
-constexpr uint32_t kKeys = 32;  // positions per step
+constexpr uint32_t kKeys = 128;      // positions per block
+constexpr uint32_t kLaneRows = 128;  // rows per lane
+constexpr uint32_t kSub = 16384;     // bytes of 128 rows x 64 dimensions
+
+template <int HD>
+struct Shape {
+  static constexpr uint32_t kLanes = HD == 256 ? 1 : 2;
+  static constexpr uint32_t kHalves = HD == 256 ? 2 : 1;          // stages per K or V block
+  static constexpr uint32_t kSubs = HD == 64 ? 1 : 2;             // 64-dimension parts per stage
+  static constexpr uint32_t kStage = kSubs * kSub;
+  static constexpr uint32_t kQ = HD / 64 * kSub;                  // bytes of one lane's queries
+  static constexpr uint32_t kStages = HD == 64 ? 10 : 5;
+  static constexpr uint32_t kSoftmaxWarps = 4 * kLanes;
+  static constexpr uint32_t kThreads = (kSoftmaxWarps + 4) * 32;
+  static constexpr uint32_t kRows = kLanes * kLaneRows;           // rows per unit
+  static constexpr uint32_t kRing = kLanes * kQ;                  // offset of the stages
+  static constexpr uint32_t kBars = kRing + kStages * kStage;     // offset of the barriers
+  static constexpr uint32_t kSmem = kBars + 512 + 1024;           // + alignment of the base
+  static constexpr uint32_t kRecord = kLaneRows * (HD + 2);       // floats of a lane's record
+};
+
+constexpr uint32_t kTmemO = 256;  // tensor-memory column of O (S buffers at 0 and 128)
+
+// One unit and its place in the list.
+struct Unit {
+  uint32_t b, kv, tile;
+  uint32_t first_row, rows, tiles, slot;  // of the sequence: its rows are count * group
+  int32_t past;                           // position of the sequence's first new token
+  uint32_t firsts, skip, seen, blocks;
+};
+
+template <int HD>
+__device__ __forceinline__ void load_sequence(const AttendParams& p, uint32_t b, Unit& u, uint32_t* err) {
+  const uint32_t count = new_rows(p, b, u.first_row, err);
+  u.b = b;
+  u.rows = count * p.group;
+  u.tiles = (u.rows + Shape<HD>::kRows - 1u) / Shape<HD>::kRows;
+  if (count) {
+    const Sequence s = sequence(p.c, b, err);
+    u.slot = s.slot;
+    u.past = static_cast<int32_t>(s.length) - static_cast<int32_t>(count);
+  }
+}
+// Last visible position + 1, numbered without the gap, of rows up to R.
+__device__ __forceinline__ uint32_t seen_by(const AttendParams& p, const Unit& u, uint32_t R) {
+  const int32_t t = u.past + static_cast<int32_t>(R / p.group);
+  return t < 0 ? 0u : static_cast<uint32_t>(t) + 1u - u.skip;
+}
+__device__ __forceinline__ uint32_t blocks_of(uint32_t seen) { return seen ? (seen + kKeys - 1u) / kKeys : 1u; }
+template <int HD>
+__device__ __forceinline__ void set_tile(const AttendParams& p, Unit& u, uint32_t tile) {
+  u.tile = tile;
+  const uint32_t R0 = tile * Shape<HD>::kRows, R1 = min(R0 + Shape<HD>::kRows, u.rows);
+  const int32_t t0 = u.past + static_cast<int32_t>(R0 / p.group);
+  const uint32_t low = p.window && t0 >= 0 && static_cast<uint32_t>(t0) >= p.window ? t0 - p.window + 1u : 0u;
+  u.firsts = min(p.sinks, low);
+  u.skip = low - u.firsts;
+  u.seen = seen_by(p, u, R1 - 1u);
+  u.blocks = blocks_of(u.seen);
+}
+template <int HD>
+__device__ __forceinline__ void next_unit(const AttendParams& p, Unit& u) {
+  if (u.tile + 1u < u.tiles) {
+    set_tile<HD>(p, u, u.tile + 1u);
+    return;
+  }
+  if (++u.kv == p.c.kv_heads) {
+    u.kv = 0;
+    do load_sequence<HD>(p, u.b + 1u, u, nullptr);
+    while (u.tiles == 0u);
+  }
+  set_tile<HD>(p, u, 0u);
+}
+// Blocks of all tiles of a sequence (one K/V head), by the whole warp: a lane
+// adds a short sequence's itself, the warp shares a long one's.
+template <int HD>
+__device__ uint64_t sequence_blocks(const AttendParams& p, Unit u) {
+  uint64_t sum = 0;
+  if (u.tiles <= 4u)
+    for (uint32_t i = 0; i < u.tiles; ++i) {
+      set_tile<HD>(p, u, i);
+      sum += u.blocks;
+    }
+  uint32_t longs = __ballot_sync(0xffffffffu, u.tiles > 4u);
+  while (longs) {
+    const int from = __ffs(longs) - 1;
+    longs &= longs - 1u;
+    Unit v = u;
+    v.rows = __shfl_sync(0xffffffffu, u.rows, from);
+    v.tiles = __shfl_sync(0xffffffffu, u.tiles, from);
+    v.past = __shfl_sync(0xffffffffu, u.past, from);
+    uint64_t part = 0;
+    for (uint32_t i = threadIdx.x & 31u; i < v.tiles; i += 32u) {
+      set_tile<HD>(p, v, i);
+      part += v.blocks;
+    }
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
+    if (static_cast<int>(threadIdx.x & 31u) == from) sum = part;
+  }
+  return sum;
+}
+
+// ---- tcgen05 ----------------------------------------------------------------
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+#define RTA_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
+#define RTA_W8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
+__device__ __forceinline__ void tc_ld32(uint32_t addr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : RTA_R8(v, 0), RTA_R8(v, 8), RTA_R8(v, 16), RTA_R8(v, 24)
+      : "r"(addr));
+}
+// Waits for this thread's loads; the 32 registers pass through it, so nothing
+// that uses them can be moved ahead.
+#define RTA_X8(v, o) "+r"(v[o]), "+r"(v[o + 1]), "+r"(v[o + 2]), "+r"(v[o + 3]), "+r"(v[o + 4]), "+r"(v[o + 5]), "+r"(v[o + 6]), "+r"(v[o + 7])
+__device__ __forceinline__ void tc_wait_ld(uint32_t* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : RTA_X8(v, 0), RTA_X8(v, 8), RTA_X8(v, 16), RTA_X8(v, 24)::"memory");
+}
+#undef RTA_X8
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      RTA_W8(v, 0), RTA_W8(v, 8)
+      : "memory");
+}
+__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      RTA_W8(v, 0), RTA_W8(v, 8), RTA_W8(v, 16), RTA_W8(v, 24)
+      : "memory");
+}
+#undef RTA_R8
+#undef RTA_W8
+
+// Shared-memory matrix descriptor, 128-byte swizzle, 8-row groups 1024 bytes
+// apart; `lbo` is the distance of 64-element parts of an MN-major operand (a
+// K-major one does not use it).
+__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3fffu) | static_cast<uint64_t>(lbo >> 4) << 16 |
+         static_cast<uint64_t>(1024u >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+// kind::f16: fp32 D, M = 128; `mn` marks B as MN-major (V: dimensions run fastest)
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t idesc(uint32_t n, bool mn) {
+  const uint32_t t = Num<T>::kBf16 ? 1u : 0u;
+  return 1u << 4 | t << 7 | t << 10 | (mn ? 1u << 16 : 0u) | (n >> 3) << 17 | (128u >> 4) << 24;
+}
+// Issued by a whole warp in uniform control flow; one elected lane issues.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\telect.sync r|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\telect.sync r|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(add)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t.reg .b32 r;\n\telect.sync r|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Bounded wait of a whole warp; false (for all its lanes) ends the role.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t* err, volatile uint32_t* stop) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const bool ok = *stop == 0u && mbar_wait(bar, parity, err);
+  return __all_sync(0xffffffffu, ok);
+}
+
+template <typename T>
+struct Slack {
+  // weights stay below 2^(slack + shift): fp16 ends at 2^16
+  static constexpr float value = Num<T>::kBf16 ? 8.f : 5.f;
+};
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(128, 1) prefill_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const AttendParams p) {
+  using S = Shape<HD>;
   using N = Num<T>;
-  constexpr uint32_t kRow = HD * 2, kChunks = kRow / 16, kSteps = HD / 16;
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t scan_part[4];
-  __shared__ uint32_t found_b, found_tile;
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t4 = lane & 3u;
-  const uint32_t kv = blockIdx.y;
-  if (threadIdx.x == 0) found_b = 0xffffffffu;
-  uint64_t base = 0;
-  for (uint32_t b0 = 0; b0 < p.c.batch; b0 += 128u) {
-    const uint32_t b = b0 + threadIdx.x;
-    uint64_t mine = 0, sum;
-    uint32_t first;
-    if (b < p.c.batch)
-      mine = (static_cast<uint64_t>(new_rows(p, b, first, blockIdx.x + blockIdx.y == 0u ? p.err : nullptr)) * p.group + kRows - 1u) / kRows;
-    const uint64_t upto = base + block_scan(mine, scan_part, sum);
-    if (mine && blockIdx.x < upto && blockIdx.x >= upto - mine) {
-      found_b = b;
-      found_tile = static_cast<uint32_t>(blockIdx.x - (upto - mine));
-    }
-    base += sum;
-  }
-  __syncthreads();
-  const uint32_t b = found_b;
-  if (b == 0xffffffffu) return;
-  uint32_t first_row;
-  const uint32_t count = new_rows(p, b, first_row, nullptr);
-  const Sequence seq = sequence(p.c, b, blockIdx.y == 0u ? p.err : nullptr);
-  const int64_t past = static_cast<int64_t>(seq.length) - count;  // position of row 0 of the sequence
-  const uint32_t R0 = found_tile * kRows, R1 = min(R0 + kRows, count * p.group);
-  const int64_t t0 = past + R0 / p.group, t1 = past + (R1 - 1u) / p.group;  // positions of the tile's queries
-  const uint32_t ta = t0 > 0 ? static_cast<uint32_t>(t0) : 0u;
-  const uint32_t low = p.window && ta >= p.window ? ta - p.window + 1u : 0u;
-  const uint32_t firsts = min(p.sinks, low), skip = low - firsts;
-  const uint32_t seen = t1 < 0 ? 0u : static_cast<uint32_t>(t1) + 1u - skip;
+  constexpr uint32_t kLanes = S::kLanes, kStages = S::kStages, kHalves = S::kHalves;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t scan_part[S::kThreads / 32];
+  __shared__ uint64_t found_at;
+  __shared__ uint32_t found_b, found_kv, found_tile, tmem_base, stop_word, last_word[2];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~uintptr_t{1023});
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
+  uint64_t* const full = bars;                 // [stages] producers -> MMA
+  uint64_t* const empty = bars + 10;           // [stages] MMA -> producers
+  uint64_t* const q_full = bars + 20;          // [lane] softmax -> MMA
+  uint64_t* const s_full = bars + 22;          // [S buffer] MMA -> softmax
+  uint64_t* const p_full = bars + 24;          // [S buffer] softmax -> MMA
+  uint64_t* const o_done = bars + 26;          // [lane] MMA -> softmax
+  uint64_t* const wrote = bars + 28;           // [lane] records written
+  uint64_t* const judged = bars + 30;          // [lane] who joins is known
+  uint64_t* const drain = bars + 32;
+  volatile uint32_t* const stop = &stop_word;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
-  int64_t t_row[2];
-  uint32_t at_row[2], head_row[2];
-  bool real[2];
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const uint32_t R = R0 + warp * 16u + g + 8u * r;
-    real[r] = R < R1;
-    t_row[r] = real[r] ? past + R / p.group : -1;
-    at_row[r] = first_row + (real[r] ? R / p.group : 0u);
-    head_row[r] = kv * p.group + R % p.group;
-  }
-  uint32_t qa[kSteps][4];
-#pragma unroll
-  for (uint32_t kk = 0; kk < kSteps; ++kk)
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        qa[kk][2 * h + r] = real[r] ? *reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + at_row[r] * p.q_row + head_row[r] * p.q_head + kk * 16u + h * 8u + 2u * t4) : 0u;
-  float o[HD / 8][4];
-#pragma unroll
-  for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, z[2] = {0.f, 0.f};
-  const uint32_t ks = smem_u32(smem), vs = ks + kKeys * kRow;
-  for (uint32_t u0 = 0; u0 < seen; u0 += kKeys) {
-    for (uint32_t i = threadIdx.x; i < kKeys * kChunks; i += 128u) {
-      const uint32_t r = i / kChunks, c = i % kChunks, u = u0 + r;
-      uint64_t off = 0;
-      bool ok = false;
-      if (u < seen) {
-        ok = locate(p.c, seq.slot, u < firsts ? u : u + skip, off);
-        if (!ok) atomicOr(p.err, RTA_DEVERR_PAGE);
-        off += kv * p.c.head_bytes + c * 16u;
-      }
-      const uint32_t dst = r * kRow + ((c ^ (r & 7u)) << 4);
-      cp_async16(ks + dst, p.c.k + off, ok);
-      cp_async16(vs + dst, p.c.v + off, ok);
+  if (threadIdx.x == 0) {
+    for (uint32_t i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 3);
+      mbar_init(&empty[i], 1);
     }
-    cp_commit();
-    cp_wait<0>();
-    __syncthreads();
-    float sc[kKeys / 8][4];
-#pragma unroll
-    for (int n = 0; n < static_cast<int>(kKeys / 8); ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-#pragma unroll
-    for (uint32_t kk = 0; kk < kSteps; ++kk)
-#pragma unroll
-      for (uint32_t n = 0; n < kKeys / 16; ++n) {
-        uint32_t f[4];
-        const uint32_t r = n * 16u + (lane & 7u) + ((lane >> 4) << 3), c = 2u * kk + ((lane >> 3) & 1u);
-        ldsm4(ks + r * kRow + ((c ^ (r & 7u)) << 4), f);
-        N::mma(sc[2 * n], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], f[0], f[1]);
-        N::mma(sc[2 * n + 1], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], f[2], f[3]);
+    for (uint32_t i = 0; i < 2u; ++i) {
+      mbar_init(&q_full[i], 4);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_done[i], 1);
+      mbar_init(&wrote[i], 4);
+      mbar_init(&judged[i], 1);
+    }
+    mbar_init(drain, 1);
+    fence_mbar_init();
+    stop_word = 0u;
+  }
+
+  // ---- the list of blocks and this CTA's range ------------------------------
+  uint64_t total = 0;
+  for (uint32_t b0 = 0; b0 < p.c.batch; b0 += S::kThreads) {
+    const uint32_t b = b0 + threadIdx.x;
+    Unit u;
+    u.tiles = 0;
+    if (b < p.c.batch) load_sequence<HD>(p, b, u, blockIdx.x == 0u ? p.err : nullptr);
+    uint64_t sum;
+    block_scan(sequence_blocks<HD>(p, u) * p.c.kv_heads, scan_part, sum);
+    total += sum;
+  }
+  if (total == 0u) return;
+  const uint64_t want = (total + 1u) / 2u;  // at least two blocks per CTA
+  const uint64_t ctas = want < gridDim.x ? want : gridDim.x;
+  if (blockIdx.x >= ctas) return;
+  const uint64_t begin = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1u) / ctas;
+  {
+    uint64_t base = 0;
+    for (uint32_t b0 = 0; b0 < p.c.batch; b0 += S::kThreads) {
+      const uint32_t b = b0 + threadIdx.x;
+      Unit u;
+      u.tiles = 0;
+      if (b < p.c.batch) load_sequence<HD>(p, b, u, nullptr);
+      uint64_t sum;
+      const uint64_t mine = sequence_blocks<HD>(p, u) * p.c.kv_heads;
+      const uint64_t upto = base + block_scan(mine, scan_part, sum);
+      if (mine && begin < upto && begin >= upto - mine) {
+        found_b = b;
+        found_at = begin - (upto - mine);
       }
-    float scale[2];
+      base += sum;
+      if (begin < base) break;
+    }
+    __syncthreads();
+  }
+  Unit first;
+  load_sequence<HD>(p, found_b, first, nullptr);
+  first.kv = 0;
+  if (warp == 0) {
+    // the K/V head, then the tile whose blocks hold the offset
+    uint64_t off = found_at;
+    const Unit all = first;
+    uint64_t per_kv = 0;
+    for (uint32_t i0 = 0; i0 < first.tiles; i0 += 32u) {
+      Unit v = all;
+      uint64_t n = 0;
+      if (i0 + lane < first.tiles) {
+        set_tile<HD>(p, v, i0 + lane);
+        n = v.blocks;
+      }
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float mx = -INFINITY;
+      for (int d = 16; d >= 1; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
+      per_kv += n;
+    }
+    const uint32_t kv = static_cast<uint32_t>(off / per_kv);
+    off -= kv * per_kv;
+    for (uint32_t i0 = 0; i0 < first.tiles; i0 += 32u) {
+      Unit v = all;
+      uint64_t n = 0;
+      if (i0 + lane < first.tiles) {
+        set_tile<HD>(p, v, i0 + lane);
+        n = v.blocks;
+      }
+      uint64_t upto = n;
 #pragma unroll
-      for (int n = 0; n < static_cast<int>(kKeys / 8); ++n)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const uint32_t u = u0 + n * 8u + 2u * t4 + x;
-          const int64_t at = u < firsts ? u : static_cast<int64_t>(u) + skip;
-          float& s = sc[n][2 * r + x];
-          s *= p.scale_log2;
-          const bool see = u < seen && at <= t_row[r] && (!p.window || at > t_row[r] - p.window || at < p.sinks);
-          if (!see) s = -INFINITY;
-          mx = fmaxf(mx, s);
+      for (int d = 1; d < 32; d <<= 1) {
+        const uint64_t o = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= static_cast<uint32_t>(d)) upto += o;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, off < upto);
+      if (hit) {
+        const int at = __ffs(hit) - 1;
+        const uint64_t before = __shfl_sync(0xffffffffu, upto - n, at);
+        if (lane == 0) {
+          found_tile = i0 + at;
+          found_at = off - before;
+          found_kv = kv;
         }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mn = fmaxf(m[r], mx), bs = mn == -INFINITY ? 0.f : mn;
-      scale[r] = m[r] == mn ? 1.f : exp2f(m[r] - bs);
-      float sum = 0.f;
-#pragma unroll
-      for (int n = 0; n < static_cast<int>(kKeys / 8); ++n)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) sum += sc[n][2 * r + x] = exp2f(sc[n][2 * r + x] - (bs - N::kShift));
-      z[r] = z[r] * scale[r] + sum;
-      m[r] = mn;
-    }
-#pragma unroll
-    for (int j = 0; j < HD / 8; ++j) {
-      o[j][0] *= scale[0];
-      o[j][1] *= scale[0];
-      o[j][2] *= scale[1];
-      o[j][3] *= scale[1];
-    }
-#pragma unroll
-    for (uint32_t n = 0; n < kKeys / 16; ++n) {
-      const uint32_t a0 = N::pack(sc[2 * n][0], sc[2 * n][1]), a1 = N::pack(sc[2 * n][2], sc[2 * n][3]);
-      const uint32_t a2 = N::pack(sc[2 * n + 1][0], sc[2 * n + 1][1]), a3 = N::pack(sc[2 * n + 1][2], sc[2 * n + 1][3]);
-#pragma unroll
-      for (uint32_t j = 0; j < HD / 8u; j += 2u) {
-        uint32_t f[4];
-        const uint32_t r = n * 16u + (lane & 7u) + (((lane >> 3) & 1u) << 3), c = j + (lane >> 4);
-        ldsm4_t(vs + r * kRow + ((c ^ (r & 7u)) << 4), f);
-        N::mma(o[j], a0, a1, a2, a3, f[0], f[1]);
-        N::mma(o[j + 1], a0, a1, a2, a3, f[2], f[3]);
+        break;
       }
+      off -= __shfl_sync(0xffffffffu, upto, 31);
     }
-    __syncthreads();
   }
-  uint32_t again[2];
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    z[r] += __shfl_xor_sync(0xffffffffu, z[r], 1);
-    z[r] += __shfl_xor_sync(0xffffffffu, z[r], 2);
-    const float inv = t_row[r] < 0 ? 0.f : 1.f / z[r];
-    bool bad = false;
-    const size_t at = static_cast<size_t>(at_row[r]) * p.heads + head_row[r];
-#pragma unroll
-    for (int j = 0; j < HD / 8; ++j) {
-      const float x = t_row[r] < 0 ? 0.f : o[j][2 * r] * inv, y = t_row[r] < 0 ? 0.f : o[j][2 * r + 1] * inv;
-      bad |= !isfinite(x) || !isfinite(y);
-      if (real[r]) *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + at * HD + j * 8 + 2u * t4) = N::pack(x, y);
-    }
-    if (real[r] && p.lse && t4 == 0u) p.lse[at] = t_row[r] < 0 ? -INFINITY : (m[r] - N::kShift + log2f(z[r])) * kLn2;
-    again[r] = __ballot_sync(0xffffffffu, bad && real[r]);
+  if (warp == kLanes * 4u) {  // the MMA warp
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_base))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = tmem_base;
+  first.kv = found_kv;
+  set_tile<HD>(p, first, found_tile);
+  const uint32_t first_a = static_cast<uint32_t>(found_at);
+  const auto lane_rows = [&](const Unit& u, uint32_t L) {
+    const uint32_t at = u.tile * S::kRows + L * kLaneRows;
+    return u.rows > at ? min(kLaneRows, u.rows - at) : 0u;
+  };
+  // blocks of lane L of a segment that takes blocks [a, e) of the unit
+  const auto lane_blocks = [&](const Unit& u, uint32_t L, uint32_t a, uint32_t e) {
+    const uint32_t rows = lane_rows(u, L);
+    if (rows == 0u) return 0u;
+    const uint32_t n = min(e, blocks_of(seen_by(p, u, u.tile * S::kRows + L * kLaneRows + rows - 1u)));
+    return n > a ? n - a : 0u;
+  };
+
+  if (warp < S::kSoftmaxWarps) {
+    // ---------------------------------------------------------------- softmax
+    const uint32_t L = warp >> 2, quarter = warp & 3u, r = quarter * 32u + lane;
+    const uint32_t lane_addr = quarter * 32u << 16, tmem_o = tmem + lane_addr + kTmemO + L * HD;
+    const uint32_t q_smem = smem_u32(smem) + L * S::kQ;
+    const float scale = p.scale_log2 == 0.f ? 1e-30f : fabsf(p.scale_log2);  // 0: all weights equal
+    const bool negative = p.scale_log2 < 0.f;
+    uint32_t it = 0, segments = 0;  // blocks of this lane, cut segments so far
+    bool ok = true, first_segment = true;
+    Unit u = first;
+    uint32_t a = first_a;
+    for (uint64_t g = begin; g < end && ok;) {
+      const uint32_t e = static_cast<uint32_t>(min(static_cast<uint64_t>(u.blocks), a + (end - g)));
+      const uint32_t rows = lane_rows(u, L), n = lane_blocks(u, L, a, e);
+      const uint32_t R = u.tile * S::kRows + L * kLaneRows + r;
+      const bool real = r < rows;
+      const uint32_t i = real ? R / p.group : 0u, head = u.kv * p.group + (real ? R % p.group : 0u);
+      const int32_t t = real ? u.past + static_cast<int32_t>(i) : -1;
+      const uint32_t row = u.first_row + i;
+      if (n) {  // the queries: a row at a time, 16 bytes per lane
+        constexpr uint32_t kChunks = HD / 8, kPer = 32 / kChunks;
+        const uint64_t off = (row * p.q_row + head * p.q_head) * 2u;
+#pragma unroll 4
+        for (uint32_t x0 = 0; x0 < 32u; x0 += kPer) {
+          const uint32_t x = x0 + lane / kChunks, c = lane % kChunks, y = quarter * 32u + x;
+          const uint64_t o = __shfl_sync(0xffffffffu, off, x);
+          const bool on = __shfl_sync(0xffffffffu, real ? 1 : 0, x) != 0;
+          cp_async16(q_smem + (c >> 3) * kSub + y * 128u + (((c & 7u) ^ (y & 7u)) << 4),
+                     static_cast<const uint8_t*>(p.q) + o + c * 16u, on);
+        }
+        cp_commit();
+        cp_wait<0>();
+        fence_async();
+        __syncwarp();
+        if (lane == 0) arrive(&q_full[L]);
+      }
+      // visible u of this row: u < s_hi or w_lo <= u < w_hi
+      const uint32_t w_hi = t < 0 ? 0u : static_cast<uint32_t>(t) + 1u - u.skip;
+      const uint32_t w_lo = p.window && t >= 0 && static_cast<uint32_t>(t) >= p.window ? t - p.window + 1u - u.skip : 0u;
+      const uint32_t s_hi = min(p.sinks, w_hi);
+      // blocks that every row of the lane sees whole: [clear_lo, clear_hi) in u
+      const int32_t t_first = u.past + static_cast<int32_t>((u.tile * S::kRows + L * kLaneRows) / p.group);
+      const int32_t t_last = rows ? u.past + static_cast<int32_t>((u.tile * S::kRows + L * kLaneRows + rows - 1u) / p.group) : -1;
+      const uint32_t clear_hi = t_first < 0 ? 0u : static_cast<uint32_t>(t_first) + 1u - u.skip;
+      const uint32_t clear_lo = p.window && t_last >= 0 && static_cast<uint32_t>(t_last) >= p.window ? t_last - p.window + 1u - u.skip : 0u;
+      float m = -INFINITY, z = 0.f;
+      for (uint32_t j = 0; j < n; ++j, ++it) {
+        const uint32_t sb = kLanes == 2 ? L : it & 1u;
+        const uint32_t tmem_s = tmem + lane_addr + sb * 128u;
+        if (!(ok = warp_wait(&s_full[sb], kLanes == 2 ? it & 1u : it >> 1 & 1u, p.err, stop))) break;
+        tc_after();
+        const uint32_t u0 = (a + j) * kKeys;
+        const bool masked = u0 < clear_lo || u0 + kKeys > clear_hi;
+        const int32_t sh = static_cast<int32_t>(s_hi) - static_cast<int32_t>(u0);
+        const int32_t lo = static_cast<int32_t>(w_lo) - static_cast<int32_t>(u0), hi = static_cast<int32_t>(w_hi) - static_cast<int32_t>(u0);
+        // 32 columns of S, masked; read twice, for the maximum and for the weights, so that a row takes 64 registers
+        const auto take = [&](uint32_t (&s)[32], uint32_t c0) {
+          if (negative) {
 #pragma unroll
-  for (int r = 0; r < 2; ++r)
-    for (uint32_t x = 0; x < 8u; ++x) {
-      if (!(again[r] >> (4u * x) & 15u)) continue;
-      const uint32_t R = R0 + warp * 16u + x + 8u * r;
-      const uint32_t t = static_cast<uint32_t>(past + R / p.group);
-      if (spoiled<T, HD>(p, seq.slot, kv, low, static_cast<uint32_t>(t1) + 1u, t))
-        row_alone<T, HD>(p, seq.slot, kv, kv * p.group + R % p.group, first_row + R / p.group, t);
+            for (int c = 0; c < 32; ++c) s[c] ^= 0x80000000u;
+          }
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              const int32_t x = static_cast<int32_t>(c0) + c;
+              if (!(x < sh || (x >= lo && x < hi))) s[c] = 0xff800000u;
+            }
+          }
+        };
+        uint32_t s[2][32];
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        tc_ld32(tmem_s, s[0]);
+#pragma unroll
+        for (uint32_t c = 0; c < 4u; ++c) {
+          tc_wait_ld(s[c & 1u]);
+          tc_ld32(tmem_s + (c + 1u) % 4u * 32u, s[(c + 1u) & 1u]);  // the last one: the first 32 again
+          take(s[c & 1u], c * 32u);
+#pragma unroll
+          for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[c & 1u][x]));
+        }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+        const bool rise = top > m + Slack<T>::value;
+        float factor = 1.f;
+        if (rise) {
+          factor = ex2(m - top);  // m = -inf: 0
+          m = top;
+        }
+        const float base = (m == -INFINITY ? 0.f : m) - N::kShift;
+        z *= factor;
+        float zs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (uint32_t c = 0; c < 4u; ++c) {
+          tc_wait_ld(s[c & 1u]);
+          if (c < 3u) tc_ld32(tmem_s + (c + 1u) * 32u, s[(c + 1u) & 1u]);
+          uint32_t(&v)[32] = s[c & 1u];
+          take(v, c * 32u);
+          uint32_t w[16];
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            const float w0 = ex2(fmaf(__uint_as_float(v[2 * x]), scale, -base)), w1 = ex2(fmaf(__uint_as_float(v[2 * x + 1]), scale, -base));
+            zs[x & 3] += w0 + w1;
+            w[x] = N::pack(w0, w1);
+          }
+          // the weights take the place of scores that have been read: columns 16 c .. of 32 c + 31
+          tc_st16(tmem_s + c * 16u, w);
+        }
+        z += (zs[0] + zs[1]) + (zs[2] + zs[3]);
+        if (j) {
+          // O holds the blocks before this one
+          if (!(ok = warp_wait(&o_done[L], (it - 1u) & 1u, p.err, stop))) break;
+          if (__any_sync(0xffffffffu, rise)) {
+            tc_after();
+#pragma unroll 1
+            for (uint32_t c = 0; c < HD; c += 32u) {
+              uint32_t o[32];
+              tc_ld32(tmem_o + c, o);
+              tc_wait_ld(o);
+#pragma unroll
+              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * factor);
+              tc_st32(tmem_o + c, o);
+            }
+          }
+        }
+        tc_wait_st();
+        tc_before();
+        __syncwarp();
+        if (lane == 0) arrive(&p_full[sb]);
+      }
+      if (!ok) break;
+      if (n) {
+        if (!(ok = warp_wait(&o_done[L], (it - 1u) & 1u, p.err, stop))) break;
+        tc_after();
+      }
+      const uint64_t unit0 = g - a, unit1 = unit0 + u.blocks;
+      const bool whole = a == 0u && e == u.blocks;
+      const size_t at = static_cast<size_t>(row) * p.heads + head;
+      T* const out = static_cast<T*>(p.out) + at * HD;
+      bool bad = false;
+      bool mine = whole;  // this CTA writes the lane's results
+      if (whole && rows) {
+        const float inv = 1.f / z;
+#pragma unroll 1
+        for (uint32_t c = 0; c < HD; c += 32u) {
+          uint32_t o[32];
+          tc_ld32(tmem_o + c, o);
+          tc_wait_ld(o);
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            const float f0 = t < 0 ? 0.f : __uint_as_float(o[2 * x]) * inv, f1 = t < 0 ? 0.f : __uint_as_float(o[2 * x + 1]) * inv;
+            bad |= !isfinite(f0) || !isfinite(f1);
+            o[x] = N::pack(f0, f1);
+          }
+          if (real)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              *reinterpret_cast<uint4*>(out + c + 8 * x) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+        }
+        if (real && p.lse) p.lse[at] = t < 0 ? -INFINITY : (m - N::kShift + log2f(z)) * kLn2;
+      } else if (rows) {
+        const auto owner = [&](uint64_t x) { return static_cast<uint32_t>(((x + 1u) * ctas - 1u) / total); };
+        const auto record = [&](uint32_t c, bool second) {
+          return p.records + (static_cast<size_t>(c * 2u + (second ? 1u : 0u)) * kLanes + L) * S::kRecord;
+        };
+        float* const rec = record(blockIdx.x, !first_segment);
+        rec[r] = m;
+        rec[kLaneRows + r] = z;
+        float4* const rec_o = reinterpret_cast<float4*>(rec + 2 * kLaneRows);
+        if (n) {
+#pragma unroll 1
+          for (uint32_t c = 0; c < HD; c += 32u) {
+            uint32_t o[32];
+            tc_ld32(tmem_o + c, o);
+            tc_wait_ld(o);
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              rec_o[(c / 4u + x) * kLaneRows + r] = make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]),
+                                                                __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
+          }
+        }
+        // ---- join: the CTA that arrives last ----------------------------------
+        const uint32_t c0 = owner(unit0), parts = owner(unit1 - 1u) - c0 + 1u;
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) arrive(&wrote[L]);
+        if (!(ok = warp_wait(&wrote[L], segments & 1u, p.err, stop))) break;
+        if (r == 0u) {
+          uint32_t* const counter = &p.counters[c0 * 2u + L];
+          const uint32_t was = atomicAdd(counter, 1u);
+          if (was == parts - 1u) *counter = 0u;
+          last_word[L] = was == parts - 1u ? 1u : 0u;
+          arrive(&judged[L]);
+        }
+        __syncwarp();
+        if (!(ok = warp_wait(&judged[L], segments & 1u, p.err, stop))) break;
+        ++segments;
+        mine = *const_cast<volatile uint32_t*>(&last_word[L]) != 0u;
+        if (mine) {
+          __threadfence();
+          const bool second0 = total * c0 / ctas != unit0;  // c0's record is its second when the unit begins inside its range
+          float mm = -INFINITY, zz = 0.f;
+          for (uint32_t j = 0; j < parts; ++j) mm = fmaxf(mm, __ldcg(record(c0 + j, j == 0u && second0) + r));
+          const float mb = mm == -INFINITY ? 0.f : mm;
+          for (uint32_t j = 0; j < parts; ++j) {
+            const float* x = record(c0 + j, j == 0u && second0);
+            const float f = ex2(__ldcg(x + r) - mb);
+            if (f != 0.f) zz += f * __ldcg(x + kLaneRows + r);
+          }
+          const float inv = 1.f / zz;
+#pragma unroll 1
+          for (uint32_t c = 0; c < HD; c += 32u) {
+            float4 o[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (uint32_t j = 0; j < parts; ++j) {
+              const float* y = record(c0 + j, j == 0u && second0);
+              const float f = ex2(__ldcg(y + r) - mb) * inv;
+              const float4* yo = reinterpret_cast<const float4*>(y + 2 * kLaneRows) + (c / 4u) * kLaneRows + r;
+              if (f != 0.f) {
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                  const float4 v = __ldcg(yo + x * kLaneRows);
+                  o[x].x += f * v.x;
+                  o[x].y += f * v.y;
+                  o[x].z += f * v.z;
+                  o[x].w += f * v.w;
+                }
+              }
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const float4 f0 = o[2 * x], f1 = o[2 * x + 1];
+              bad |= !isfinite(f0.x) || !isfinite(f0.y) || !isfinite(f0.z) || !isfinite(f0.w) || !isfinite(f1.x) ||
+                     !isfinite(f1.y) || !isfinite(f1.z) || !isfinite(f1.w);
+              uint4 w = make_uint4(N::pack(f0.x, f0.y), N::pack(f0.z, f0.w), N::pack(f1.x, f1.y), N::pack(f1.z, f1.w));
+              if (t < 0) w = make_uint4(0u, 0u, 0u, 0u);
+              if (real) *reinterpret_cast<uint4*>(out + c + 8 * x) = w;
+            }
+          }
+          if (real && p.lse) p.lse[at] = t < 0 ? -INFINITY : (mm - N::kShift + log2f(zz)) * kLn2;
+        }
+      }
+      uint32_t again = __ballot_sync(0xffffffffu, mine && bad && real && t >= 0);
+      while (again) {  // see row_alone
+        const int x = __ffs(again) - 1;
+        again &= again - 1u;
+        const uint32_t tx = __shfl_sync(0xffffffffu, t, x), hx = __shfl_sync(0xffffffffu, head, x), rx = __shfl_sync(0xffffffffu, row, x);
+        if (spoiled<T, HD>(p, u.slot, u.kv, u.firsts + u.skip, u.seen + u.skip, tx)) row_alone<T, HD>(p, u.slot, u.kv, hx, rx, tx);
+      }
+      first_segment = false;
+      g += e - a;
+      a = 0;
+      if (g < end) next_unit<HD>(p, u);
     }
+    if (!ok) *stop = 1u;
+  } else if (warp == S::kSoftmaxWarps) {
+    // -------------------------------------------------------------------- MMA
+    const uint32_t q0 = smem_u32(smem), ring = q0 + S::kRing;
+    uint32_t st = 0, it[2] = {0, 0}, segs[2] = {0, 0};  // stages consumed, blocks and segments of each lane
+    bool ok = true;
+    Unit u = first;
+    uint32_t a = first_a;
+    const auto wait_stage = [&](uint32_t x) { return warp_wait(&full[x % kStages], x / kStages & 1u, p.err, stop); };
+    // S (+)= Q K^T over the dimensions of one stage
+    const auto qk = [&](uint32_t L, uint32_t sbuf, uint32_t x, uint32_t half) {
+      const uint32_t qa = q0 + L * S::kQ + half * 2u * kSub, kb = ring + x % kStages * S::kStage;
+#pragma unroll
+      for (uint32_t k = 0; k < S::kSubs * 4u; ++k)
+        mma_ss(tmem + sbuf * 128u, desc(qa + (k >> 2) * kSub + (k & 3u) * 32u, 16u), desc(kb + (k >> 2) * kSub + (k & 3u) * 32u, 16u),
+               idesc<T>(kKeys, false), half || k ? 1u : 0u);
+    };
+    // O[dimensions of one stage] (+)= w V
+    const auto pv = [&](uint32_t L, uint32_t sbuf, uint32_t x, uint32_t half, bool fresh) {
+      const uint32_t vb = ring + x % kStages * S::kStage;
+#pragma unroll
+      for (uint32_t k = 0; k < kKeys / 16u; ++k)
+        mma_ts(tmem + kTmemO + L * HD + half * 128u, tmem + sbuf * 128u + k * 8u, desc(vb + k * 2048u, kSub),
+               idesc<T>(S::kSubs * 64u, true), fresh && k == 0u ? 0u : 1u);
+    };
+    for (uint64_t g = begin; g < end && ok;) {
+      const uint32_t e = static_cast<uint32_t>(min(static_cast<uint64_t>(u.blocks), a + (end - g)));
+      const uint32_t n = e - a;
+      uint32_t ln[2];
+      ln[0] = lane_blocks(u, 0, a, e);
+      ln[1] = kLanes == 2 ? lane_blocks(u, 1, a, e) : 0u;
+#pragma unroll
+      for (uint32_t L = 0; L < kLanes; ++L)
+        if (ok && ln[L]) ok = warp_wait(&q_full[L], segs[L]++ & 1u, p.err, stop);
+      if (!ok) break;
+      if constexpr (kLanes == 2) {
+        if (!(ok = wait_stage(st))) break;
+        tc_after();
+#pragma unroll
+        for (uint32_t L = 0; L < 2u; ++L)
+          if (ln[L]) {
+            qk(L, L, st, 0);
+            commit(&s_full[L]);
+          }
+        commit(&empty[st % kStages]);
+        ++st;
+        for (uint32_t j = 0; j < n && ok; ++j) {
+          const bool more = j + 1u < n;
+          const uint32_t kst = st, vst = st + (more ? 1u : 0u);
+          if (!(ok = (!more || wait_stage(kst)) && wait_stage(vst))) break;
+#pragma unroll
+          for (uint32_t L = 0; L < 2u; ++L)
+            if (ok && j < ln[L]) {
+              if (!(ok = warp_wait(&p_full[L], it[L] & 1u, p.err, stop))) break;
+              tc_after();
+              pv(L, L, vst, 0, j == 0u);
+              commit(&o_done[L]);
+              ++it[L];
+              if (j + 1u < ln[L]) {
+                qk(L, L, kst, 0);
+                commit(&s_full[L]);
+              }
+            }
+          if (!ok) break;
+          if (more) commit(&empty[kst % kStages]);
+          commit(&empty[vst % kStages]);
+          st = vst + 1u;
+        }
+      } else {
+        for (uint32_t h = 0; h < kHalves && ok; ++h) {
+          if (!(ok = wait_stage(st))) break;
+          tc_after();
+          qk(0, it[0] & 1u, st, h);
+          commit(&empty[st++ % kStages]);
+        }
+        if (!ok) break;
+        commit(&s_full[it[0] & 1u]);
+        for (uint32_t j = 0; j < n && ok; ++j, ++it[0]) {
+          const uint32_t sb = it[0] & 1u;
+          if (j + 1u < n) {
+            for (uint32_t h = 0; h < kHalves && ok; ++h) {
+              if (!(ok = wait_stage(st))) break;
+              tc_after();
+              qk(0, sb ^ 1u, st, h);
+              commit(&empty[st++ % kStages]);
+            }
+            if (!ok) break;
+            commit(&s_full[sb ^ 1u]);
+          }
+          if (!(ok = warp_wait(&p_full[sb], it[0] >> 1 & 1u, p.err, stop))) break;
+          for (uint32_t h = 0; h < kHalves && ok; ++h) {
+            if (!(ok = wait_stage(st))) break;
+            tc_after();
+            pv(0, sb, st, h, j == 0u);
+            commit(&empty[st++ % kStages]);
+          }
+          if (!ok) break;
+          commit(&o_done[0]);
+        }
+      }
+      g += n;
+      a = 0;
+      if (g < end) next_unit<HD>(p, u);
+    }
+    if (!ok) *stop = 1u;
+    commit(drain);  // every MMA issued above has completed once this arrives
+    (void)mbar_wait(drain, 0u, nullptr);
+    __syncwarp();
+  } else {
+    // -------------------------------------------------------------- producers
+    constexpr uint32_t kOwn = 44;  // rows of a stage per warp: 44, 44, 40
+    const uint32_t w = warp - S::kSoftmaxWarps - 1u, row0 = w * kOwn, mine = min(kOwn, kKeys - row0);
+    const uint32_t ring = smem_u32(smem) + S::kRing;
+    uint32_t st = 0, told = 0;  // stages issued, and made known to the MMA warp
+    bool ok = true;
+    Unit u = first;
+    uint32_t a = first_a;
+    const auto tell = [&]() {
+      fence_async();
+      __syncwarp();
+      if (lane == 0) arrive(&full[told % kStages]);
+      ++told;
+    };
+    // page of position `block * 128 + row0 + lane + 32 x`, -1 where nothing is visible
+    const auto look = [&](uint32_t block, uint32_t x) -> int32_t {
+      const uint32_t l = lane + 32u * x, at = block * kKeys + row0 + l;
+      if (l >= mine || at >= u.seen) return -1;
+      const uint32_t pos = at < u.firsts ? at : at + u.skip;
+      const int32_t page = p.c.table[static_cast<size_t>(u.slot) * p.c.width + page_of(p.c, pos)];
+      if (static_cast<uint32_t>(page) < p.c.pages) return page;
+      atomicOr(p.err, RTA_DEVERR_PAGE);
+      return -1;
+    };
+    const auto resolve = [&](uint32_t block, uint32_t x, int32_t page) -> uint64_t {
+      if (page < 0) return ~0ull;
+      const uint32_t at = block * kKeys + row0 + lane + 32u * x, pos = at < u.firsts ? at : at + u.skip;
+      return static_cast<uint64_t>(page) * p.c.page_bytes + static_cast<uint64_t>(pos - page_of(p.c, pos) * p.c.page_size) * p.c.pos_bytes +
+             static_cast<uint64_t>(u.kv) * p.c.head_bytes;
+    };
+    // one stage: dimensions [128 half, ..) of a block's K or V rows
+    const auto copy = [&](const uint8_t* base, uint64_t off0, uint64_t off1, uint32_t half) {
+      const uint32_t s = st % kStages, par = (st / kStages & 1u) ^ 1u;
+      if (!__all_sync(0xffffffffu, mbar_try_wait(&empty[s], par))) {
+        cp_wait<0>();  // nothing may wait for copies that have landed while this warp waits
+        while (told < st) tell();
+        if (!(ok = warp_wait(&empty[s], par, p.err, stop))) return;
+      }
+      const uint32_t dst = ring + s * S::kStage, c = lane & 7u;
+#pragma unroll
+      for (uint32_t x = 0; x < kOwn / 4u; ++x) {
+        const uint32_t l = x * 4u + (lane >> 3);
+        const uint64_t o = x < 8u ? __shfl_sync(0xffffffffu, off0, l) : __shfl_sync(0xffffffffu, off1, l - 32u);
+        const uint32_t row = row0 + l;
+        if (l < mine) {
+          const uint8_t* src = base + (o == ~0ull ? 0ull : o) + half * 256u + c * 16u;
+          const uint32_t to = dst + row * 128u + ((c ^ (row & 7u)) << 4);
+#pragma unroll
+          for (uint32_t y = 0; y < S::kSubs; ++y) cp_async16(to + y * kSub, src + y * 128u, o != ~0ull);
+        }
+      }
+      cp_commit();
+      ++st;
+      if (st - told > 2u) {
+        cp_wait<2>();
+        tell();
+      }
+    };
+    for (uint64_t g = begin; g < end && ok;) {
+      const uint32_t e = static_cast<uint32_t>(min(static_cast<uint64_t>(u.blocks), a + (end - g)));
+      uint64_t k0 = resolve(a, 0, look(a, 0)), k1 = resolve(a, 1, look(a, 1));
+      int32_t n0 = look(a + 1u, 0), n1 = look(a + 1u, 1);
+      for (uint32_t h = 0; h < kHalves && ok; ++h) copy(p.c.k, k0, k1, h);
+      for (uint32_t j = a; j < e && ok; ++j) {
+        const uint64_t v0 = k0, v1 = k1;
+        if (j + 1u < e) {
+          k0 = resolve(j + 1u, 0, n0);
+          k1 = resolve(j + 1u, 1, n1);
+          n0 = look(j + 2u, 0);
+          n1 = look(j + 2u, 1);
+          for (uint32_t h = 0; h < kHalves && ok; ++h) copy(p.c.k, k0, k1, h);
+        }
+        for (uint32_t h = 0; h < kHalves && ok; ++h) copy(p.c.v, v0, v1, h);
+      }
+      g += e - a;
+      a = 0;
+      if (g < end) next_unit<HD>(p, u);
+    }
+    cp_wait<0>();
+    if (ok)
+      while (told < st) tell();
+    else
+      *stop = 1u;
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  if (warp == S::kSoftmaxWarps)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 template <typename T, int HD>
 cudaError_t launch(const AttendParams& p, cudaStream_t s) {
-  constexpr uint32_t smem = 2 * kKeys * HD * 2;
-  const uint64_t tiles = (static_cast<uint64_t>(p.rows) * p.group + kRows - 1u) / kRows + p.c.batch;
-  prefill_kernel<T, HD><<<dim3(static_cast<uint32_t>(tiles), p.c.kv_heads), 128, smem, s>>>(p);
+  static std::atomic<int> sms_of[64];
+  static std::mutex m;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  int sms = sms_of[dev].load(std::memory_order_acquire);
+  if (sms <= 0) {
+    std::lock_guard<std::mutex> lock(m);
+    e = cudaFuncSetAttribute(prefill_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(Shape<HD>::kSmem));
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return e;
+    if (sms <= 0) return cudaErrorInvalidDevice;
+    sms_of[dev].store(sms, std::memory_order_release);
+  }
+  const uint32_t ctas = static_cast<uint32_t>(sms) < kMaxCtas ? static_cast<uint32_t>(sms) : kMaxCtas;
+  prefill_kernel<T, HD><<<ctas, Shape<HD>::kThreads, Shape<HD>::kSmem, s>>>(p);
   return cudaGetLastError();
 }
 template <typename T>
@@ -205,7 +869,10 @@ cudaError_t by_dim(const AttendParams& p, cudaStream_t s) {
 
 }  // namespace
 
-size_t prefill_record_bytes() { return static_cast<size_t>(kMaxCtas) * 2u * 256u * (128u + 2u) * 4u; }
+size_t prefill_record_bytes() {
+  const size_t one = Shape<256>::kRecord, two = 2 * Shape<128>::kRecord;
+  return static_cast<size_t>(kMaxCtas) * 2u * (one > two ? one : two) * 4u;
+}
 
 cudaError_t launch_prefill(const AttendParams& p, int fmt, cudaStream_t s) {
   return fmt == kF16 ? by_dim<__half>(p, s) : by_dim<__nv_bfloat16>(p, s);
