@@ -163,12 +163,6 @@ __device__ __forceinline__ void tc_wait_ld(uint32_t* v) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : RTA_X8(v, 0), RTA_X8(v, 8), RTA_X8(v, 16), RTA_X8(v, 24)::"memory");
 }
 #undef RTA_X8
-__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
-      RTA_W8(v, 0), RTA_W8(v, 8)
-      : "memory");
-}
 __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* v) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
@@ -192,19 +186,34 @@ __device__ __forceinline__ constexpr uint32_t idesc(uint32_t n, bool mn) {
   const uint32_t t = Num<T>::kBf16 ? 1u : 0u;
   return 1u << 4 | t << 7 | t << 10 | (mn ? 1u << 16 : 0u) | (n >> 3) << 17 | (128u >> 4) << 24;
 }
-// Issued by a whole warp in uniform control flow; one elected lane issues.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t add) {
+// Four k steps, issued by a whole warp in uniform control flow under one
+// election.  The first of them overwrites D when `add` is 0.
+template <uint32_t ASTEP, uint32_t BSTEP>  // in descriptor units (16 bytes)
+__device__ __forceinline__ void mma_ss4(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t add) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\telect.sync r|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(add)
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+      "add.u64 a1, %1, %5;\n\tadd.u64 a2, a1, %5;\n\tadd.u64 a3, a2, %5;\n\t"
+      "add.u64 b1, %2, %6;\n\tadd.u64 b2, b1, %6;\n\tadd.u64 b3, b2, %6;\n\t"
+      "elect.sync r|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, 1;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, 1;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, 1;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(add), "n"(ASTEP), "n"(BSTEP)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t add) {
+template <uint32_t ASTEP, uint32_t BSTEP>  // tensor-memory columns; descriptor units
+__device__ __forceinline__ void mma_ts4(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t add) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\telect.sync r|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(id), "r"(add)
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 r, a1, a2, a3;\n\t.reg .b64 b1, b2, b3;\n\t"
+      "add.u32 a1, %1, %5;\n\tadd.u32 a2, a1, %5;\n\tadd.u32 a3, a2, %5;\n\t"
+      "add.u64 b1, %2, %6;\n\tadd.u64 b2, b1, %6;\n\tadd.u64 b3, b2, %6;\n\t"
+      "elect.sync r|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, 1;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, 1;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, 1;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(add), "n"(ASTEP), "n"(BSTEP)
       : "memory");
 }
 __device__ __forceinline__ void commit(uint64_t* bar) {
@@ -222,11 +231,35 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// (x, y) = (x, y) * a + b and (x, y) += (a, b), two at a time
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b) {
+  asm("{\n\t.reg .b64 v, s, t;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 s, {%2, %2};\n\tmov.b64 t, {%3, %3};\n\t"
+      "fma.rn.f32x2 v, v, s, t;\n\tmov.b64 {%0, %1}, v;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
+  asm("{\n\t.reg .b64 v, s;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 s, {%2, %3};\n\tadd.rn.f32x2 v, v, s;\n\t"
+      "mov.b64 {%0, %1}, v;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
 // Bounded wait of a whole warp; false (for all its lanes) ends the role.
+// Inline to the end: a kernel that moves registers between its warps cannot
+// call functions.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t* err, volatile uint32_t* stop) {
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-  const bool ok = *stop == 0u && mbar_wait(bar, parity, err);
-  return __all_sync(0xffffffffu, ok);
+  const uint64_t start = globaltimer();
+  for (uint32_t spin = 1;; ++spin) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((spin & 63u) == 0u) {
+      const bool late = globaltimer() - start > RTA_WAIT_NS;
+      if (__any_sync(0xffffffffu, late || *stop != 0u)) {
+        if (late && err) atomicOr(err, RTA_DEVERR_TIMEOUT);
+        return false;
+      }
+    }
+  }
 }
 
 template <typename T>
@@ -243,7 +276,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t scan_part[S::kThreads / 32];
   __shared__ uint64_t found_at;
-  __shared__ uint32_t found_b, found_kv, found_tile, tmem_base, stop_word, last_word[2];
+  __shared__ uint32_t found_b, found_kv, found_tile, tmem_base, stop_word, never, last_word[2];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~uintptr_t{1023});
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
   uint64_t* const full = bars;                 // [stages] producers -> MMA
@@ -273,7 +306,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     }
     mbar_init(drain, 1);
     fence_mbar_init();
-    stop_word = 0u;
+    stop_word = never = 0u;
   }
 
   // ---- the list of blocks and this CTA's range ------------------------------
@@ -385,11 +418,13 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
 
   if (warp < S::kSoftmaxWarps) {
     // ---------------------------------------------------------------- softmax
+    // 2 x 128 x 208 + 128 x 80 registers of the launch's 384 x 168
+    if constexpr (kLanes == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const uint32_t L = warp >> 2, quarter = warp & 3u, r = quarter * 32u + lane;
     const uint32_t lane_addr = quarter * 32u << 16, tmem_o = tmem + lane_addr + kTmemO + L * HD;
     const uint32_t q_smem = smem_u32(smem) + L * S::kQ;
-    const float scale = p.scale_log2 == 0.f ? 1e-30f : fabsf(p.scale_log2);  // 0: all weights equal
-    const bool negative = p.scale_log2 < 0.f;
+    // 0: all weights equal; a negative one: the MMA negates the queries
+    const float scale = p.scale_log2 == 0.f ? 1e-30f : fabsf(p.scale_log2);
     uint32_t it = 0, segments = 0;  // blocks of this lane, cut segments so far
     bool ok = true, first_segment = true;
     Unit u = first;
@@ -438,58 +473,65 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
         const bool masked = u0 < clear_lo || u0 + kKeys > clear_hi;
         const int32_t sh = static_cast<int32_t>(s_hi) - static_cast<int32_t>(u0);
         const int32_t lo = static_cast<int32_t>(w_lo) - static_cast<int32_t>(u0), hi = static_cast<int32_t>(w_hi) - static_cast<int32_t>(u0);
-        // 32 columns of S, masked; read twice, for the maximum and for the weights, so that a row takes 64 registers
-        const auto take = [&](uint32_t (&s)[32], uint32_t c0) {
-          if (negative) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) s[c] ^= 0x80000000u;
-          }
+        uint32_t s[2][32], w[64];
+        const auto mask = [&](uint32_t (&v)[32], int32_t c0) {
           if (masked) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              const int32_t x = static_cast<int32_t>(c0) + c;
-              if (!(x < sh || (x >= lo && x < hi))) s[c] = 0xff800000u;
-            }
+            for (int c = 0; c < 32; ++c)
+              if (!(c0 + c < sh || (c0 + c >= lo && c0 + c < hi))) v[c] = 0xff800000u;
           }
         };
-        uint32_t s[2][32];
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        tc_ld32(tmem_s, s[0]);
+        const auto largest = [&](const uint32_t (&v)[32], float (&mx)[4]) {
 #pragma unroll
-        for (uint32_t c = 0; c < 4u; ++c) {
-          tc_wait_ld(s[c & 1u]);
-          tc_ld32(tmem_s + (c + 1u) % 4u * 32u, s[(c + 1u) & 1u]);  // the last one: the first 32 again
-          take(s[c & 1u], c * 32u);
+          for (int c = 0; c < 32; c += 2)
+            mx[c >> 1 & 3] = fmaxf(fmaxf(mx[c >> 1 & 3], __uint_as_float(v[c])), __uint_as_float(v[c + 1]));
+        };
+        float before = m, sum;
+        if (j == 0u) {  // the first block's maximum; later ones rarely exceed m by the slack
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          tc_ld32(tmem_s, s[0]);
 #pragma unroll
-          for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[c & 1u][x]));
-        }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-        const bool rise = top > m + Slack<T>::value;
-        float factor = 1.f;
-        if (rise) {
-          factor = ex2(m - top);  // m = -inf: 0
-          m = top;
-        }
-        const float base = (m == -INFINITY ? 0.f : m) - N::kShift;
-        z *= factor;
-        float zs[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (uint32_t c = 0; c < 4u; ++c) {
-          tc_wait_ld(s[c & 1u]);
-          if (c < 3u) tc_ld32(tmem_s + (c + 1u) * 32u, s[(c + 1u) & 1u]);
-          uint32_t(&v)[32] = s[c & 1u];
-          take(v, c * 32u);
-          uint32_t w[16];
-#pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            const float w0 = ex2(fmaf(__uint_as_float(v[2 * x]), scale, -base)), w1 = ex2(fmaf(__uint_as_float(v[2 * x + 1]), scale, -base));
-            zs[x & 3] += w0 + w1;
-            w[x] = N::pack(w0, w1);
+          for (uint32_t c = 0; c < 4u; ++c) {
+            tc_wait_ld(s[c & 1u]);
+            if (c < 3u) tc_ld32(tmem_s + (c + 1u) * 32u, s[(c + 1u) & 1u]);
+            mask(s[c & 1u], c * 32);
+            largest(s[c & 1u], mx);
           }
-          // the weights take the place of scores that have been read: columns 16 c .. of 32 c + 31
-          tc_st16(tmem_s + c * 16u, w);
+          m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
         }
-        z += (zs[0] + zs[1]) + (zs[2] + zs[3]);
+        while (true) {
+          const float base = N::kShift - (m == -INFINITY ? 0.f : m);
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float zs[4][2] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+          tc_ld32(tmem_s, s[0]);
+#pragma unroll
+          for (uint32_t c = 0; c < 4u; ++c) {
+            tc_wait_ld(s[c & 1u]);
+            if (c < 3u) tc_ld32(tmem_s + (c + 1u) * 32u, s[(c + 1u) & 1u]);
+            uint32_t(&v)[32] = s[c & 1u];
+            mask(v, c * 32);
+            largest(v, mx);
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              float w0 = __uint_as_float(v[2 * x]), w1 = __uint_as_float(v[2 * x + 1]);
+              fma2(w0, w1, scale, base);
+              w0 = ex2(w0);
+              w1 = ex2(w1);
+              add2(zs[x & 3][0], zs[x & 3][1], w0, w1);
+              w[c * 16u + x] = N::pack(w0, w1);
+            }
+          }
+          sum = ((zs[0][0] + zs[0][1]) + (zs[1][0] + zs[1][1])) + ((zs[2][0] + zs[2][1]) + (zs[3][0] + zs[3][1]));
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+          const bool rise = top > m + Slack<T>::value;
+          if (!__any_sync(0xffffffffu, rise)) break;
+          if (rise) m = top;  // and again, with the new maximum
+        }
+        const bool rise = m != before;
+        const float factor = rise ? ex2(before - m) : 1.f;  // before = -inf: 0
+        z = z * factor + sum;
+        tc_st32(tmem_s, w);  // the weights take the place of the scores
+        tc_st32(tmem_s + 32, w + 32);
         if (j) {
           // O holds the blocks before this one
           if (!(ok = warp_wait(&o_done[L], (it - 1u) & 1u, p.err, stop))) break;
@@ -639,27 +681,29 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     if (!ok) *stop = 1u;
   } else if (warp == S::kSoftmaxWarps) {
     // -------------------------------------------------------------------- MMA
+    if constexpr (kLanes == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     const uint32_t q0 = smem_u32(smem), ring = q0 + S::kRing;
     uint32_t st = 0, it[2] = {0, 0}, segs[2] = {0, 0};  // stages consumed, blocks and segments of each lane
     bool ok = true;
     Unit u = first;
     uint32_t a = first_a;
     const auto wait_stage = [&](uint32_t x) { return warp_wait(&full[x % kStages], x / kStages & 1u, p.err, stop); };
+    const uint64_t high = desc(0u, 16u), high_v = desc(0u, kSub);
+    const uint32_t id_s = idesc<T>(kKeys, false) | (p.scale_log2 < 0.f ? 1u << 13 : 0u);
     // S (+)= Q K^T over the dimensions of one stage
     const auto qk = [&](uint32_t L, uint32_t sbuf, uint32_t x, uint32_t half) {
       const uint32_t qa = q0 + L * S::kQ + half * 2u * kSub, kb = ring + x % kStages * S::kStage;
-#pragma unroll
-      for (uint32_t k = 0; k < S::kSubs * 4u; ++k)
-        mma_ss(tmem + sbuf * 128u, desc(qa + (k >> 2) * kSub + (k & 3u) * 32u, 16u), desc(kb + (k >> 2) * kSub + (k & 3u) * 32u, 16u),
-               idesc<T>(kKeys, false), half || k ? 1u : 0u);
+#pragma unroll 1
+      for (uint32_t k = 0; k < S::kSubs; ++k)
+        mma_ss4<2, 2>(tmem + sbuf * 128u, high + ((qa + k * kSub) >> 4), high + ((kb + k * kSub) >> 4), id_s, half + k);
     };
     // O[dimensions of one stage] (+)= w V
     const auto pv = [&](uint32_t L, uint32_t sbuf, uint32_t x, uint32_t half, bool fresh) {
       const uint32_t vb = ring + x % kStages * S::kStage;
-#pragma unroll
-      for (uint32_t k = 0; k < kKeys / 16u; ++k)
-        mma_ts(tmem + kTmemO + L * HD + half * 128u, tmem + sbuf * 128u + k * 8u, desc(vb + k * 2048u, kSub),
-               idesc<T>(S::kSubs * 64u, true), fresh && k == 0u ? 0u : 1u);
+#pragma unroll 1
+      for (uint32_t k = 0; k < kKeys / 16u; k += 4u)
+        mma_ts4<8, 128>(tmem + kTmemO + L * HD + half * 128u, tmem + sbuf * 128u + k * 8u, high_v + ((vb + k * 2048u) >> 4),
+                        idesc<T>(S::kSubs * 64u, true), fresh && k == 0u ? 0u : 1u);
     };
     for (uint64_t g = begin; g < end && ok;) {
       const uint32_t e = static_cast<uint32_t>(min(static_cast<uint64_t>(u.blocks), a + (end - g)));
@@ -742,10 +786,11 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     }
     if (!ok) *stop = 1u;
     commit(drain);  // every MMA issued above has completed once this arrives
-    (void)mbar_wait(drain, 0u, nullptr);
+    (void)warp_wait(drain, 0u, nullptr, &never);
     __syncwarp();
   } else {
     // -------------------------------------------------------------- producers
+    if constexpr (kLanes == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     constexpr uint32_t kOwn = 44;  // rows of a stage per warp: 44, 44, 40
     const uint32_t w = warp - S::kSoftmaxWarps - 1u, row0 = w * kOwn, mine = min(kOwn, kKeys - row0);
     const uint32_t ring = smem_u32(smem) + S::kRing;
