@@ -39,9 +39,11 @@ struct AttendParams {
   void* out;
   float* lse;
   uint32_t* err;
-  uint32_t* counters;  // [kMaxCtas][2], zero between calls
+  uint32_t* counters;  // [kMaxCtas], zero between calls
+  void* cuts;  // [kMaxCtas] units that are cut, of kCutBytes each
   float* records;
 };
+constexpr uint32_t kCutBytes = 64;
 
 // q: the queries' format (kF32, kF16 or kBF16); fmt: the pool's.
 cudaError_t launch_decode(const AttendParams& p, int fmt, int q, cudaStream_t s);

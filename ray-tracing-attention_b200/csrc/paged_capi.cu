@@ -40,9 +40,11 @@ const char* bad_map(const rta_page_pool* p, const rta_page_map* m) {
   return nullptr;
 }
 
-// Workspace: error word and padding, the counters of split units, then either
-// the split records of an attention call or the plan of a bookkeeping call.
-constexpr size_t kErr = 256, kCounters = (paged::kMaxCtas * 8u + 255u) / 256u * 256u, kBody = kErr + kCounters;
+// Workspace: error word and padding, the counters and descriptions of split
+// units, then either the split records of an attention call or the plan of a
+// bookkeeping call.
+constexpr size_t kErr = 256, kCounters = (paged::kMaxCtas * 4u + 255u) / 256u * 256u,
+                 kCuts = (paged::kMaxCtas * paged::kCutBytes + 255u) / 256u * 256u, kBody = kErr + kCounters + kCuts;
 size_t workspace_bytes_of(const rta_page_pool* p, const rta_page_map* m) {
   size_t body = paged::decode_record_bytes();
   if (paged::prefill_record_bytes() > body) body = paged::prefill_record_bytes();
@@ -83,10 +85,11 @@ paged::View view(const rta_page_pool* p, const rta_page_map* m, uint32_t layer, 
 
 struct Workspace {
   uint32_t *err, *counters;
-  void* body;
+  void *cuts, *body;
   explicit Workspace(void* ws)
       : err(static_cast<uint32_t*>(ws)),
         counters(reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(ws) + kErr)),
+        cuts(static_cast<uint8_t*>(ws) + kErr + kCounters),
         body(static_cast<uint8_t*>(ws) + kBody) {}
 };
 
@@ -125,6 +128,7 @@ const char* attend_params(const rta_page_pool* pool, const rta_page_map* map, ui
   p.lse = lse;
   p.err = w.err;
   p.counters = w.counters;
+  p.cuts = w.cuts;
   p.records = static_cast<float*>(w.body);
   p.starts = nullptr;
   p.rows = batch;

@@ -18,7 +18,7 @@
 //
 // Work: the blocks of all units form one list, cut evenly over the CTAs (one
 // per SM) whatever the lengths are; a lane of a unit that is cut leaves a
-// record (m, z, O) per CTA and the CTA that arrives last joins them in order.
+// record (m, z, O) per CTA, which a second launch joins in order, many CTAs to a unit.
 //
 // Roles (all waits bounded):
 //   softmax    four warps per lane, a thread per row: load Q, take S from
@@ -61,6 +61,16 @@ struct Shape {
 };
 
 constexpr uint32_t kTmemO = 256;  // tensor-memory column of O (S buffers at 0 and 128)
+
+// A unit that begins in a CTA's range and ends in another's: at most one per CTA.
+struct Cut {
+  uint32_t parts;   // CTAs that hold a part of it, from this one on; 0: no such unit
+  uint32_t second;  // this CTA's record of it is its second (the others': their first)
+  uint32_t first_row, R0, rows, kv, slot;
+  int32_t past;
+  uint32_t low, high;
+};
+__device__ __forceinline__ Cut* p_cuts(const AttendParams& p) { return static_cast<Cut*>(p.cuts); }
 
 // One unit and its place in the list.
 struct Unit {
@@ -276,7 +286,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t scan_part[S::kThreads / 32];
   __shared__ uint64_t found_at;
-  __shared__ uint32_t found_b, found_kv, found_tile, tmem_base, stop_word, never, last_word[2];
+  __shared__ uint32_t found_b, found_kv, found_tile, tmem_base, stop_word, never;
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~uintptr_t{1023});
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
   uint64_t* const full = bars;                 // [stages] producers -> MMA
@@ -285,9 +295,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
   uint64_t* const s_full = bars + 22;          // [S buffer] MMA -> softmax
   uint64_t* const p_full = bars + 24;          // [S buffer] softmax -> MMA
   uint64_t* const o_done = bars + 26;          // [lane] MMA -> softmax
-  uint64_t* const wrote = bars + 28;           // [lane] records written
-  uint64_t* const judged = bars + 30;          // [lane] who joins is known
-  uint64_t* const drain = bars + 32;
+  uint64_t* const drain = bars + 28;
   volatile uint32_t* const stop = &stop_word;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
@@ -301,13 +309,14 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
       mbar_init(&o_done[i], 1);
-      mbar_init(&wrote[i], 4);
-      mbar_init(&judged[i], 1);
     }
     mbar_init(drain, 1);
     fence_mbar_init();
     stop_word = never = 0u;
   }
+
+  pdl_launch_dependents();  // the joining launch waits for this grid's end by itself
+  if (threadIdx.x == 0) p_cuts(p)[blockIdx.x].parts = 0u;
 
   // ---- the list of blocks and this CTA's range ------------------------------
   uint64_t total = 0;
@@ -425,10 +434,31 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     const uint32_t q_smem = smem_u32(smem) + L * S::kQ;
     // 0: all weights equal; a negative one: the MMA negates the queries
     const float scale = p.scale_log2 == 0.f ? 1e-30f : fabsf(p.scale_log2);
-    uint32_t it = 0, segments = 0;  // blocks of this lane, cut segments so far
+    uint32_t it = 0;  // blocks of this lane
     bool ok = true, first_segment = true;
     Unit u = first;
     uint32_t a = first_a;
+    // the queries of a lane, a row at a time, 16 bytes per thread
+    const auto load_queries = [&](const Unit& v) {
+      constexpr uint32_t kChunks = HD / 8, kPer = 32 / kChunks;
+      const uint32_t R = v.tile * S::kRows + L * kLaneRows + r;
+      const bool real = r < lane_rows(v, L);
+      const uint64_t off = real ? ((v.first_row + R / p.group) * p.q_row + (v.kv * p.group + R % p.group) * p.q_head) * 2u : 0u;
+#pragma unroll 4
+      for (uint32_t x0 = 0; x0 < 32u; x0 += kPer) {
+        const uint32_t x = x0 + lane / kChunks, c = lane % kChunks, y = quarter * 32u + x;
+        const uint64_t o = __shfl_sync(0xffffffffu, off, x);
+        const bool on = __shfl_sync(0xffffffffu, real ? 1 : 0, x) != 0;
+        cp_async16(q_smem + (c >> 3) * kSub + y * 128u + (((c & 7u) ^ (y & 7u)) << 4),
+                   static_cast<const uint8_t*>(p.q) + o + c * 16u, on);
+      }
+      cp_commit();
+      cp_wait<0>();
+      fence_async();
+      __syncwarp();
+      if (lane == 0) arrive(&q_full[L]);
+    };
+    if (lane_blocks(u, L, a, static_cast<uint32_t>(min(static_cast<uint64_t>(u.blocks), a + (end - begin))))) load_queries(u);
     for (uint64_t g = begin; g < end && ok;) {
       const uint32_t e = static_cast<uint32_t>(min(static_cast<uint64_t>(u.blocks), a + (end - g)));
       const uint32_t rows = lane_rows(u, L), n = lane_blocks(u, L, a, e);
@@ -437,23 +467,6 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
       const uint32_t i = real ? R / p.group : 0u, head = u.kv * p.group + (real ? R % p.group : 0u);
       const int32_t t = real ? u.past + static_cast<int32_t>(i) : -1;
       const uint32_t row = u.first_row + i;
-      if (n) {  // the queries: a row at a time, 16 bytes per lane
-        constexpr uint32_t kChunks = HD / 8, kPer = 32 / kChunks;
-        const uint64_t off = (row * p.q_row + head * p.q_head) * 2u;
-#pragma unroll 4
-        for (uint32_t x0 = 0; x0 < 32u; x0 += kPer) {
-          const uint32_t x = x0 + lane / kChunks, c = lane % kChunks, y = quarter * 32u + x;
-          const uint64_t o = __shfl_sync(0xffffffffu, off, x);
-          const bool on = __shfl_sync(0xffffffffu, real ? 1 : 0, x) != 0;
-          cp_async16(q_smem + (c >> 3) * kSub + y * 128u + (((c & 7u) ^ (y & 7u)) << 4),
-                     static_cast<const uint8_t*>(p.q) + o + c * 16u, on);
-        }
-        cp_commit();
-        cp_wait<0>();
-        fence_async();
-        __syncwarp();
-        if (lane == 0) arrive(&q_full[L]);
-      }
       // visible u of this row: u < s_hi or w_lo <= u < w_hi
       const uint32_t w_hi = t < 0 ? 0u : static_cast<uint32_t>(t) + 1u - u.skip;
       const uint32_t w_lo = p.window && t >= 0 && static_cast<uint32_t>(t) >= p.window ? t - p.window + 1u - u.skip : 0u;
@@ -554,17 +567,24 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
         if (lane == 0) arrive(&p_full[sb]);
       }
       if (!ok) break;
+      // Every S of this unit has been computed, so its queries are done with:
+      // the next unit's take their place, and its first S is computed while
+      // this one's results are written.
+      Unit next = u;
+      const uint64_t g_next = g + (e - a);
+      if (g_next < end) {
+        next_unit<HD>(p, next);
+        if (lane_blocks(next, L, 0u, static_cast<uint32_t>(min(static_cast<uint64_t>(next.blocks), end - g_next)))) load_queries(next);
+      }
       if (n) {
         if (!(ok = warp_wait(&o_done[L], (it - 1u) & 1u, p.err, stop))) break;
         tc_after();
       }
-      const uint64_t unit0 = g - a, unit1 = unit0 + u.blocks;
       const bool whole = a == 0u && e == u.blocks;
-      const size_t at = static_cast<size_t>(row) * p.heads + head;
-      T* const out = static_cast<T*>(p.out) + at * HD;
       bool bad = false;
-      bool mine = whole;  // this CTA writes the lane's results
       if (whole && rows) {
+        const size_t at = static_cast<size_t>(row) * p.heads + head;
+        T* const out = static_cast<T*>(p.out) + at * HD;
         const float inv = 1.f / z;
 #pragma unroll 1
         for (uint32_t c = 0; c < HD; c += 32u) {
@@ -584,11 +604,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
         }
         if (real && p.lse) p.lse[at] = t < 0 ? -INFINITY : (m - N::kShift + log2f(z)) * kLn2;
       } else if (rows) {
-        const auto owner = [&](uint64_t x) { return static_cast<uint32_t>(((x + 1u) * ctas - 1u) / total); };
-        const auto record = [&](uint32_t c, bool second) {
-          return p.records + (static_cast<size_t>(c * 2u + (second ? 1u : 0u)) * kLanes + L) * S::kRecord;
-        };
-        float* const rec = record(blockIdx.x, !first_segment);
+        float* const rec = p.records + (static_cast<size_t>(blockIdx.x * 2u + (first_segment ? 0u : 1u)) * kLanes + L) * S::kRecord;
         rec[r] = m;
         rec[kLaneRows + r] = z;
         float4* const rec_o = reinterpret_cast<float4*>(rec + 2 * kLaneRows);
@@ -604,69 +620,21 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
                                                                 __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
           }
         }
-        // ---- join: the CTA that arrives last ----------------------------------
-        const uint32_t c0 = owner(unit0), parts = owner(unit1 - 1u) - c0 + 1u;
-        __threadfence();
-        __syncwarp();
-        if (lane == 0) arrive(&wrote[L]);
-        if (!(ok = warp_wait(&wrote[L], segments & 1u, p.err, stop))) break;
-        if (r == 0u) {
-          uint32_t* const counter = &p.counters[c0 * 2u + L];
-          const uint32_t was = atomicAdd(counter, 1u);
-          if (was == parts - 1u) *counter = 0u;
-          last_word[L] = was == parts - 1u ? 1u : 0u;
-          arrive(&judged[L]);
-        }
-        __syncwarp();
-        if (!(ok = warp_wait(&judged[L], segments & 1u, p.err, stop))) break;
-        ++segments;
-        mine = *const_cast<volatile uint32_t*>(&last_word[L]) != 0u;
-        if (mine) {
-          __threadfence();
-          const bool second0 = total * c0 / ctas != unit0;  // c0's record is its second when the unit begins inside its range
-          float mm = -INFINITY, zz = 0.f;
-          for (uint32_t j = 0; j < parts; ++j) mm = fmaxf(mm, __ldcg(record(c0 + j, j == 0u && second0) + r));
-          const float mb = mm == -INFINITY ? 0.f : mm;
-          for (uint32_t j = 0; j < parts; ++j) {
-            const float* x = record(c0 + j, j == 0u && second0);
-            const float f = ex2(__ldcg(x + r) - mb);
-            if (f != 0.f) zz += f * __ldcg(x + kLaneRows + r);
-          }
-          const float inv = 1.f / zz;
-#pragma unroll 1
-          for (uint32_t c = 0; c < HD; c += 32u) {
-            float4 o[8];
-#pragma unroll
-            for (int x = 0; x < 8; ++x) o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (uint32_t j = 0; j < parts; ++j) {
-              const float* y = record(c0 + j, j == 0u && second0);
-              const float f = ex2(__ldcg(y + r) - mb) * inv;
-              const float4* yo = reinterpret_cast<const float4*>(y + 2 * kLaneRows) + (c / 4u) * kLaneRows + r;
-              if (f != 0.f) {
-#pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                  const float4 v = __ldcg(yo + x * kLaneRows);
-                  o[x].x += f * v.x;
-                  o[x].y += f * v.y;
-                  o[x].z += f * v.z;
-                  o[x].w += f * v.w;
-                }
-              }
-            }
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const float4 f0 = o[2 * x], f1 = o[2 * x + 1];
-              bad |= !isfinite(f0.x) || !isfinite(f0.y) || !isfinite(f0.z) || !isfinite(f0.w) || !isfinite(f1.x) ||
-                     !isfinite(f1.y) || !isfinite(f1.z) || !isfinite(f1.w);
-              uint4 w = make_uint4(N::pack(f0.x, f0.y), N::pack(f0.z, f0.w), N::pack(f1.x, f1.y), N::pack(f1.z, f1.w));
-              if (t < 0) w = make_uint4(0u, 0u, 0u, 0u);
-              if (real) *reinterpret_cast<uint4*>(out + c + 8 * x) = w;
-            }
-          }
-          if (real && p.lse) p.lse[at] = t < 0 ? -INFINITY : (mm - N::kShift + log2f(zz)) * kLn2;
+        if (a == 0u && threadIdx.x == 0u) {  // this unit begins here: what the second launch has to know of it
+          Cut& cut = p_cuts(p)[blockIdx.x];
+          cut.parts = static_cast<uint32_t>(((g + u.blocks) * ctas - 1u) / total) - blockIdx.x + 1u;
+          cut.second = first_segment ? 0u : 1u;
+          cut.first_row = u.first_row;
+          cut.R0 = u.tile * S::kRows;
+          cut.rows = min(S::kRows, u.rows - cut.R0);
+          cut.kv = u.kv;
+          cut.slot = u.slot;
+          cut.past = u.past;
+          cut.low = u.firsts + u.skip;
+          cut.high = u.seen + u.skip;
         }
       }
-      uint32_t again = __ballot_sync(0xffffffffu, mine && bad && real && t >= 0);
+      uint32_t again = __ballot_sync(0xffffffffu, bad && real && t >= 0);
       while (again) {  // see row_alone
         const int x = __ffs(again) - 1;
         again &= again - 1u;
@@ -674,9 +642,9 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
         if (spoiled<T, HD>(p, u.slot, u.kv, u.firsts + u.skip, u.seen + u.skip, tx)) row_alone<T, HD>(p, u.slot, u.kv, hx, rx, tx);
       }
       first_segment = false;
-      g += e - a;
+      g = g_next;
       a = 0;
-      if (g < end) next_unit<HD>(p, u);
+      u = next;
     }
     if (!ok) *stop = 1u;
   } else if (warp == S::kSoftmaxWarps) {
@@ -804,18 +772,20 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
       if (lane == 0) arrive(&full[told % kStages]);
       ++told;
     };
-    // page of position `block * 128 + row0 + lane + 32 x`, -1 where nothing is visible
+    // Table entry of position `block * 128 + row0 + lane + 32 x`, kNone where
+    // nothing is visible; resolved to an offset a block later, when it is here.
+    constexpr int32_t kNone = INT32_MIN;
     const auto look = [&](uint32_t block, uint32_t x) -> int32_t {
       const uint32_t l = lane + 32u * x, at = block * kKeys + row0 + l;
-      if (l >= mine || at >= u.seen) return -1;
+      if (l >= mine || at >= u.seen) return kNone;
       const uint32_t pos = at < u.firsts ? at : at + u.skip;
-      const int32_t page = p.c.table[static_cast<size_t>(u.slot) * p.c.width + page_of(p.c, pos)];
-      if (static_cast<uint32_t>(page) < p.c.pages) return page;
-      atomicOr(p.err, RTA_DEVERR_PAGE);
-      return -1;
+      return p.c.table[static_cast<size_t>(u.slot) * p.c.width + page_of(p.c, pos)];
     };
     const auto resolve = [&](uint32_t block, uint32_t x, int32_t page) -> uint64_t {
-      if (page < 0) return ~0ull;
+      if (static_cast<uint32_t>(page) >= p.c.pages) {
+        if (page != kNone) atomicOr(p.err, RTA_DEVERR_PAGE);
+        return ~0ull;
+      }
       const uint32_t at = block * kKeys + row0 + lane + 32u * x, pos = at < u.firsts ? at : at + u.skip;
       return static_cast<uint64_t>(page) * p.c.page_bytes + static_cast<uint64_t>(pos - page_of(p.c, pos) * p.c.page_size) * p.c.pos_bytes +
              static_cast<uint64_t>(u.kv) * p.c.head_bytes;
@@ -881,6 +851,95 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
+// Joins the records of cut units: blockIdx.x is the CTA in whose range the unit
+// begins, blockIdx.y sixteen of its rows.  O = sum_j 2^(m_j - max m) O_j over
+// sum_j 2^(m_j - max m) z_j.
+constexpr uint32_t kJoinRows = 16;
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) prefill_join_kernel(const AttendParams p) {
+  using S = Shape<HD>;
+  using N = Num<T>;
+  __shared__ float weight[kMaxCtas][kJoinRows];
+  __shared__ uint32_t bad_rows;
+  pdl_wait();
+  const Cut cut = p_cuts(p)[blockIdx.x];
+  const uint32_t y0 = blockIdx.y * kJoinRows;  // first row within the unit
+  if (cut.parts == 0u || y0 >= cut.rows) return;
+  if (threadIdx.x == 0) bad_rows = 0u;
+  const uint32_t L = y0 / kLaneRows, r0 = y0 % kLaneRows;
+  const auto record = [&](uint32_t j) {
+    return p.records + (static_cast<size_t>((blockIdx.x + j) * 2u + (j == 0u ? cut.second : 0u)) * S::kLanes + L) * S::kRecord;
+  };
+  const auto place = [&](uint32_t y, uint32_t& row, uint32_t& head, int32_t& t) {
+    const uint32_t R = cut.R0 + y;
+    row = cut.first_row + R / p.group;
+    head = cut.kv * p.group + R % p.group;
+    t = cut.past + static_cast<int32_t>(R / p.group);
+  };
+  {  // weights: sixteen threads per row
+    const uint32_t x = threadIdx.x / 16u, k = threadIdx.x % 16u;
+    float mm = -INFINITY, zz = 0.f;
+    for (uint32_t j = k; j < cut.parts; j += 16u) mm = fmaxf(mm, record(j)[r0 + x]);
+#pragma unroll
+    for (int d = 8; d >= 1; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+    const float base = mm == -INFINITY ? 0.f : mm;
+    for (uint32_t j = k; j < cut.parts; j += 16u) {
+      const float f = ex2(record(j)[r0 + x] - base);
+      if (f != 0.f) zz += f * record(j)[kLaneRows + r0 + x];
+    }
+#pragma unroll
+    for (int d = 8; d >= 1; d >>= 1) zz += __shfl_xor_sync(0xffffffffu, zz, d);
+    const float inv = 1.f / zz;
+    for (uint32_t j = k; j < cut.parts; j += 16u) weight[j][x] = ex2(record(j)[r0 + x] - base) * inv;
+    if (p.lse && k == 0u && y0 + x < cut.rows) {
+      uint32_t row, head;
+      int32_t t;
+      place(y0 + x, row, head, t);
+      p.lse[static_cast<size_t>(row) * p.heads + head] = t < 0 ? -INFINITY : (mm - N::kShift + log2f(zz)) * kLn2;
+    }
+  }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < kJoinRows * (HD / 8); i += 256u) {
+    const uint32_t x = i % kJoinRows, d8 = i / kJoinRows;  // eight dimensions of a row
+    if (y0 + x >= cut.rows) continue;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+#pragma unroll 4
+    for (uint32_t j = 0; j < cut.parts; ++j) {
+      const float f = weight[j][x];
+      if (f == 0.f) continue;  // an empty part has no O
+      const float4* o = reinterpret_cast<const float4*>(record(j) + 2 * kLaneRows) + 2u * d8 * kLaneRows + r0 + x;
+      const float4 u = __ldcg(o), v = __ldcg(o + kLaneRows);
+      a.x += f * u.x;
+      a.y += f * u.y;
+      a.z += f * u.z;
+      a.w += f * u.w;
+      b.x += f * v.x;
+      b.y += f * v.y;
+      b.z += f * v.z;
+      b.w += f * v.w;
+    }
+    uint32_t row, head;
+    int32_t t;
+    place(y0 + x, row, head, t);
+    uint4 w = make_uint4(N::pack(a.x, a.y), N::pack(a.z, a.w), N::pack(b.x, b.y), N::pack(b.z, b.w));
+    if (t < 0)
+      w = make_uint4(0u, 0u, 0u, 0u);
+    else if (!isfinite(a.x) || !isfinite(a.y) || !isfinite(a.z) || !isfinite(a.w) || !isfinite(b.x) || !isfinite(b.y) ||
+             !isfinite(b.z) || !isfinite(b.w))
+      atomicOr(&bad_rows, 1u << x);
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (static_cast<size_t>(row) * p.heads + head) * HD + d8 * 8u) = w;
+  }
+  __syncthreads();
+  for (uint32_t x = threadIdx.x >> 5; x < kJoinRows; x += 8u) {  // see row_alone
+    if (!(bad_rows >> x & 1u)) continue;
+    uint32_t row, head;
+    int32_t t;
+    place(y0 + x, row, head, t);
+    if (spoiled<T, HD>(p, cut.slot, cut.kv, cut.low, cut.high, static_cast<uint32_t>(t)))
+      row_alone<T, HD>(p, cut.slot, cut.kv, head, row, static_cast<uint32_t>(t));
+  }
+}
+
 template <typename T, int HD>
 cudaError_t launch(const AttendParams& p, cudaStream_t s) {
   static std::atomic<int> sms_of[64];
@@ -901,7 +960,18 @@ cudaError_t launch(const AttendParams& p, cudaStream_t s) {
   }
   const uint32_t ctas = static_cast<uint32_t>(sms) < kMaxCtas ? static_cast<uint32_t>(sms) : kMaxCtas;
   prefill_kernel<T, HD><<<ctas, Shape<HD>::kThreads, Shape<HD>::kSmem, s>>>(p);
-  return cudaGetLastError();
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, Shape<HD>::kRows / kJoinRows);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, prefill_join_kernel<T, HD>, p);
 }
 template <typename T>
 cudaError_t by_dim(const AttendParams& p, cudaStream_t s) {
