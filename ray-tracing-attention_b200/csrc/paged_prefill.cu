@@ -254,6 +254,15 @@ __device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
       : "+f"(x), "+f"(y)
       : "f"(a), "f"(b));
 }
+// Whether a phase has ended, without waiting (mbar_try_wait may suspend the thread).
+__device__ __forceinline__ bool phase_ended(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0,1,0,p; }"
+               : "=r"(done)
+               : "r"(smem_u32(bar)), "r"(parity)
+               : "memory");
+  return done != 0;
+}
 // Bounded wait of a whole warp; false (for all its lanes) ends the role.
 // Inline to the end: a kernel that moves registers between its warps cannot
 // call functions.
@@ -483,17 +492,21 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
         if (!(ok = warp_wait(&s_full[sb], kLanes == 2 ? it & 1u : it >> 1 & 1u, p.err, stop))) break;
         tc_after();
         const uint32_t u0 = (a + j) * kKeys;
-        const bool masked = u0 < clear_lo || u0 + kKeys > clear_hi;
-        const int32_t sh = static_cast<int32_t>(s_hi) - static_cast<int32_t>(u0);
-        const int32_t lo = static_cast<int32_t>(w_lo) - static_cast<int32_t>(u0), hi = static_cast<int32_t>(w_hi) - static_cast<int32_t>(u0);
         uint32_t s[2][32], w[64];
-        const auto mask = [&](uint32_t (&v)[32], int32_t c0) {
-          if (masked) {
+        if (u0 < clear_lo || u0 + kKeys > clear_hi) {  // -inf where a row does not see, in place
+          const int32_t sh = static_cast<int32_t>(s_hi) - static_cast<int32_t>(u0);
+          const int32_t lo = static_cast<int32_t>(w_lo) - static_cast<int32_t>(u0), hi = static_cast<int32_t>(w_hi) - static_cast<int32_t>(u0);
+#pragma unroll 1
+          for (int32_t c0 = 0; c0 < 128; c0 += 32) {
+            tc_ld32(tmem_s + c0, s[0]);
+            tc_wait_ld(s[0]);
 #pragma unroll
             for (int c = 0; c < 32; ++c)
-              if (!(c0 + c < sh || (c0 + c >= lo && c0 + c < hi))) v[c] = 0xff800000u;
+              if (!(c0 + c < sh || (c0 + c >= lo && c0 + c < hi))) s[0][c] = 0xff800000u;
+            tc_st32(tmem_s + c0, s[0]);
           }
-        };
+          tc_wait_st();
+        }
         const auto largest = [&](const uint32_t (&v)[32], float (&mx)[4]) {
 #pragma unroll
           for (int c = 0; c < 32; c += 2)
@@ -507,7 +520,6 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
           for (uint32_t c = 0; c < 4u; ++c) {
             tc_wait_ld(s[c & 1u]);
             if (c < 3u) tc_ld32(tmem_s + (c + 1u) * 32u, s[(c + 1u) & 1u]);
-            mask(s[c & 1u], c * 32);
             largest(s[c & 1u], mx);
           }
           m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
@@ -522,7 +534,6 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
             tc_wait_ld(s[c & 1u]);
             if (c < 3u) tc_ld32(tmem_s + (c + 1u) * 32u, s[(c + 1u) & 1u]);
             uint32_t(&v)[32] = s[c & 1u];
-            mask(v, c * 32);
             largest(v, mx);
 #pragma unroll
             for (int x = 0; x < 16; ++x) {
@@ -793,8 +804,8 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     // one stage: dimensions [128 half, ..) of a block's K or V rows
     const auto copy = [&](const uint8_t* base, uint64_t off0, uint64_t off1, uint32_t half) {
       const uint32_t s = st % kStages, par = (st / kStages & 1u) ^ 1u;
-      if (!__all_sync(0xffffffffu, mbar_try_wait(&empty[s], par))) {
-        cp_wait<0>();  // nothing may wait for copies that have landed while this warp waits
+      if (!__all_sync(0xffffffffu, phase_ended(&empty[s], par))) {
+        cp_wait<0>();  // the MMA warp must know of every stage issued while this warp waits
         while (told < st) tell();
         if (!(ok = warp_wait(&empty[s], par, p.err, stop))) return;
       }
