@@ -109,6 +109,10 @@ __device__ __forceinline__ void set_tile(const AttendParams& p, Unit& u, uint32_
   u.seen = seen_by(p, u, R1 - 1u);
   u.blocks = blocks_of(u.seen);
 }
+// What a unit costs: its blocks, and about as much as kEntry of them to fill
+// and to empty the pipeline (a segment of the list that holds only a unit's
+// entry holds nothing).
+constexpr uint32_t kEntry = 2;
 template <int HD>
 __device__ __forceinline__ void next_unit(const AttendParams& p, Unit& u) {
   if (u.tile + 1u < u.tiles) {
@@ -122,15 +126,15 @@ __device__ __forceinline__ void next_unit(const AttendParams& p, Unit& u) {
   }
   set_tile<HD>(p, u, 0u);
 }
-// Blocks of all tiles of a sequence (one K/V head), by the whole warp: a lane
+// Cost of all tiles of a sequence (one K/V head), by the whole warp: a lane
 // adds a short sequence's itself, the warp shares a long one's.
 template <int HD>
-__device__ uint64_t sequence_blocks(const AttendParams& p, Unit u) {
+__device__ uint64_t sequence_cost(const AttendParams& p, Unit u) {
   uint64_t sum = 0;
   if (u.tiles <= 4u)
     for (uint32_t i = 0; i < u.tiles; ++i) {
       set_tile<HD>(p, u, i);
-      sum += u.blocks;
+      sum += u.blocks + kEntry;
     }
   uint32_t longs = __ballot_sync(0xffffffffu, u.tiles > 4u);
   while (longs) {
@@ -143,7 +147,7 @@ __device__ uint64_t sequence_blocks(const AttendParams& p, Unit u) {
     uint64_t part = 0;
     for (uint32_t i = threadIdx.x & 31u; i < v.tiles; i += 32u) {
       set_tile<HD>(p, v, i);
-      part += v.blocks;
+      part += v.blocks + kEntry;
     }
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
@@ -151,6 +155,32 @@ __device__ uint64_t sequence_blocks(const AttendParams& p, Unit u) {
   }
   return sum;
 }
+
+// The segments of a CTA's range: blocks [a, e) of unit u, one after the other.
+template <int HD>
+struct Walk {
+  Unit u;
+  uint64_t unit0, left;  // the unit's place in the list; what is left of the range
+  uint32_t at, a, e;     // place in the unit
+  __device__ __forceinline__ bool step(const AttendParams& p) {
+    while (left) {
+      uint32_t cost = u.blocks + kEntry;
+      if (at == cost) {
+        unit0 += cost;
+        at = 0;
+        next_unit<HD>(p, u);
+        cost = u.blocks + kEntry;
+      }
+      const uint32_t take = static_cast<uint32_t>(min(left, static_cast<uint64_t>(cost - at)));
+      a = at > kEntry ? at - kEntry : 0u;
+      at += take;
+      e = at > kEntry ? at - kEntry : 0u;
+      left -= take;
+      if (e > a) return true;
+    }
+    return false;
+  }
+};
 
 // ---- tcgen05 ----------------------------------------------------------------
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -241,6 +271,11 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if one of them is
+  float y;
+  asm("{\n\t.reg .f32 t;\n\tmax.NaN.f32 t, %1, %2;\n\tmax.NaN.f32 %0, t, %3;\n\t}" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 // (x, y) = (x, y) * a + b and (x, y) += (a, b), two at a time
 __device__ __forceinline__ void fma2(float& x, float& y, float a, float b) {
   asm("{\n\t.reg .b64 v, s, t;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 s, {%2, %2};\n\tmov.b64 t, {%3, %3};\n\t"
@@ -248,11 +283,42 @@ __device__ __forceinline__ void fma2(float& x, float& y, float a, float b) {
       : "+f"(x), "+f"(y)
       : "f"(a), "f"(b));
 }
+__device__ __forceinline__ void fma2v(float& x, float& y, float a, float c, float b, float d) {  // (x a + b, y c + d)
+  asm("{\n\t.reg .b64 v, s, t;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 s, {%2, %3};\n\tmov.b64 t, {%4, %5};\n\t"
+      "fma.rn.f32x2 v, v, s, t;\n\tmov.b64 {%0, %1}, v;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(c), "f"(b), "f"(d));
+}
 __device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
   asm("{\n\t.reg .b64 v, s;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 s, {%2, %3};\n\tadd.rn.f32x2 v, v, s;\n\t"
       "mov.b64 {%0, %1}, v;\n\t}"
       : "+f"(x), "+f"(y)
       : "f"(a), "f"(b));
+}
+// 2^x for two numbers on the FMA and integer pipes, for the share of a row's
+// exponentials that the special-function unit (16 per cycle and SM; it bounds a
+// pass) has no time for: x = n + f with n the nearest integer (rounded by adding
+// 1.5 2^23), 2^f by the polynomial of degree 4 of least relative error on
+// [-1/2, 1/2] (Remez exchange, 2.7e-6: below 2^-18, as the sum of the weights
+// keeps it), n added to the exponent.  x is below 2^7; below -126 it counts as
+// -126.
+__device__ __forceinline__ void exp2_pair(float& x, float& y) {
+  constexpr float kMagic = 12582912.f;
+  x = fmaxf(x, -126.f);
+  y = fmaxf(y, -126.f);
+  float tx = x, ty = y;
+  add2(tx, ty, kMagic, kMagic);
+  float nx = tx, ny = ty;
+  add2(nx, ny, -kMagic, -kMagic);
+  fma2v(nx, ny, -1.f, -1.f, x, y);  // f
+  float px, py;
+  px = py = 0.009570102207362652f;
+  fma2v(px, py, nx, ny, 0.05591785907745361f, 0.05591785907745361f);
+  fma2v(px, py, nx, ny, 0.240247443318367f, 0.240247443318367f);
+  fma2v(px, py, nx, ny, 0.6931217908859253f, 0.6931217908859253f);
+  fma2v(px, py, nx, ny, 0.9999992847442627f, 0.9999992847442627f);
+  x = __uint_as_float(__float_as_uint(px) + (__float_as_uint(tx) << 23));
+  y = __uint_as_float(__float_as_uint(py) + (__float_as_uint(ty) << 23));
 }
 // Whether a phase has ended, without waiting (mbar_try_wait may suspend the thread).
 __device__ __forceinline__ bool phase_ended(uint64_t* bar, uint32_t parity) {
@@ -335,11 +401,11 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     u.tiles = 0;
     if (b < p.c.batch) load_sequence<HD>(p, b, u, blockIdx.x == 0u ? p.err : nullptr);
     uint64_t sum;
-    block_scan(sequence_blocks<HD>(p, u) * p.c.kv_heads, scan_part, sum);
+    block_scan(sequence_cost<HD>(p, u) * p.c.kv_heads, scan_part, sum);
     total += sum;
   }
   if (total == 0u) return;
-  const uint64_t want = (total + 1u) / 2u;  // at least two blocks per CTA
+  const uint64_t want = (total + kEntry + 1u) / (kEntry + 2u);  // at least about two blocks per CTA
   const uint64_t ctas = want < gridDim.x ? want : gridDim.x;
   if (blockIdx.x >= ctas) return;
   const uint64_t begin = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1u) / ctas;
@@ -351,7 +417,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
       u.tiles = 0;
       if (b < p.c.batch) load_sequence<HD>(p, b, u, nullptr);
       uint64_t sum;
-      const uint64_t mine = sequence_blocks<HD>(p, u) * p.c.kv_heads;
+      const uint64_t mine = sequence_cost<HD>(p, u) * p.c.kv_heads;
       const uint64_t upto = base + block_scan(mine, scan_part, sum);
       if (mine && begin < upto && begin >= upto - mine) {
         found_b = b;
@@ -375,7 +441,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
       uint64_t n = 0;
       if (i0 + lane < first.tiles) {
         set_tile<HD>(p, v, i0 + lane);
-        n = v.blocks;
+        n = v.blocks + kEntry;
       }
 #pragma unroll
       for (int d = 16; d >= 1; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
@@ -388,7 +454,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
       uint64_t n = 0;
       if (i0 + lane < first.tiles) {
         set_tile<HD>(p, v, i0 + lane);
-        n = v.blocks;
+        n = v.blocks + kEntry;
       }
       uint64_t upto = n;
 #pragma unroll
@@ -421,7 +487,11 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
   const uint32_t tmem = tmem_base;
   first.kv = found_kv;
   set_tile<HD>(p, first, found_tile);
-  const uint32_t first_a = static_cast<uint32_t>(found_at);
+  Walk<HD> walk;
+  walk.u = first;
+  walk.at = static_cast<uint32_t>(found_at);
+  walk.unit0 = begin - walk.at;
+  walk.left = end - begin;
   const auto lane_rows = [&](const Unit& u, uint32_t L) {
     const uint32_t at = u.tile * S::kRows + L * kLaneRows;
     return u.rows > at ? min(kLaneRows, u.rows - at) : 0u;
@@ -445,8 +515,6 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     const float scale = p.scale_log2 == 0.f ? 1e-30f : fabsf(p.scale_log2);
     uint32_t it = 0;  // blocks of this lane
     bool ok = true, first_segment = true;
-    Unit u = first;
-    uint32_t a = first_a;
     // the queries of a lane, a row at a time, 16 bytes per thread
     const auto load_queries = [&](const Unit& v) {
       constexpr uint32_t kChunks = HD / 8, kPer = 32 / kChunks;
@@ -467,9 +535,12 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
       __syncwarp();
       if (lane == 0) arrive(&q_full[L]);
     };
-    if (lane_blocks(u, L, a, static_cast<uint32_t>(min(static_cast<uint64_t>(u.blocks), a + (end - begin))))) load_queries(u);
-    for (uint64_t g = begin; g < end && ok;) {
-      const uint32_t e = static_cast<uint32_t>(min(static_cast<uint64_t>(u.blocks), a + (end - g)));
+    bool more = walk.step(p);
+    if (more && lane_blocks(walk.u, L, walk.a, walk.e)) load_queries(walk.u);
+    while (more && ok) {
+      const Unit u = walk.u;
+      const uint32_t a = walk.a, e = walk.e;
+      const uint64_t unit_last = walk.unit0 + u.blocks + kEntry - 1u;  // the unit's last place in the list
       const uint32_t rows = lane_rows(u, L), n = lane_blocks(u, L, a, e);
       const uint32_t R = u.tile * S::kRows + L * kLaneRows + r;
       const bool real = r < rows;
@@ -510,7 +581,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
         const auto largest = [&](const uint32_t (&v)[32], float (&mx)[4]) {
 #pragma unroll
           for (int c = 0; c < 32; c += 2)
-            mx[c >> 1 & 3] = fmaxf(fmaxf(mx[c >> 1 & 3], __uint_as_float(v[c])), __uint_as_float(v[c + 1]));
+            mx[c >> 1 & 3] = max3(mx[c >> 1 & 3], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
         };
         float before = m, sum;
         if (j == 0u) {  // the first block's maximum; later ones rarely exceed m by the slack
@@ -522,7 +593,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
             if (c < 3u) tc_ld32(tmem_s + (c + 1u) * 32u, s[(c + 1u) & 1u]);
             largest(s[c & 1u], mx);
           }
-          m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+          m = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * scale;
         }
         while (true) {
           const float base = N::kShift - (m == -INFINITY ? 0.f : m);
@@ -539,16 +610,23 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
             for (int x = 0; x < 16; ++x) {
               float w0 = __uint_as_float(v[2 * x]), w1 = __uint_as_float(v[2 * x + 1]);
               fma2(w0, w1, scale, base);
-              w0 = ex2(w0);
-              w1 = ex2(w1);
+              if (x % 4 == 3) {
+                exp2_pair(w0, w1);
+              } else {
+                w0 = ex2(w0);
+                w1 = ex2(w1);
+              }
               add2(zs[x & 3][0], zs[x & 3][1], w0, w1);
               w[c * 16u + x] = N::pack(w0, w1);
             }
           }
           sum = ((zs[0][0] + zs[0][1]) + (zs[1][0] + zs[1][1])) + ((zs[2][0] + zs[2][1]) + (zs[3][0] + zs[3][1]));
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+          const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * scale;
           const bool rise = top > m + Slack<T>::value;
-          if (!__any_sync(0xffffffffu, rise)) break;
+          if (!__any_sync(0xffffffffu, rise)) {
+            if (!(top < INFINITY)) sum = NAN;  // a NaN or +inf score: the row has no weights
+            break;
+          }
           if (rise) m = top;  // and again, with the new maximum
         }
         const bool rise = m != before;
@@ -581,12 +659,8 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
       // Every S of this unit has been computed, so its queries are done with:
       // the next unit's take their place, and its first S is computed while
       // this one's results are written.
-      Unit next = u;
-      const uint64_t g_next = g + (e - a);
-      if (g_next < end) {
-        next_unit<HD>(p, next);
-        if (lane_blocks(next, L, 0u, static_cast<uint32_t>(min(static_cast<uint64_t>(next.blocks), end - g_next)))) load_queries(next);
-      }
+      more = walk.step(p);
+      if (more && lane_blocks(walk.u, L, walk.a, walk.e)) load_queries(walk.u);
       if (n) {
         if (!(ok = warp_wait(&o_done[L], (it - 1u) & 1u, p.err, stop))) break;
         tc_after();
@@ -633,7 +707,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
         }
         if (a == 0u && threadIdx.x == 0u) {  // this unit begins here: what the second launch has to know of it
           Cut& cut = p_cuts(p)[blockIdx.x];
-          cut.parts = static_cast<uint32_t>(((g + u.blocks) * ctas - 1u) / total) - blockIdx.x + 1u;
+          cut.parts = static_cast<uint32_t>(((unit_last + 1u) * ctas - 1u) / total) - blockIdx.x + 1u;
           cut.second = first_segment ? 0u : 1u;
           cut.first_row = u.first_row;
           cut.R0 = u.tile * S::kRows;
@@ -653,9 +727,6 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
         if (spoiled<T, HD>(p, u.slot, u.kv, u.firsts + u.skip, u.seen + u.skip, tx)) row_alone<T, HD>(p, u.slot, u.kv, hx, rx, tx);
       }
       first_segment = false;
-      g = g_next;
-      a = 0;
-      u = next;
     }
     if (!ok) *stop = 1u;
   } else if (warp == S::kSoftmaxWarps) {
@@ -664,8 +735,6 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     const uint32_t q0 = smem_u32(smem), ring = q0 + S::kRing;
     uint32_t st = 0, it[2] = {0, 0}, segs[2] = {0, 0};  // stages consumed, blocks and segments of each lane
     bool ok = true;
-    Unit u = first;
-    uint32_t a = first_a;
     const auto wait_stage = [&](uint32_t x) { return warp_wait(&full[x % kStages], x / kStages & 1u, p.err, stop); };
     const uint64_t high = desc(0u, 16u), high_v = desc(0u, kSub);
     const uint32_t id_s = idesc<T>(kKeys, false) | (p.scale_log2 < 0.f ? 1u << 13 : 0u);
@@ -684,9 +753,9 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
         mma_ts4<8, 128>(tmem + kTmemO + L * HD + half * 128u, tmem + sbuf * 128u + k * 8u, high_v + ((vb + k * 2048u) >> 4),
                         idesc<T>(S::kSubs * 64u, true), fresh && k == 0u ? 0u : 1u);
     };
-    for (uint64_t g = begin; g < end && ok;) {
-      const uint32_t e = static_cast<uint32_t>(min(static_cast<uint64_t>(u.blocks), a + (end - g)));
-      const uint32_t n = e - a;
+    while (ok && walk.step(p)) {
+      const Unit& u = walk.u;
+      const uint32_t a = walk.a, e = walk.e, n = e - a;
       uint32_t ln[2];
       ln[0] = lane_blocks(u, 0, a, e);
       ln[1] = kLanes == 2 ? lane_blocks(u, 1, a, e) : 0u;
@@ -759,9 +828,6 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
           commit(&o_done[0]);
         }
       }
-      g += n;
-      a = 0;
-      if (g < end) next_unit<HD>(p, u);
     }
     if (!ok) *stop = 1u;
     commit(drain);  // every MMA issued above has completed once this arrives
@@ -775,8 +841,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     const uint32_t ring = smem_u32(smem) + S::kRing;
     uint32_t st = 0, told = 0;  // stages issued, and made known to the MMA warp
     bool ok = true;
-    Unit u = first;
-    uint32_t a = first_a;
+    const Unit& u = walk.u;
     const auto tell = [&]() {
       fence_async();
       __syncwarp();
@@ -829,8 +894,8 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
         tell();
       }
     };
-    for (uint64_t g = begin; g < end && ok;) {
-      const uint32_t e = static_cast<uint32_t>(min(static_cast<uint64_t>(u.blocks), a + (end - g)));
+    while (ok && walk.step(p)) {
+      const uint32_t a = walk.a, e = walk.e;
       uint64_t k0 = resolve(a, 0, look(a, 0)), k1 = resolve(a, 1, look(a, 1));
       int32_t n0 = look(a + 1u, 0), n1 = look(a + 1u, 1);
       for (uint32_t h = 0; h < kHalves && ok; ++h) copy(p.c.k, k0, k1, h);
@@ -845,9 +910,6 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
         }
         for (uint32_t h = 0; h < kHalves && ok; ++h) copy(p.c.v, v0, v1, h);
       }
-      g += e - a;
-      a = 0;
-      if (g < end) next_unit<HD>(p, u);
     }
     cp_wait<0>();
     if (ok)
