@@ -334,7 +334,7 @@ RTA_API size_t rta_paged_workspace_bytes(const rta_page_pool* pool, const rta_pa
  *   h / (heads / kv_heads);  lse[b][h] = log sum_p exp(scale q . k_p)
  * q: element (b, h, d) at q + b * q_row_stride + h * q_head_stride + d, 16-byte
  * aligned rows, q_format the pool's format, or RTA_F32 with an RTA_F16 pool;
- * out [batch][heads][head_dim] contiguous in q's format; lse [batch][heads]
+ * out [batch][heads][head_dim] contiguous (16-byte aligned) in q's format; lse [batch][heads]
  * fp32 or NULL.  A sequence of length 0 gives zeros and lse -inf.  heads is a
  * multiple of kv_heads, at most 128 query heads per K/V head. */
 RTA_API rta_status rta_paged_decode(const rta_page_pool* pool, const rta_page_map* map, uint32_t layer,
@@ -347,7 +347,7 @@ RTA_API rta_status rta_paged_decode(const rta_page_pool* pool, const rta_page_ma
  * starts[b] .. starts[b + 1] - 1 (device, batch + 1 entries, ascending from 0
  * to rows), already written to the pages and counted in lengths; row i of m
  * sits at position t = lengths[slot] - m + i.  q_format is the pool's format;
- * out [rows][heads][head_dim], lse [rows][heads].  A row before position 0
+ * out [rows][heads][head_dim] (32-byte aligned), lse [rows][heads].  A row before position 0
  * (more new rows than the sequence is long) gives zeros and lse -inf.  What a
  * row does not see never reaches it, non-finite values included. */
 RTA_API rta_status rta_paged_prefill(const rta_page_pool* pool, const rta_page_map* map, uint32_t layer,

@@ -36,6 +36,7 @@ struct AttendParams {
   float scale_log2;        // scale * log2(e): the softmax runs in base 2
   float scale;
   uint32_t window, sinks;
+  uint32_t align;  // prefill: reads begin at multiples of this many positions
   void* out;
   float* lse;
   uint32_t* err;

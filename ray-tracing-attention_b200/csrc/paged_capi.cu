@@ -124,6 +124,7 @@ const char* attend_params(const rta_page_pool* pool, const rta_page_map* map, ui
   p.scale_log2 = scale * 1.4426950408889634f;
   p.window = window;
   p.sinks = sinks;
+  p.align = 1;
   p.out = out;
   p.lse = lse;
   p.err = w.err;
@@ -208,6 +209,7 @@ rta_status rta_paged_prefill(const rta_page_pool* pool, const rta_page_map* map,
   const char* why = attend_params(pool, map, layer, slots, batch, q, q_format, heads, q_row_stride, q_head_stride,
                                   scale, window, sinks, out, lse, workspace, workspace_bytes, false, p);
   if (!why && !starts) why = "null starts";
+  if (!why && !aligned(out, 32)) why = "out must be 32-byte aligned";
   if (!why && (rows == 0 || static_cast<uint64_t>(rows) * heads >= (1ull << 31))) why = "rows is at least 1, rows * heads below 2^31";
   if (why) return refuse("rta_paged_prefill", why);
   p.starts = starts;

@@ -160,9 +160,9 @@ __device__ __forceinline__ uint32_t new_rows(const AttendParams& p, uint32_t b, 
 // A matrix product multiplies the values of masked positions by a weight of
 // zero, and 0 * inf and 0 * NaN are NaN.  A row whose result is not finite is
 // therefore looked at again: if a position that its tile read but the row does
-// not see (`low` .. `high` around the row's own window) holds a non-finite
-// value, the row is computed over its visible positions alone.  Both run on
-// one full warp; a lane owns HD / 32 neighbouring dimensions.
+// not see (of [sinks, firsts) and [low, high)) holds a non-finite value, the row
+// is computed over its visible positions alone.  Both run on one full warp; a
+// lane owns HD / 32 neighbouring dimensions.
 template <typename T, int HD>
 __device__ __forceinline__ void load_dims(const void* row, uint32_t lane, float (&x)[HD / 32]) {
   const T* r = static_cast<const T*>(row) + lane * (HD / 32);
@@ -171,11 +171,13 @@ __device__ __forceinline__ void load_dims(const void* row, uint32_t lane, float 
 }
 
 template <typename T, int HD>
-__device__ bool spoiled(const AttendParams& p, uint32_t slot, uint32_t kv, uint32_t low, uint32_t high, uint32_t t) {
+__device__ bool spoiled(const AttendParams& p, uint32_t slot, uint32_t kv, uint32_t firsts, uint32_t low, uint32_t high,
+                        uint32_t t) {
   const uint32_t lane = threadIdx.x & 31u;
   const uint32_t mine = p.window && t >= p.window ? t - p.window + 1u : 0u;  // the row's window: mine .. t
   bool bad = false;
-  for (uint32_t x = low; x < high; ++x) {
+  for (uint32_t x = p.sinks < firsts ? p.sinks : low; x < high; ++x) {
+    if (x >= firsts && x < low) x = low;
     if (x <= t && (x >= mine || x < p.sinks)) {
       x = x < mine ? x : t;  // visible: go on behind it
       continue;

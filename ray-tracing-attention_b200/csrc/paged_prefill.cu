@@ -9,12 +9,15 @@
 // unit needs are the first tokens, then a run of neighbours up to its last
 // row's own; they are numbered without the gap, u < firsts ? u : u + skip.
 //
-// Mathematics.  One pass over the blocks with a running maximum and sum per
-// row, in base 2: S = Q K^T, w = 2^(scale_log2 S - m), O += w V, z += sum w.
-// m follows a block's maximum only when that exceeds it by 2^kSlack: the
-// weights then stay below 2^(kSlack + shift), O and z carry the same factor,
-// and O is seldom rescaled.  w enters the second product rounded to the cache's type
-// (its one rounding; the sum takes w itself).
+// Mathematics.  One pass over the blocks, in base 2: S = Q K^T, w = 2^(scale_log2
+// S - m), O += w V, z += sum w, with a reference m per row.  m is the maximum of
+// the first positions the row sees, and stays while a block's weights add up to
+// less than Room: a row's result is O / z whatever m is, so m only has to keep
+// the weights in range, and the maximum of later blocks is not looked for (a
+// pass over S is bounded by its exponentials and conversions).  Otherwise the
+// block is weighed again with its own maximum and O and z are scaled.  w enters
+// the second product rounded to the cache's type (its one rounding; the sum
+// takes w itself).
 //
 // Work: the blocks of all units form one list, cut evenly over the CTAs (one
 // per SM) whatever the lengths are; a lane of a unit that is cut leaves a
@@ -26,12 +29,17 @@
 //              write results or records
 //   MMA        one warp issues S = Q K^T (both operands in shared memory) and
 //              O += w V (w from tensor memory)
-//   producers  three warps copy K and V blocks into a ring of stages (128
-//              positions x up to 128 dimensions, 128-byte swizzle)
+//   producers  three warps bring K and V blocks into a ring of stages (128
+//              positions x up to 128 dimensions, 128-byte swizzle): by TMA, a
+//              box of positions of one page at a time, where the page size is a
+//              multiple of 32; otherwise, and for a unit's last block (its end is
+//              filled with zeros), row by row with 16-byte copies
 // head_dim 256: one lane, two S buffers, so that S of the next block is
 // computed under this block's softmax; 64 and 128: two lanes take turns.
 #include <atomic>
 #include <mutex>
+
+#include <cuda.h>
 
 #include "paged_device.cuh"
 
@@ -68,9 +76,16 @@ struct Cut {
   uint32_t second;  // this CTA's record of it is its second (the others': their first)
   uint32_t first_row, R0, rows, kv, slot;
   int32_t past;
-  uint32_t low, high;
+  uint32_t firsts, low, high;
 };
 __device__ __forceinline__ Cut* p_cuts(const AttendParams& p) { return static_cast<Cut*>(p.cuts); }
+
+// K and V as TMA sees them: (dimension, position in the page, head, page), or
+// head before position where that is the order of the strides.
+struct Maps {
+  CUtensorMap k, v;
+  uint32_t box, heads_first;  // positions per box, 0: no TMA
+};
 
 // One unit and its place in the list.
 struct Unit {
@@ -103,8 +118,10 @@ __device__ __forceinline__ void set_tile(const AttendParams& p, Unit& u, uint32_
   u.tile = tile;
   const uint32_t R0 = tile * Shape<HD>::kRows, R1 = min(R0 + Shape<HD>::kRows, u.rows);
   const int32_t t0 = u.past + static_cast<int32_t>(R0 / p.group);
-  const uint32_t low = p.window && t0 >= 0 && static_cast<uint32_t>(t0) >= p.window ? t0 - p.window + 1u : 0u;
-  u.firsts = min(p.sinks, low);
+  // what is read begins and ends the first tokens at whole boxes
+  uint32_t low = p.window && t0 >= 0 && static_cast<uint32_t>(t0) >= p.window ? t0 - p.window + 1u : 0u;
+  low -= low % p.align;
+  u.firsts = min((min(p.sinks, 1u << 30) + p.align - 1u) / p.align * p.align, low);
   u.skip = low - u.firsts;
   u.seen = seen_by(p, u, R1 - 1u);
   u.blocks = blocks_of(u.seen);
@@ -262,6 +279,11 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
       "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar))
       : "memory");
 }
+__device__ __forceinline__ void store32(void* at, const uint32_t* v) {  // 32 bytes, 32-byte aligned
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 __device__ __forceinline__ void arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -283,42 +305,19 @@ __device__ __forceinline__ void fma2(float& x, float& y, float a, float b) {
       : "+f"(x), "+f"(y)
       : "f"(a), "f"(b));
 }
-__device__ __forceinline__ void fma2v(float& x, float& y, float a, float c, float b, float d) {  // (x a + b, y c + d)
-  asm("{\n\t.reg .b64 v, s, t;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 s, {%2, %3};\n\tmov.b64 t, {%4, %5};\n\t"
-      "fma.rn.f32x2 v, v, s, t;\n\tmov.b64 {%0, %1}, v;\n\t}"
-      : "+f"(x), "+f"(y)
-      : "f"(a), "f"(c), "f"(b), "f"(d));
-}
 __device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
   asm("{\n\t.reg .b64 v, s;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 s, {%2, %3};\n\tadd.rn.f32x2 v, v, s;\n\t"
       "mov.b64 {%0, %1}, v;\n\t}"
       : "+f"(x), "+f"(y)
       : "f"(a), "f"(b));
 }
-// 2^x for two numbers on the FMA and integer pipes, for the share of a row's
-// exponentials that the special-function unit (16 per cycle and SM; it bounds a
-// pass) has no time for: x = n + f with n the nearest integer (rounded by adding
-// 1.5 2^23), 2^f by the polynomial of degree 4 of least relative error on
-// [-1/2, 1/2] (Remez exchange, 2.7e-6: below 2^-18, as the sum of the weights
-// keeps it), n added to the exponent.  x is below 2^7; below -126 it counts as
-// -126.
-__device__ __forceinline__ void exp2_pair(float& x, float& y) {
-  constexpr float kMagic = 12582912.f;
-  x = fmaxf(x, -126.f);
-  y = fmaxf(y, -126.f);
-  float tx = x, ty = y;
-  add2(tx, ty, kMagic, kMagic);
-  float nx = tx, ny = ty;
-  add2(nx, ny, -kMagic, -kMagic);
-  fma2v(nx, ny, -1.f, -1.f, x, y);  // f
-  float px, py;
-  px = py = 0.009570102207362652f;
-  fma2v(px, py, nx, ny, 0.05591785907745361f, 0.05591785907745361f);
-  fma2v(px, py, nx, ny, 0.240247443318367f, 0.240247443318367f);
-  fma2v(px, py, nx, ny, 0.6931217908859253f, 0.6931217908859253f);
-  fma2v(px, py, nx, ny, 0.9999992847442627f, 0.9999992847442627f);
-  x = __uint_as_float(__float_as_uint(px) + (__float_as_uint(tx) << 23));
-  y = __uint_as_float(__float_as_uint(py) + (__float_as_uint(ty) << 23));
+__device__ __forceinline__ void tma4(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, int32_t w,
+                                     uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+          dst),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
 }
 // Whether a phase has ended, without waiting (mbar_try_wait may suspend the thread).
 __device__ __forceinline__ bool phase_ended(uint64_t* bar, uint32_t parity) {
@@ -347,14 +346,14 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32
   }
 }
 
+// A block's weights may add up to this much (each is then below it) before the
+// row takes a new reference: fp16 weights end at 2^16, bf16 ones have fp32's range.
 template <typename T>
-struct Slack {
-  // weights stay below 2^(slack + shift): fp16 ends at 2^16
-  static constexpr float value = Num<T>::kBf16 ? 8.f : 5.f;
+struct Room {
+  static constexpr float value = Num<T>::kBf16 ? 1.152921504606846976e18f : 16384.f;  // 2^60, 2^14
 };
-
 template <typename T, int HD>
-__global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const AttendParams p, const __grid_constant__ Maps maps) {
   using S = Shape<HD>;
   using N = Num<T>;
   constexpr uint32_t kLanes = S::kLanes, kStages = S::kStages, kHalves = S::kHalves;
@@ -556,7 +555,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
       const int32_t t_last = rows ? u.past + static_cast<int32_t>((u.tile * S::kRows + L * kLaneRows + rows - 1u) / p.group) : -1;
       const uint32_t clear_hi = t_first < 0 ? 0u : static_cast<uint32_t>(t_first) + 1u - u.skip;
       const uint32_t clear_lo = p.window && t_last >= 0 && static_cast<uint32_t>(t_last) >= p.window ? t_last - p.window + 1u - u.skip : 0u;
-      float m = -INFINITY, z = 0.f;
+      float m = t < 0 ? 0.f : -INFINITY, z = 0.f;  // a row that sees nothing needs no reference
       for (uint32_t j = 0; j < n; ++j, ++it) {
         const uint32_t sb = kLanes == 2 ? L : it & 1u;
         const uint32_t tmem_s = tmem + lane_addr + sb * 128u;
@@ -569,6 +568,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
           const int32_t lo = static_cast<int32_t>(w_lo) - static_cast<int32_t>(u0), hi = static_cast<int32_t>(w_hi) - static_cast<int32_t>(u0);
 #pragma unroll 1
           for (int32_t c0 = 0; c0 < 128; c0 += 32) {
+            if (u0 + c0 >= clear_lo && u0 + c0 + 32u <= clear_hi) continue;
             tc_ld32(tmem_s + c0, s[0]);
             tc_wait_ld(s[0]);
 #pragma unroll
@@ -578,26 +578,29 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
           }
           tc_wait_st();
         }
-        const auto largest = [&](const uint32_t (&v)[32], float (&mx)[4]) {
+        // the largest score of the first `columns` (NaN if one of them is)
+        const auto largest = [&](uint32_t columns) {
+          float x = -INFINITY;
+#pragma unroll 1
+          for (uint32_t c = 0; c < columns; c += 32u) {
+            tc_ld32(tmem_s + c, s[0]);
+            tc_wait_ld(s[0]);
+            float mx[4] = {x, x, x, x};
 #pragma unroll
-          for (int c = 0; c < 32; c += 2)
-            mx[c >> 1 & 3] = max3(mx[c >> 1 & 3], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
-        };
-        float before = m, sum;
-        if (j == 0u) {  // the first block's maximum; later ones rarely exceed m by the slack
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          tc_ld32(tmem_s, s[0]);
-#pragma unroll
-          for (uint32_t c = 0; c < 4u; ++c) {
-            tc_wait_ld(s[c & 1u]);
-            if (c < 3u) tc_ld32(tmem_s + (c + 1u) * 32u, s[(c + 1u) & 1u]);
-            largest(s[c & 1u], mx);
+            for (int i = 0; i < 32; i += 2)
+              mx[i >> 1 & 3] = max3(mx[i >> 1 & 3], __uint_as_float(s[0][i]), __uint_as_float(s[0][i + 1]));
+            x = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
           }
-          m = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * scale;
+          return x * scale;
+        };
+        const float before = m;
+        for (uint32_t columns = 32u; columns <= kKeys && __any_sync(0xffffffffu, m == -INFINITY); columns *= 4u) {
+          const float x = largest(columns);  // 32 positions give most rows a reference, all of the block the rest
+          if (m == -INFINITY) m = x;
         }
-        while (true) {
-          const float base = N::kShift - (m == -INFINITY ? 0.f : m);
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float sum;
+        for (bool again = false;;) {
+          const float base = m == -INFINITY ? 0.f : -m;
           float zs[4][2] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
           tc_ld32(tmem_s, s[0]);
 #pragma unroll
@@ -605,30 +608,24 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
             tc_wait_ld(s[c & 1u]);
             if (c < 3u) tc_ld32(tmem_s + (c + 1u) * 32u, s[(c + 1u) & 1u]);
             uint32_t(&v)[32] = s[c & 1u];
-            largest(v, mx);
 #pragma unroll
             for (int x = 0; x < 16; ++x) {
               float w0 = __uint_as_float(v[2 * x]), w1 = __uint_as_float(v[2 * x + 1]);
               fma2(w0, w1, scale, base);
-              if (x % 4 == 3) {
-                exp2_pair(w0, w1);
-              } else {
-                w0 = ex2(w0);
-                w1 = ex2(w1);
-              }
+              w0 = ex2(w0);
+              w1 = ex2(w1);
               add2(zs[x & 3][0], zs[x & 3][1], w0, w1);
               w[c * 16u + x] = N::pack(w0, w1);
             }
           }
           sum = ((zs[0][0] + zs[0][1]) + (zs[1][0] + zs[1][1])) + ((zs[2][0] + zs[2][1]) + (zs[3][0] + zs[3][1]));
-          const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * scale;
-          const bool rise = top > m + Slack<T>::value;
-          if (!__any_sync(0xffffffffu, rise)) {
-            if (!(top < INFINITY)) sum = NAN;  // a NaN or +inf score: the row has no weights
-            break;
-          }
-          if (rise) m = top;  // and again, with the new maximum
+          const bool over = !(sum < Room<T>::value);
+          if (again || !__any_sync(0xffffffffu, over)) break;
+          const float x = largest(kKeys);
+          if (over) m = x;
+          again = true;
         }
+        if (!(m < INFINITY)) sum = NAN;  // a NaN or +inf score: the row has no weights
         const bool rise = m != before;
         const float factor = rise ? ex2(before - m) : 1.f;  // before = -inf: 0
         z = z * factor + sum;
@@ -682,12 +679,12 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
             bad |= !isfinite(f0) || !isfinite(f1);
             o[x] = N::pack(f0, f1);
           }
-          if (real)
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              *reinterpret_cast<uint4*>(out + c + 8 * x) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+          if (real) {
+            store32(out + c, o);
+            store32(out + c + 16, o + 8);
+          }
         }
-        if (real && p.lse) p.lse[at] = t < 0 ? -INFINITY : (m - N::kShift + log2f(z)) * kLn2;
+        if (real && p.lse) p.lse[at] = t < 0 ? -INFINITY : (m + log2f(z)) * kLn2;
       } else if (rows) {
         float* const rec = p.records + (static_cast<size_t>(blockIdx.x * 2u + (first_segment ? 0u : 1u)) * kLanes + L) * S::kRecord;
         rec[r] = m;
@@ -715,6 +712,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
           cut.kv = u.kv;
           cut.slot = u.slot;
           cut.past = u.past;
+          cut.firsts = u.firsts;
           cut.low = u.firsts + u.skip;
           cut.high = u.seen + u.skip;
         }
@@ -724,7 +722,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
         const int x = __ffs(again) - 1;
         again &= again - 1u;
         const uint32_t tx = __shfl_sync(0xffffffffu, t, x), hx = __shfl_sync(0xffffffffu, head, x), rx = __shfl_sync(0xffffffffu, row, x);
-        if (spoiled<T, HD>(p, u.slot, u.kv, u.firsts + u.skip, u.seen + u.skip, tx)) row_alone<T, HD>(p, u.slot, u.kv, hx, rx, tx);
+        if (spoiled<T, HD>(p, u.slot, u.kv, u.firsts, u.firsts + u.skip, u.seen + u.skip, tx)) row_alone<T, HD>(p, u.slot, u.kv, hx, rx, tx);
       }
       first_segment = false;
     }
@@ -866,14 +864,57 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
       return static_cast<uint64_t>(page) * p.c.page_bytes + static_cast<uint64_t>(pos - page_of(p.c, pos) * p.c.page_size) * p.c.pos_bytes +
              static_cast<uint64_t>(u.kv) * p.c.head_bytes;
     };
-    // one stage: dimensions [128 half, ..) of a block's K or V rows
-    const auto copy = [&](const uint8_t* base, uint64_t off0, uint64_t off1, uint32_t half) {
+    const auto flush = [&]() {
+      cp_wait<0>();
+      while (told < st) tell();
+    };
+    // waits until the next stage is free
+    const auto next_stage = [&]() {
       const uint32_t s = st % kStages, par = (st / kStages & 1u) ^ 1u;
       if (!__all_sync(0xffffffffu, phase_ended(&empty[s], par))) {
-        cp_wait<0>();  // the MMA warp must know of every stage issued while this warp waits
-        while (told < st) tell();
-        if (!(ok = warp_wait(&empty[s], par, p.err, stop))) return;
+        flush();  // the MMA warp must know of every stage issued while this warp waits
+        ok = warp_wait(&empty[s], par, p.err, stop);
       }
+      return s;
+    };
+    // one stage by TMA: lane i of the first producer brings box i, of `page`
+    const uint32_t boxes = maps.box ? kKeys / maps.box : 0u;
+    const auto bring = [&](const CUtensorMap* map, int32_t page, uint32_t block, uint32_t half) {
+      flush();
+      const uint32_t s = next_stage();
+      if (!ok) return;
+      if (w == 0u) {
+        if (lane == 0) mbar_expect_tx(&full[s], S::kStage);
+        __syncwarp();
+        if (lane < boxes) {
+          const uint32_t at = block * kKeys + lane * maps.box, pos = at < u.firsts ? at : at + u.skip;
+          const int32_t y = static_cast<int32_t>(pos - page_of(p.c, pos) * p.c.page_size), kv = static_cast<int32_t>(u.kv);
+          // a page outside the pool is flagged and read as zeros, as TMA reads outside its bounds
+          if (static_cast<uint32_t>(page) >= p.c.pages) {
+            atomicOr(p.err, RTA_DEVERR_PAGE);
+            page = static_cast<int32_t>(p.c.pages);
+          }
+          const uint32_t dst = ring + s * S::kStage + lane * maps.box * 128u;
+#pragma unroll
+          for (uint32_t x = 0; x < S::kSubs; ++x)
+            tma4(dst + x * kSub, map, static_cast<int32_t>(half * 128u + x * 64u), maps.heads_first ? kv : y,
+                 maps.heads_first ? y : kv, page, &full[s]);
+        }
+      } else if (lane == 0) {
+        arrive(&full[s]);
+      }
+      told = ++st;
+    };
+    const auto box_page = [&](uint32_t block) -> int32_t {
+      const uint32_t at = block * kKeys + lane * maps.box;
+      if (w != 0u || lane >= boxes || at >= u.seen) return 0;
+      const uint32_t pos = at < u.firsts ? at : at + u.skip;
+      return p.c.table[static_cast<size_t>(u.slot) * p.c.width + page_of(p.c, pos)];
+    };
+    // one stage row by row: dimensions [128 half, ..) of a block's K or V rows
+    const auto copy = [&](const uint8_t* base, uint64_t off0, uint64_t off1, uint32_t half) {
+      const uint32_t s = next_stage();
+      if (!ok) return;
       const uint32_t dst = ring + s * S::kStage, c = lane & 7u;
 #pragma unroll
       for (uint32_t x = 0; x < kOwn / 4u; ++x) {
@@ -896,26 +937,52 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     };
     while (ok && walk.step(p)) {
       const uint32_t a = walk.a, e = walk.e;
-      uint64_t k0 = resolve(a, 0, look(a, 0)), k1 = resolve(a, 1, look(a, 1));
-      int32_t n0 = look(a + 1u, 0), n1 = look(a + 1u, 1);
-      for (uint32_t h = 0; h < kHalves && ok; ++h) copy(p.c.k, k0, k1, h);
-      for (uint32_t j = a; j < e && ok; ++j) {
-        const uint64_t v0 = k0, v1 = k1;
-        if (j + 1u < e) {
-          k0 = resolve(j + 1u, 0, n0);
-          k1 = resolve(j + 1u, 1, n1);
-          n0 = look(j + 2u, 0);
-          n1 = look(j + 2u, 1);
-          for (uint32_t h = 0; h < kHalves && ok; ++h) copy(p.c.k, k0, k1, h);
+      // blocks [a, whole) lie inside the sequence and come by TMA
+      const uint32_t whole = maps.box ? min(e, max(a, u.seen / kKeys)) : a;
+      int32_t kp = box_page(a), np = box_page(a + 1u), vp = 0;  // pages of this K block, the next, and the V block
+      uint64_t k0 = 0, k1 = 0, v0 = 0, v1 = 0;
+      int32_t n0 = kNone, n1 = kNone;
+      if (whole < a + 2u) {
+        n0 = look(whole, 0);
+        n1 = look(whole, 1);
+      }
+      for (uint32_t j = a; j <= e && ok; ++j) {  // K of block j, then V of block j - 1
+        v0 = k0;
+        v1 = k1;
+        if (j < e) {
+          if (j < whole) {
+            for (uint32_t h = 0; h < kHalves && ok; ++h) bring(&maps.k, kp, j, h);
+          } else {
+            k0 = resolve(j, 0, n0);
+            k1 = resolve(j, 1, n1);
+            for (uint32_t h = 0; h < kHalves && ok; ++h) copy(p.c.k, k0, k1, h);
+          }
+          if (j + 1u >= whole) {
+            n0 = look(j + 1u, 0);
+            n1 = look(j + 1u, 1);
+          }
         }
-        for (uint32_t h = 0; h < kHalves && ok; ++h) copy(p.c.v, v0, v1, h);
+        if (j > a && ok) {
+          if (j - 1u < whole) {
+            for (uint32_t h = 0; h < kHalves && ok; ++h) bring(&maps.v, vp, j - 1u, h);
+          } else {
+            for (uint32_t h = 0; h < kHalves && ok; ++h) copy(p.c.v, v0, v1, h);
+          }
+        }
+        vp = kp;
+        kp = np;
+        np = box_page(j + 2u);
       }
     }
     cp_wait<0>();
     if (ok)
       while (told < st) tell();
-    else
+    else {
       *stop = 1u;
+      if (w == 0u)  // boxes still on their way have landed before the CTA exits (bounded)
+        for (uint32_t x = st > kStages ? st - kStages : 0u; x < st; ++x)
+          (void)warp_wait(&full[x % kStages], x / kStages & 1u, nullptr, &never);
+    }
   }
   tc_before();
   __syncthreads();
@@ -968,7 +1035,7 @@ __global__ void __launch_bounds__(256) prefill_join_kernel(const AttendParams p)
       uint32_t row, head;
       int32_t t;
       place(y0 + x, row, head, t);
-      p.lse[static_cast<size_t>(row) * p.heads + head] = t < 0 ? -INFINITY : (mm - N::kShift + log2f(zz)) * kLn2;
+      p.lse[static_cast<size_t>(row) * p.heads + head] = t < 0 ? -INFINITY : (mm + log2f(zz)) * kLn2;
     }
   }
   __syncthreads();
@@ -1008,9 +1075,58 @@ __global__ void __launch_bounds__(256) prefill_join_kernel(const AttendParams p)
     uint32_t row, head;
     int32_t t;
     place(y0 + x, row, head, t);
-    if (spoiled<T, HD>(p, cut.slot, cut.kv, cut.low, cut.high, static_cast<uint32_t>(t)))
+    if (spoiled<T, HD>(p, cut.slot, cut.kv, cut.firsts, cut.low, cut.high, static_cast<uint32_t>(t)))
       row_alone<T, HD>(p, cut.slot, cut.kv, head, row, static_cast<uint32_t>(t));
   }
+}
+
+// Tensor maps of the call's layer, if pages hold whole boxes of at least 32
+// positions and the strides are of the kind that TMA takes; otherwise box = 0 and
+// rows are copied.  A box costs about as much to issue whatever its size: boxes of
+// 16 positions made 8192 rows of 256-dimension heads 886 us where copied rows took
+// 676, boxes of 32 and 64 positions saved 4 and 2 percent of ragged batches.
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encoder() {
+  static EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  return fn;
+}
+template <typename T>
+void encode(const AttendParams& p, Maps& maps) {
+  maps.box = 0;
+  maps.heads_first = p.c.head_bytes < p.c.pos_bytes ? 1u : 0u;
+  uint32_t box = 128;
+  while (p.c.page_size % box) box /= 2u;
+  const EncodeFn fn = encoder();
+  if (box < 32u || !fn) return;
+  // a dimension of extent 1 is never stepped over: give it the stride that its neighbours ask for
+  uint64_t pos = p.c.pos_bytes, head = p.c.head_bytes, page = p.c.page_bytes;
+  const uint64_t row = p.c.head_dim * 2u;
+  if (p.c.kv_heads == 1u) {
+    maps.heads_first = 0u;
+    head = pos * p.c.page_size;
+  }
+  if (p.c.pages == 1u) page = maps.heads_first ? pos * p.c.page_size : head * p.c.kv_heads;
+  if (pos < row || head < row || page < row) return;
+  const uint64_t a = maps.heads_first ? p.c.kv_heads : p.c.page_size, b = maps.heads_first ? p.c.page_size : p.c.kv_heads;
+  const cuuint64_t dims[4] = {p.c.head_dim, a, b, p.c.pages};
+  const cuuint64_t strides[3] = {maps.heads_first ? head : pos, maps.heads_first ? pos : head, page};
+  const cuuint32_t boxes[4] = {64u, maps.heads_first ? 1u : box, maps.heads_first ? box : 1u, 1u}, steps[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type = Num<T>::kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  for (int i = 0; i < 2; ++i)
+    if (fn(i ? &maps.v : &maps.k, type, 4, const_cast<uint8_t*>(i ? p.c.v : p.c.k), dims, strides, boxes, steps,
+           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return;
+  maps.box = box;
 }
 
 template <typename T, int HD>
@@ -1032,7 +1148,11 @@ cudaError_t launch(const AttendParams& p, cudaStream_t s) {
     sms_of[dev].store(sms, std::memory_order_release);
   }
   const uint32_t ctas = static_cast<uint32_t>(sms) < kMaxCtas ? static_cast<uint32_t>(sms) : kMaxCtas;
-  prefill_kernel<T, HD><<<ctas, Shape<HD>::kThreads, Shape<HD>::kSmem, s>>>(p);
+  Maps maps;
+  AttendParams q = p;
+  encode<T>(p, maps);
+  q.align = maps.box ? maps.box : 1u;
+  prefill_kernel<T, HD><<<ctas, Shape<HD>::kThreads, Shape<HD>::kSmem, s>>>(q, maps);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
@@ -1044,7 +1164,7 @@ cudaError_t launch(const AttendParams& p, cudaStream_t s) {
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, prefill_join_kernel<T, HD>, p);
+  return cudaLaunchKernelEx(&cfg, prefill_join_kernel<T, HD>, q);
 }
 template <typename T>
 cudaError_t by_dim(const AttendParams& p, cudaStream_t s) {
