@@ -29,7 +29,7 @@
 //              write results or records
 //   MMA        one warp issues S = Q K^T (both operands in shared memory) and
 //              O += w V (w from tensor memory)
-//   producers  three warps bring K and V blocks into a ring of stages (128
+//   producers  three or seven warps bring K and V blocks into a ring of stages (128
 //              positions x up to 128 dimensions, 128-byte swizzle): by TMA, a
 //              box of positions of one page at a time, where the page size is a
 //              multiple of 32; otherwise, and for a unit's last block (its end is
@@ -60,7 +60,9 @@ struct Shape {
   static constexpr uint32_t kQ = HD / 64 * kSub;                  // bytes of one lane's queries
   static constexpr uint32_t kStages = HD == 64 ? 10 : 5;
   static constexpr uint32_t kSoftmaxWarps = 4 * kLanes;
-  static constexpr uint32_t kThreads = (kSoftmaxWarps + 4) * 32;
+  static constexpr uint32_t kProducers = HD == 256 ? 7 : 3;
+  static constexpr uint32_t kOwn = HD == 256 ? 20 : 44;           // rows of a stage per producer (the last one: the rest)
+  static constexpr uint32_t kThreads = (kSoftmaxWarps + 1 + kProducers) * 32;
   static constexpr uint32_t kRows = kLanes * kLaneRows;           // rows per unit
   static constexpr uint32_t kRing = kLanes * kQ;                  // offset of the stages
   static constexpr uint32_t kBars = kRing + kStages * kStage;     // offset of the barriers
@@ -375,7 +377,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
 
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < kStages; ++i) {
-      mbar_init(&full[i], 3);
+      mbar_init(&full[i], S::kProducers);
       mbar_init(&empty[i], 1);
     }
     for (uint32_t i = 0; i < 2u; ++i) {
@@ -505,8 +507,9 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
 
   if (warp < S::kSoftmaxWarps) {
     // ---------------------------------------------------------------- softmax
-    // 2 x 128 x 208 + 128 x 80 registers of the launch's 384 x 168
+    // registers of the launch: 384 x 168 = 64512; two lanes: 256 x 208 + 128 x 80, one lane: 128 x 240 + 256 x 128
     if constexpr (kLanes == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 240;");
     const uint32_t L = warp >> 2, quarter = warp & 3u, r = quarter * 32u + lane;
     const uint32_t lane_addr = quarter * 32u << 16, tmem_o = tmem + lane_addr + kTmemO + L * HD;
     const uint32_t q_smem = smem_u32(smem) + L * S::kQ;
@@ -529,13 +532,18 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
                    static_cast<const uint8_t*>(p.q) + o + c * 16u, on);
       }
       cp_commit();
+    };
+    const auto queries_here = [&]() {
       cp_wait<0>();
       fence_async();
       __syncwarp();
       if (lane == 0) arrive(&q_full[L]);
     };
     bool more = walk.step(p);
-    if (more && lane_blocks(walk.u, L, walk.a, walk.e)) load_queries(walk.u);
+    if (more && lane_blocks(walk.u, L, walk.a, walk.e)) {
+      load_queries(walk.u);
+      queries_here();
+    }
     while (more && ok) {
       const Unit u = walk.u;
       const uint32_t a = walk.a, e = walk.e;
@@ -633,7 +641,8 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
         tc_st32(tmem_s + 32, w + 32);
         if (j) {
           // O holds the blocks before this one
-          if (!(ok = warp_wait(&o_done[L], (it - 1u) & 1u, p.err, stop))) break;
+          // (two lanes: S of this block was computed after O of the one before)
+          if (kLanes == 1 && !(ok = warp_wait(&o_done[L], (it - 1u) & 1u, p.err, stop))) break;
           if (__any_sync(0xffffffffu, rise)) {
             tc_after();
 #pragma unroll 1
@@ -655,9 +664,12 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
       if (!ok) break;
       // Every S of this unit has been computed, so its queries are done with:
       // the next unit's take their place, and its first S is computed while
-      // this one's results are written.
+      // this one's results are written.  (Loading them a block earlier put the
+      // search for the next unit into the loop over blocks: 8 percent slower.)
       more = walk.step(p);
-      if (more && lane_blocks(walk.u, L, walk.a, walk.e)) load_queries(walk.u);
+      const bool ahead = more && lane_blocks(walk.u, L, walk.a, walk.e);
+      if (ahead) load_queries(walk.u);
+      if (ahead) queries_here();
       if (n) {
         if (!(ok = warp_wait(&o_done[L], (it - 1u) & 1u, p.err, stop))) break;
         tc_after();
@@ -668,22 +680,26 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
         const size_t at = static_cast<size_t>(row) * p.heads + head;
         T* const out = static_cast<T*>(p.out) + at * HD;
         const float inv = 1.f / z;
-#pragma unroll 1
+        float odd[2] = {0.f, 0.f};  // NaN once a result is not finite
+#pragma unroll 1  // (unrolled: 10 percent slower, the loop over blocks leaves the instruction cache)
         for (uint32_t c = 0; c < HD; c += 32u) {
           uint32_t o[32];
           tc_ld32(tmem_o + c, o);
           tc_wait_ld(o);
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
-            const float f0 = t < 0 ? 0.f : __uint_as_float(o[2 * x]) * inv, f1 = t < 0 ? 0.f : __uint_as_float(o[2 * x + 1]) * inv;
-            bad |= !isfinite(f0) || !isfinite(f1);
-            o[x] = N::pack(f0, f1);
+            float f0 = __uint_as_float(o[2 * x]), f1 = __uint_as_float(o[2 * x + 1]);
+            fma2(f0, f1, inv, 0.f);
+            o[x] = t < 0 ? 0u : N::pack(f0, f1);
+            fma2(f0, f1, 0.f, 0.f);
+            add2(odd[0], odd[1], f0, f1);
           }
           if (real) {
             store32(out + c, o);
             store32(out + c + 16, o + 8);
           }
         }
+        bad = !(odd[0] + odd[1] == 0.f);
         if (real && p.lse) p.lse[at] = t < 0 ? -INFINITY : (m + log2f(z)) * kLn2;
       } else if (rows) {
         float* const rec = p.records + (static_cast<size_t>(blockIdx.x * 2u + (first_segment ? 0u : 1u)) * kLanes + L) * S::kRecord;
@@ -730,6 +746,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
   } else if (warp == S::kSoftmaxWarps) {
     // -------------------------------------------------------------------- MMA
     if constexpr (kLanes == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
     const uint32_t q0 = smem_u32(smem), ring = q0 + S::kRing;
     uint32_t st = 0, it[2] = {0, 0}, segs[2] = {0, 0};  // stages consumed, blocks and segments of each lane
     bool ok = true;
@@ -834,7 +851,8 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
   } else {
     // -------------------------------------------------------------- producers
     if constexpr (kLanes == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    constexpr uint32_t kOwn = 44;  // rows of a stage per warp: 44, 44, 40
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
+    constexpr uint32_t kOwn = S::kOwn;
     const uint32_t w = warp - S::kSoftmaxWarps - 1u, row0 = w * kOwn, mine = min(kOwn, kKeys - row0);
     const uint32_t ring = smem_u32(smem) + S::kRing;
     uint32_t st = 0, told = 0;  // stages issued, and made known to the MMA warp
