@@ -10,6 +10,24 @@
 namespace rta {
 namespace paged {
 
+// A launch that may begin under the kernel before it: every kernel of the paged
+// cache waits (griddepcontrol.wait) before it touches memory, so only the launch
+// itself overlaps.
+template <typename... P, typename... A>
+inline cudaError_t launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, A&&... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // CTAs of an attention launch at most (one per SM): bounds the split records.
 constexpr uint32_t kMaxCtas = 160;
 

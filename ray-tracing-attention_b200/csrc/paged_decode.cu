@@ -93,8 +93,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
   const uint32_t per_seq = p.c.kv_heads * blocks;
   Q* const out = static_cast<Q*>(p.out);
 
+  pdl_wait();
+  pdl_launch_dependents();
+
   // ---- the list of tiles: its length, and this CTA's range -----------------
-  uint64_t total = 0;
+  uint64_t total = 0, own = 0, own_upto = 0;  // this thread's (last) sequence in the list
   for (uint32_t b0 = 0; b0 < p.c.batch; b0 += kThreads) {
     const uint32_t b = b0 + threadIdx.x;
     uint64_t mine = 0, sum;
@@ -109,7 +112,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
           for (uint32_t h = 0; h < p.heads; ++h) p.lse[static_cast<size_t>(b) * p.heads + h] = -INFINITY;
       }
     }
-    block_scan(mine, scan_part, sum);
+    own = mine;
+    own_upto = total + block_scan(mine, scan_part, sum);
     total += sum;
   }
   if (total == 0u) return;
@@ -121,7 +125,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
   const auto owner = [&](uint64_t t) { return static_cast<uint32_t>(((t + 1u) * ctas - 1u) / total); };
 
   // ---- the unit that holds the first tile ----------------------------------
-  {
+  if (p.c.batch <= kThreads) {
+    if (own && begin < own_upto && begin >= own_upto - own) {
+      found_b = threadIdx.x;
+      found_at = begin - (own_upto - own);
+    }
+    __syncthreads();
+  } else {
     uint64_t base = 0;
     for (uint32_t b0 = 0; b0 < p.c.batch; b0 += kThreads) {
       const uint32_t b = b0 + threadIdx.x;
@@ -405,20 +415,46 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
           if (p.lse && lane == 0u)
             p.lse[static_cast<size_t>(u.b) * p.heads + head0 + h] = (mm - N::kShift + log2f(zz)) * kLn2;
         }
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < heads * (HD / 4); i += kThreads) {
-          const uint32_t h = i / (HD / 4), d = i % (HD / 4) * 4u;
-          float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-          for (uint32_t j = 0; j < parts; ++j) {
-            const float f = weight[h * kMaxCtas + j];
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(record(c0 + j) + kRecHeader + h * HD + d));
-            oo.x += x.x * f;
-            oo.y += x.y * f;
-            oo.z += x.z * f;
-            oo.w += x.w * f;
+        // the records' O come through shared memory, as many at a time as fit:
+        // all their 16-byte copies are in flight at once
+        constexpr uint32_t kWeights = kMaxCtas * kHeadsMax * 4, kEach = (S::kHeads * (HD / 4) + kThreads - 1u) / kThreads;
+        float* const stage = reinterpret_cast<float*>(smem + kWeights);
+        const uint32_t quads = heads * (HD / 4), fit = min(parts, (S::kSmem - kWeights) / (quads * 16u));
+        float4 oo[kEach];
+#pragma unroll
+        for (uint32_t k = 0; k < kEach; ++k) oo[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t j0 = 0; j0 < parts; j0 += fit) {
+          const uint32_t n = min(fit, parts - j0);
+          __syncthreads();  // the weights are there; the copies before have been used
+          for (uint32_t j = 0; j < n; ++j) {
+            const float* from = record(c0 + j0 + j) + kRecHeader;
+            for (uint32_t i = threadIdx.x; i < quads; i += kThreads)
+              cp_async16(smem_u32(stage + (j * quads + i) * 4u), from + i * 4u, true);
           }
-          store4(out + (static_cast<size_t>(u.b) * p.heads + head0 + h) * HD + d, oo);
+          cp_commit();
+          cp_wait<0>();
+          __syncthreads();
+#pragma unroll
+          for (uint32_t k = 0; k < kEach; ++k) {
+            const uint32_t i = k * kThreads + threadIdx.x;
+            if (i < quads) {
+              const uint32_t h = i / (HD / 4);
+              for (uint32_t j = 0; j < n; ++j) {
+                const float f = weight[h * kMaxCtas + j0 + j];
+                const float4 x = *reinterpret_cast<const float4*>(stage + (j * quads + i) * 4u);
+                oo[k].x += x.x * f;
+                oo[k].y += x.y * f;
+                oo[k].z += x.z * f;
+                oo[k].w += x.w * f;
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kEach; ++k) {
+          const uint32_t i = k * kThreads + threadIdx.x;
+          if (i < quads)
+            store4(out + (static_cast<size_t>(u.b) * p.heads + head0 + i / (HD / 4)) * HD + i % (HD / 4) * 4u, oo[k]);
         }
       }
     }
@@ -454,8 +490,7 @@ cudaError_t launch(const AttendParams& p, cudaStream_t s) {
     sms_of[dev].store(sms, std::memory_order_release);
   }
   const uint32_t ctas = static_cast<uint32_t>(sms) < kMaxCtas ? static_cast<uint32_t>(sms) : kMaxCtas;
-  decode_kernel<T, Q, HD, WARPS, STAGES, PAIR><<<ctas, WARPS * 32, smem, s>>>(p);
-  return cudaGetLastError();
+  return launch_early(decode_kernel<T, Q, HD, WARPS, STAGES, PAIR>, dim3(ctas), dim3(WARPS * 32), smem, s, p);
 }
 
 template <typename T, typename Q, bool PAIR>

@@ -391,6 +391,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     stop_word = never = 0u;
   }
 
+  pdl_wait();
   pdl_launch_dependents();  // the joining launch waits for this grid's end by itself
   if (threadIdx.x == 0) p_cuts(p)[blockIdx.x].parts = 0u;
 
@@ -1020,6 +1021,7 @@ __global__ void __launch_bounds__(256) prefill_join_kernel(const AttendParams p)
   __shared__ float weight[kMaxCtas][kJoinRows];
   __shared__ uint32_t bad_rows;
   pdl_wait();
+  pdl_launch_dependents();
   const Cut cut = p_cuts(p)[blockIdx.x];
   const uint32_t y0 = blockIdx.y * kJoinRows;  // first row within the unit
   if (cut.parts == 0u || y0 >= cut.rows) return;
@@ -1170,19 +1172,9 @@ cudaError_t launch(const AttendParams& p, cudaStream_t s) {
   AttendParams q = p;
   encode<T>(p, maps);
   q.align = maps.box ? maps.box : 1u;
-  prefill_kernel<T, HD><<<ctas, Shape<HD>::kThreads, Shape<HD>::kSmem, s>>>(q, maps);
-  e = cudaGetLastError();
+  e = launch_early(prefill_kernel<T, HD>, dim3(ctas), dim3(Shape<HD>::kThreads), Shape<HD>::kSmem, s, q, maps);
   if (e != cudaSuccess) return e;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, Shape<HD>::kRows / kJoinRows);
-  cfg.blockDim = dim3(256);
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, prefill_join_kernel<T, HD>, q);
+  return launch_early(prefill_join_kernel<T, HD>, dim3(ctas, Shape<HD>::kRows / kJoinRows), dim3(256), 0, s, q);
 }
 template <typename T>
 cudaError_t by_dim(const AttendParams& p, cudaStream_t s) {

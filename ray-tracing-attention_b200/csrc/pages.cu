@@ -37,6 +37,8 @@ __device__ __forceinline__ uint4 convert8<__nv_bfloat16, float>(const float* src
 
 template <typename T, typename X>
 __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
   const uint32_t lane = threadIdx.x & 31u;
   const uint64_t item = static_cast<uint64_t>(blockIdx.x) * 8u + (threadIdx.x >> 5);
   if (item >= static_cast<uint64_t>(p.rows) * p.c.kv_heads) return;
@@ -115,6 +117,8 @@ __device__ uint32_t list_free(const int32_t* refs, uint32_t pages, uint32_t want
 }
 
 __global__ void map_copy_kernel(MapArrays from, MapArrays to, uint32_t pages, uint32_t slots, uint64_t cells) {
+  pdl_wait();
+  pdl_launch_dependents();
   const uint64_t stride = static_cast<uint64_t>(gridDim.x) * blockDim.x;
   const uint64_t t = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   for (uint64_t i = t; i < cells; i += stride) to.table[i] = from.table[i];
@@ -123,6 +127,8 @@ __global__ void map_copy_kernel(MapArrays from, MapArrays to, uint32_t pages, ui
 }
 
 __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const PagesParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
   __shared__ uint64_t part[32];
   const Plan plan(p.plan, p.pages, p.slot_count);
   uint64_t total = 0;
@@ -170,6 +176,8 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const PagesParams
 // Claims the destinations, ranks the partly filled last pages, takes a page
 // for each; the launch after it shares the full pages and copies the rest.
 __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagesParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
   __shared__ uint64_t part[32];
   __shared__ uint32_t fault;
   const Plan plan(p.plan, p.pages, p.slot_count);
@@ -232,6 +240,8 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagesPara
 }
 
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagesParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
   __shared__ uint64_t part[32];
   const Plan plan(p.plan, p.pages, p.slot_count);
   uint64_t mine = 0, live;
@@ -277,6 +287,8 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagesP
 }
 
 __global__ void __launch_bounds__(kPlanThreads) copy_plan_kernel(const PagesParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
   const Plan plan(p.plan, p.pages, p.slot_count);
   for (uint32_t i = threadIdx.x; i < p.count; i += kPlanThreads) {
     const uint32_t s = p.a[i], d = p.b[i];
@@ -295,6 +307,8 @@ constexpr uint32_t kPiece = 4096;  // bytes one warp moves per step: eight 16-by
 
 template <int KIND>
 __global__ void __launch_bounds__(256) move_kernel(const PagesParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
   const Plan plan(p.plan, p.pages, p.slot_count);
   const uint32_t lane = threadIdx.x & 31u;
   const uint64_t warps = static_cast<uint64_t>(gridDim.x) * 8u;
@@ -368,6 +382,8 @@ __global__ void __launch_bounds__(256) move_kernel(const PagesParams p) {
 }
 
 __global__ void __launch_bounds__(256) free_kernel(const PagesParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
   __shared__ int32_t length;
   const int32_t slot = p.a[blockIdx.x];
   if (slot < 0 || static_cast<uint32_t>(slot) >= p.slot_count) {
@@ -412,14 +428,12 @@ cudaError_t launch_append(const AppendParams& p, int fmt, int in_fmt, cudaStream
   if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
   const dim3 grid(static_cast<uint32_t>(blocks));
   if (fmt == kF16 && in_fmt == kF32)
-    append_kernel<__half, float><<<grid, 256, 0, s>>>(p);
-  else if (fmt == kF16)
-    append_kernel<__half, __half><<<grid, 256, 0, s>>>(p);
-  else if (in_fmt == kF32)
-    append_kernel<__nv_bfloat16, float><<<grid, 256, 0, s>>>(p);
-  else
-    append_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, 256, 0, s>>>(p);
-  return cudaGetLastError();
+    return launch_early(append_kernel<__half, float>, grid, dim3(256), 0, s, p);
+  if (fmt == kF16)
+    return launch_early(append_kernel<__half, __half>, grid, dim3(256), 0, s, p);
+  if (in_fmt == kF32)
+    return launch_early(append_kernel<__nv_bfloat16, float>, grid, dim3(256), 0, s, p);
+  return launch_early(append_kernel<__nv_bfloat16, __nv_bfloat16>, grid, dim3(256), 0, s, p);
 }
 
 cudaError_t launch_map_copy(const MapArrays& from, const MapArrays& to, uint32_t pages, uint32_t slots,
@@ -427,38 +441,29 @@ cudaError_t launch_map_copy(const MapArrays& from, const MapArrays& to, uint32_t
   const uint64_t cells = static_cast<uint64_t>(slots) * width;
   const uint64_t most = cells > pages ? cells : pages;
   const uint64_t blocks = (most + 1023u) / 1024u;
-  map_copy_kernel<<<static_cast<uint32_t>(blocks < 592u ? (blocks ? blocks : 1u) : 592u), 256, 0, s>>>(from, to, pages, slots,
-                                                                                                  cells);
-  return cudaGetLastError();
+  return launch_early(map_copy_kernel, dim3(static_cast<uint32_t>(blocks < 592u ? (blocks ? blocks : 1u) : 592u)), dim3(256),
+                      0, s, from, to, pages, slots, cells);
 }
 cudaError_t launch_reserve(const PagesParams& p, cudaStream_t s) {
-  reserve_kernel<<<1, kPlanThreads, 0, s>>>(p);
-  return cudaGetLastError();
+  return launch_early(reserve_kernel, dim3(1), dim3(kPlanThreads), 0, s, p);
 }
 cudaError_t launch_fork(const PagesParams& p, cudaStream_t s) {
-  fork_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_early(fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p);
   if (e != cudaSuccess) return e;
-  move_kernel<kMoveFork><<<kMoveBlocks, 256, 0, s>>>(p);
-  return cudaGetLastError();
+  return launch_early(move_kernel<kMoveFork>, dim3(kMoveBlocks), dim3(256), 0, s, p);
 }
 cudaError_t launch_free(const PagesParams& p, cudaStream_t s) {
-  free_kernel<<<p.count, 256, 0, s>>>(p);
-  return cudaGetLastError();
+  return launch_early(free_kernel, dim3(p.count), dim3(256), 0, s, p);
 }
 cudaError_t launch_compact(const PagesParams& p, cudaStream_t s) {
-  compact_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_early(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p);
   if (e != cudaSuccess) return e;
-  move_kernel<kMoveCompact><<<kMoveBlocks, 256, 0, s>>>(p);
-  return cudaGetLastError();
+  return launch_early(move_kernel<kMoveCompact>, dim3(kMoveBlocks), dim3(256), 0, s, p);
 }
 cudaError_t launch_copy(const PagesParams& p, cudaStream_t s) {
-  copy_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_early(copy_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p);
   if (e != cudaSuccess) return e;
-  move_kernel<kMoveCopy><<<kMoveBlocks, 256, 0, s>>>(p);
-  return cudaGetLastError();
+  return launch_early(move_kernel<kMoveCopy>, dim3(kMoveBlocks), dim3(256), 0, s, p);
 }
 
 }  // namespace paged

@@ -114,7 +114,7 @@ class PagedCache:
 
     def _out(self, q: torch.Tensor, out: torch.Tensor | None, lse: bool):
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=self.device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous():
             raise ValueError("out must be contiguous and have q's shape, type and device")
         return out, torch.empty(q.shape[:2], dtype=torch.float32, device=self.device) if lse else None
@@ -247,7 +247,7 @@ class PagedCache:
     def _stream(self) -> int:
         if torch.cuda.current_device() != self.device.index:
             raise ValueError(f"the cache lives on {self.device}, another device is current")
-        return torch.cuda.current_stream().cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.device.index)  # current_stream() builds an object: 3 us
 
 
 __all__ = ["PageMap", "PagedCache"]
