@@ -306,13 +306,12 @@ RTA_API rta_status rta_workspace_error(const void* workspace, size_t workspace_b
  * (0: free).  width * page_size must stay below 2^31.
  *
  * Every call takes a workspace of rta_paged_workspace_bytes() bytes, 16-byte
- * aligned, that the caller zeroes ONCE before its first use (the attention
- * calls leave their counters zeroed).  Calls that share a workspace, or a map
+ * aligned, whose first word the caller zeroes ONCE before its first use.  Calls that share a workspace, or a map
  * that one of them writes, must be ordered on one stream.  Device-side checks
  * accumulate in the workspace's first word, read by rta_workspace_error and
  * cleared by zeroing that word: 4 = the map names a page outside the pool or
  * one without references, 8 = not enough free pages, 16 = a bad slot or count;
- * 1 = a bounded device-side wait expired (then zero the whole workspace).
+ * 1 = a bounded device-side wait expired.
  * `slots` (device, `batch` entries) names the sequences of a call; NULL means
  * slots 0 .. batch - 1. */
 typedef struct rta_page_pool {

@@ -58,7 +58,6 @@ struct AttendParams {
   void* out;
   float* lse;
   uint32_t* err;
-  uint32_t* counters;  // [kMaxCtas], zero between calls
   void* cuts;  // [kMaxCtas] units that are cut, of kCutBytes each
   float* records;
 };

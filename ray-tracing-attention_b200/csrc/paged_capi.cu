@@ -40,11 +40,9 @@ const char* bad_map(const rta_page_pool* p, const rta_page_map* m) {
   return nullptr;
 }
 
-// Workspace: error word and padding, the counters and descriptions of split
-// units, then either the split records of an attention call or the plan of a
-// bookkeeping call.
-constexpr size_t kErr = 256, kCounters = (paged::kMaxCtas * 4u + 255u) / 256u * 256u,
-                 kCuts = (paged::kMaxCtas * paged::kCutBytes + 255u) / 256u * 256u, kBody = kErr + kCounters + kCuts;
+// Workspace: error word and padding, the descriptions of cut units, then either
+// their records (an attention call) or the plan of a bookkeeping call.
+constexpr size_t kErr = 256, kCuts = (paged::kMaxCtas * paged::kCutBytes + 255u) / 256u * 256u, kBody = kErr + kCuts;
 size_t workspace_bytes_of(const rta_page_pool* p, const rta_page_map* m) {
   size_t body = paged::decode_record_bytes();
   if (paged::prefill_record_bytes() > body) body = paged::prefill_record_bytes();
@@ -84,12 +82,11 @@ paged::View view(const rta_page_pool* p, const rta_page_map* m, uint32_t layer, 
 }
 
 struct Workspace {
-  uint32_t *err, *counters;
+  uint32_t* err;
   void *cuts, *body;
   explicit Workspace(void* ws)
       : err(static_cast<uint32_t*>(ws)),
-        counters(reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(ws) + kErr)),
-        cuts(static_cast<uint8_t*>(ws) + kErr + kCounters),
+        cuts(static_cast<uint8_t*>(ws) + kErr),
         body(static_cast<uint8_t*>(ws) + kBody) {}
 };
 
@@ -128,7 +125,6 @@ const char* attend_params(const rta_page_pool* pool, const rta_page_map* map, ui
   p.out = out;
   p.lse = lse;
   p.err = w.err;
-  p.counters = w.counters;
   p.cuts = w.cuts;
   p.records = static_cast<float*>(w.body);
   p.starts = nullptr;

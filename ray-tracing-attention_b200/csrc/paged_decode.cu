@@ -11,7 +11,13 @@
 // every CTA takes an equal contiguous range of it, whatever the lengths are
 // (they are read on the device, so a step graph replays with them).  A unit
 // that lies inside one range is written at once; one that is cut leaves a
-// record per CTA, and the CTA that arrives last joins them in CTA order.
+// record per CTA, which a second launch joins, a CTA per head.
+//
+// The kernel is bound by HBM, so everything else has to stay out of the way of
+// the copies: each warp owns a ring of tiles that it fills by 16-byte copies
+// two tiles ahead, across the ends of units; the page of a tile is looked up
+// one tile before its copies; the next unit's queries are copied while this
+// one's tiles are read.
 #include <atomic>
 #include <mutex>
 
@@ -27,6 +33,16 @@ constexpr uint32_t kRecHeader = 2 * kHeadsMax;  // m and z of a record's heads
 
 __host__ __device__ constexpr uint32_t record_floats(uint32_t hd) { return kRecHeader + kHeadsMax * hd; }
 
+// A unit that begins in a CTA's range and ends in another's: at most one per CTA.
+struct Cut {
+  uint32_t parts;   // CTAs that hold a part of it, from this one on; 0: no such unit
+  uint32_t second;  // this CTA's record of it is its second (the others': their first)
+  uint32_t b, head0, heads;
+};
+__device__ __forceinline__ Cut& cut_of(const AttendParams& p, uint32_t cta) {
+  return *reinterpret_cast<Cut*>(static_cast<uint8_t*>(p.cuts) + cta * kCutBytes);
+}
+
 // PAIR: rows g and g + 8 of the MMA are the two 16-bit halves of head g's
 // operand (x = T(x) + T(x - T(x))), so weights, and fp32 queries, enter with
 // about twice the bits of T at no extra MMA; up to 8 heads per unit.
@@ -38,10 +54,11 @@ struct Shape {
   static constexpr uint32_t kChunks = kRow / 16;       // 16-byte chunks per row
   static constexpr uint32_t kStage = 2 * kTile * kRow; // K rows then V rows
   static constexpr uint32_t kRing = WARPS * STAGES * kStage;
-  static constexpr uint32_t kJoin = WARPS * kHeads * (HD + 2) * 4;
-  static constexpr uint32_t kSmem = (kRing > kJoin ? kRing : kJoin) > kMaxCtas * kHeadsMax * 4
-                                        ? (kRing > kJoin ? kRing : kJoin)
-                                        : kMaxCtas * kHeadsMax * 4;
+  static constexpr uint32_t kQueries = kHeads * HD * sizeof(Q);  // one unit's
+  // the warps' results are added a part of the dimensions at a time, in 16 KB
+  static constexpr uint32_t kPasses = WARPS * kHeads * HD * 4 / 16384 ? WARPS * kHeads * HD * 4 / 16384 : 1;
+  static constexpr uint32_t kJoin = WARPS * kHeads * (HD / kPasses) * 4;
+  static constexpr uint32_t kSmem = kRing + 2 * kQueries + kJoin;
 };
 
 struct Unit {  // one (sequence, K/V head, head block)
@@ -60,14 +77,11 @@ __device__ __forceinline__ void visible(const AttendParams& p, const Sequence& s
   u.tiles = (u.seen + kTile - 1u) / kTile;
 }
 
-template <typename Q>
-__device__ __forceinline__ float load_q(const Q* q);
-template <>
-__device__ __forceinline__ float load_q<float>(const float* q) { return *q; }
-template <>
-__device__ __forceinline__ float load_q<__half>(const __half* q) { return __half2float(*q); }
-template <>
-__device__ __forceinline__ float load_q<__nv_bfloat16>(const __nv_bfloat16* q) { return __bfloat162float(*q); }
+__device__ __forceinline__ float2 two(const float* q) { return *reinterpret_cast<const float2*>(q); }
+__device__ __forceinline__ float2 two(const __half* q) { return __half22float2(*reinterpret_cast<const __half2*>(q)); }
+__device__ __forceinline__ float2 two(const __nv_bfloat16* q) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(q));
+}
 
 __device__ __forceinline__ void store4(float* dst, float4 v) { *reinterpret_cast<float4*>(dst) = v; }
 __device__ __forceinline__ void store4(__half* dst, float4 v) {
@@ -87,14 +101,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
   __shared__ uint32_t found_b;
   __shared__ uint64_t found_at;
   __shared__ float join_m[WARPS][S::kHeads], join_z[WARPS][S::kHeads];
-  __shared__ uint32_t last_arrival;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t4 = lane & 3u;
   const uint32_t blocks = (p.group + S::kHeads - 1u) / S::kHeads;  // head blocks per K/V head
   const uint32_t per_seq = p.c.kv_heads * blocks;
   Q* const out = static_cast<Q*>(p.out);
-
   pdl_wait();
   pdl_launch_dependents();
+  if (threadIdx.x == 0) cut_of(p, blockIdx.x).parts = 0u;
 
   // ---- the list of tiles: its length, and this CTA's range -----------------
   uint64_t total = 0, own = 0, own_upto = 0;  // this thread's (last) sequence in the list
@@ -151,71 +164,139 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
     }
     __syncthreads();
   }
-  Unit u;
-  u.b = found_b;
-  visible(p, sequence(p.c, u.b, nullptr), u);
-  u.pr = static_cast<uint32_t>(found_at / u.tiles);
-  uint32_t a = static_cast<uint32_t>(found_at % u.tiles);  // first tile of the segment in the unit
+  // ---- segments: tiles [a, e) of one unit, one after the other --------------
+  struct Segment {
+    Unit u;
+    uint32_t a, e;
+  };
+  uint64_t at = begin;  // place in the list behind the segments taken so far
+  const auto take = [&](Segment& s) {  // s.u is set: its tiles from s.a on that are this CTA's
+    s.e = static_cast<uint32_t>(min(static_cast<uint64_t>(s.u.tiles), s.a + (end - at)));
+    at += s.e - s.a;
+  };
+  const auto follow = [&](const Segment& s, Segment& next) {  // false: there is none
+    if (at >= end) return false;
+    next.u = s.u;
+    if (++next.u.pr == per_seq) {
+      next.u.pr = 0;
+      do visible(p, sequence(p.c, ++next.u.b, nullptr), next.u);
+      while (next.u.tiles == 0u);
+    }
+    next.a = 0;
+    take(next);
+    return true;
+  };
+  const auto first_head = [&](const Unit& u) { return u.pr / blocks * p.group + u.pr % blocks * S::kHeads; };
+  const auto heads_of = [&](const Unit& u) { return min(S::kHeads, p.group - u.pr % blocks * S::kHeads); };
+  const auto copy_queries = [&](const Unit& u, uint32_t to) {  // rows past the unit's heads become zeros
+    constexpr uint32_t kPer = HD * sizeof(Q) / 16;
+    const uint32_t heads = heads_of(u);
+    const Q* q = static_cast<const Q*>(p.q) + static_cast<size_t>(u.b) * p.q_row + static_cast<size_t>(first_head(u)) * p.q_head;
+    const uint32_t dst = smem_u32(smem + S::kRing + to * S::kQueries);
+    for (uint32_t i = threadIdx.x; i < S::kHeads * kPer; i += kThreads) {
+      const uint32_t h = i / kPer;
+      cp_async16(dst + i * 16u, q + (h < heads ? h * p.q_head : 0u) + i % kPer * (16u / sizeof(Q)), h < heads);
+    }
+  };
 
+  Segment cur, next;
+  cur.u.b = found_b;
+  visible(p, sequence(p.c, cur.u.b, nullptr), cur.u);
+  cur.u.pr = static_cast<uint32_t>(found_at / cur.u.tiles);
+  cur.a = static_cast<uint32_t>(found_at % cur.u.tiles);
+  take(cur);
+  next = cur;
+
+  // ---- this warp's tiles: warp, warp + WARPS, .. of every segment -----------
   const uint32_t ring = smem_u32(smem) + warp * STAGES * S::kStage;
-  bool first_segment = true;
-  for (uint64_t t = begin; t < end;) {
-    const uint32_t e = static_cast<uint32_t>(min(static_cast<uint64_t>(u.tiles), a + (end - t)));
-    const uint32_t kv = u.pr / blocks, head0 = kv * p.group + (u.pr % blocks) * S::kHeads;
-    const uint32_t heads = min(S::kHeads, p.group - (u.pr % blocks) * S::kHeads);
+  uint32_t issued = 0, consumed = 0;  // tiles; tile n lies in stage n % STAGES
+  // the next tile to issue: lane r < 16 holds the page of its position r and
+  // the bytes inside the page
+  bool in_next = false, have = false;
+  uint32_t tile = cur.a + warp;
+  int32_t page = -1;
+  uint32_t real = 0;
+  uint64_t inside = 0;
+  const auto look = [&](const Segment& s) {
+    const uint32_t n = tile * kTile + (lane & 15u);
+    real = n < s.u.seen ? 1u : 0u;
+    const uint32_t pos = n < s.u.first ? n : n + s.u.skip;
+    const uint32_t j = real ? page_of(p.c, pos) : 0u;
+    page = real ? p.c.table[static_cast<size_t>(s.u.slot) * p.c.width + j] : 0;
+    inside = static_cast<uint64_t>(pos - j * p.c.page_size) * p.c.pos_bytes + static_cast<uint64_t>(s.u.pr / blocks) * p.c.head_bytes;
+  };
+  const auto find = [&](bool more) {  // the tile at or after `tile`, in this segment or the next
+    have = false;
+    if (!in_next) {
+      if (tile < cur.e) {
+        have = true;
+        look(cur);
+        return;
+      }
+      if (!more) return;
+      in_next = true;
+      tile = next.a + warp;
+    }
+    if (tile < next.e) {
+      have = true;
+      look(next);
+    }
+  };
+  const auto issue = [&](bool more) {
+    const bool good = static_cast<uint32_t>(page) < p.c.pages;
+    if (real && !good) atomicOr(p.err, RTA_DEVERR_PAGE);
+    const uint32_t ok = real && good ? 1u : 0u;  // 0: the position becomes zeros
+    const uint64_t off = ok ? static_cast<uint64_t>(static_cast<uint32_t>(page)) * p.c.page_bytes + inside : 0u;
+    constexpr uint32_t kPer = 32 / S::kChunks;  // rows per warp instruction
+    const uint32_t st = ring + issued % STAGES * S::kStage;
+#pragma unroll
+    for (uint32_t r0 = 0; r0 < kTile; r0 += kPer) {
+      const uint32_t r = r0 + lane / S::kChunks, c = lane % S::kChunks;
+      const uint64_t o = __shfl_sync(0xffffffffu, off, r) + c * 16u;
+      const bool on = __shfl_sync(0xffffffffu, ok, r) != 0u;
+      const uint32_t dst = st + r * S::kRow + ((c ^ (r & 7u)) << 4);
+      cp_async16(dst, p.c.k + o, on);
+      cp_async16(dst + kTile * S::kRow, p.c.v + o, on);
+    }
+    cp_commit();
+    ++issued;
+    tile += WARPS;
+    find(more);
+  };
 
-    // One tile's rows: lane r < 16 looks position r up, then every lane copies
-    // its 16-byte chunks; what lies past the visible positions becomes zeros.
-    const auto issue = [&](uint32_t i, uint32_t stage) {
-      uint64_t off = 0;
-      uint32_t ok = 0;
-      const uint32_t at = i * kTile + (lane & 15u);
-      if (i < e && at < u.seen) {
-        ok = locate(p.c, u.slot, at < u.first ? at : at + u.skip, off) ? 1u : 0u;
-        if (!ok) atomicOr(p.err, RTA_DEVERR_PAGE);
-        off += static_cast<uint64_t>(kv) * p.c.head_bytes;
-      }
-      if (i < e) {
-        constexpr uint32_t kPer = 32 / S::kChunks;  // rows per warp instruction
-        const uint32_t st = ring + stage * S::kStage;
-#pragma unroll
-        for (uint32_t r0 = 0; r0 < kTile; r0 += kPer) {
-          const uint32_t r = r0 + lane / S::kChunks, c = lane % S::kChunks;
-          const uint64_t o = __shfl_sync(0xffffffffu, off, r) + c * 16u;
-          const bool real = __shfl_sync(0xffffffffu, ok, r) != 0u;
-          const uint32_t dst = st + r * S::kRow + ((c ^ (r & 7u)) << 4);
-          cp_async16(dst, p.c.k + o, real);
-          cp_async16(dst + kTile * S::kRow, p.c.v + o, real);
-        }
-      }
-      cp_commit();
-    };
-#pragma unroll
-    for (uint32_t s = 0; s + 1u < STAGES; ++s) issue(a + warp + s * WARPS, s);
+  find(false);
+  copy_queries(cur.u, 0);
+  bool more = follow(cur, next);
+  if (!have) find(more);
+  while (have && issued < STAGES - 1u) issue(more);
+  if (issued == 0u) cp_commit();
+  cp_wait<0>();
+  __syncthreads();  // the queries are there
+  for (uint32_t segment = 0;; ++segment) {
+    const Unit u = cur.u;
+    const uint32_t a = cur.a, e = cur.e, head0 = first_head(u), heads = heads_of(u);
+    if (more) copy_queries(next.u, (segment + 1u) & 1u);  // part of the next group of copies
 
     // Query fragments (A operand: rows are heads, k is the dimension).
     uint32_t qa[kSteps][4];
     {
-      const Q* qb = static_cast<const Q*>(p.q) + static_cast<size_t>(u.b) * p.q_row + static_cast<size_t>(head0) * p.q_head;
-      const Q* q0 = qb + static_cast<size_t>(g) * p.q_head;
-      const Q* q1 = qb + static_cast<size_t>(g + 8u) * p.q_head;
-      const bool on0 = g < heads, on1 = !PAIR && g + 8u < heads;
+      const Q* q0 = reinterpret_cast<const Q*>(smem + S::kRing + (segment & 1u) * S::kQueries) + g * HD + 2u * t4;
 #pragma unroll
       for (uint32_t kk = 0; kk < kSteps; ++kk)
 #pragma unroll
         for (uint32_t h = 0; h < 2u; ++h) {
-          const uint32_t d = kk * 16u + h * 8u + 2u * t4;
-          const float x0 = on0 ? load_q<Q>(q0 + d) : 0.f, x1 = on0 ? load_q<Q>(q0 + d + 1u) : 0.f;
-          qa[kk][2u * h] = N::pack(x0, x1);
+          const float2 x = two(q0 + kk * 16u + h * 8u);
+          qa[kk][2u * h] = N::pack(x.x, x.y);
           if (PAIR) {
             if (sizeof(Q) == 4) {
               const float2 hi = N::unpack(qa[kk][2u * h]);
-              qa[kk][2u * h + 1u] = N::pack(x0 - hi.x, x1 - hi.y);
+              qa[kk][2u * h + 1u] = N::pack(x.x - hi.x, x.y - hi.y);
             } else {
               qa[kk][2u * h + 1u] = 0u;
             }
           } else {
-            qa[kk][2u * h + 1u] = N::pack(on1 ? load_q<Q>(q1 + d) : 0.f, on1 ? load_q<Q>(q1 + d + 1u) : 0.f);
+            const float2 y = two(q0 + 8 * HD + kk * 16u + h * 8u);
+            qa[kk][2u * h + 1u] = N::pack(y.x, y.y);
           }
         }
     }
@@ -228,12 +309,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
 #pragma unroll
     for (int r = 0; r < kRows; ++r) m[r] = -INFINITY, z[r] = 0.f;
 
-    uint32_t stage = 0;
     for (uint32_t i = a + warp; i < e; i += WARPS) {
-      issue(i + (STAGES - 1) * WARPS, stage == 0u ? STAGES - 1u : stage - 1u);
-      cp_wait<STAGES - 1>();
+      while (have && issued < consumed + STAGES) issue(more);
+      if (issued == consumed + STAGES)
+        cp_wait<STAGES - 1>();
+      else
+        cp_wait<0>();
       __syncwarp();
-      const uint32_t st = ring + stage * S::kStage;
+      const uint32_t st = ring + consumed % STAGES * S::kStage;
       // scores: two 8-position columns, even and odd dimension steps apart
       float sc[2][2][4];
 #pragma unroll
@@ -319,13 +402,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
         }
       }
       __syncwarp();
-      stage = stage + 1u == STAGES ? 0u : stage + 1u;
+      ++consumed;
     }
-    cp_wait<0>();
 
     // ---- add the warps of this CTA -----------------------------------------
-    __syncthreads();  // every warp is done with the ring
-    float* const join = reinterpret_cast<float*>(smem);  // [warp][head][HD]
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       z[r] += __shfl_xor_sync(0xffffffffu, z[r], 1);
@@ -335,138 +415,158 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
         join_z[warp][g + 8 * r] = z[r];
       }
     }
-#pragma unroll
-    for (int j = 0; j < HD / 8; ++j) {
-      float* row = join + (warp * S::kHeads + g) * HD + j * 8 + 2u * t4;
-      if (PAIR) {
-        *reinterpret_cast<float2*>(row) = make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3]);
-      } else {
-        *reinterpret_cast<float2*>(row) = make_float2(o[j][0], o[j][1]);
-        *reinterpret_cast<float2*>(row + 8 * HD) = make_float2(o[j][2], o[j][3]);
-      }
-    }
-    __syncthreads();
-    const uint64_t unit0 = t - a, unit1 = unit0 + u.tiles;  // the unit's tiles in the list
     const bool whole = a == 0u && e == u.tiles;
-    float* const rec = p.records + static_cast<size_t>(blockIdx.x * 2u + (first_segment ? 0u : 1u)) * record_floats(HD);
-    for (uint32_t i = threadIdx.x; i < heads * (HD / 4); i += kThreads) {
-      const uint32_t h = i / (HD / 4), d = i % (HD / 4) * 4u;
-      float mm = -INFINITY;
+    float* const rec = p.records + static_cast<size_t>(blockIdx.x * 2u + (segment ? 1u : 0u)) * record_floats(HD);
+    float* const join = reinterpret_cast<float*>(smem + S::kRing + 2 * S::kQueries);  // [warp][head][dimensions of a pass]
+    constexpr uint32_t kDims = HD / S::kPasses;
+    cp_commit();
+    cp_wait<0>();  // the next unit's queries, and its first tiles, are there
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, join_m[w][h]);
-      const float base = mm == -INFINITY ? 0.f : mm;
-      float zz = 0.f;
-      float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t pass = 0; pass < S::kPasses; ++pass) {
+      if (pass) __syncthreads();
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float f = exp2f(join_m[w][h] - base);
-        const float4 x = *reinterpret_cast<const float4*>(join + (w * S::kHeads + h) * HD + d);
-        zz += join_z[w][h] * f;
-        oo.x += x.x * f;
-        oo.y += x.y * f;
-        oo.z += x.z * f;
-        oo.w += x.w * f;
-      }
-      if (whole) {
-        const float inv = 1.f / zz;
-        const size_t row = static_cast<size_t>(u.b) * p.heads + head0 + h;
-        store4(out + row * HD + d, make_float4(oo.x * inv, oo.y * inv, oo.z * inv, oo.w * inv));
-        if (p.lse && d == 0u) p.lse[row] = (mm - N::kShift + log2f(zz)) * kLn2;
-      } else {
-        store4(rec + kRecHeader + h * HD + d, oo);
-        if (d == 0u) {
-          rec[h] = mm;
-          rec[kHeadsMax + h] = zz;
+      for (uint32_t j = 0; j < kDims / 8u; ++j) {
+        const float(&x)[4] = o[pass * (kDims / 8u) + j];
+        float* row = join + (warp * S::kHeads + g) * kDims + j * 8u + 2u * t4;
+        if (PAIR) {
+          *reinterpret_cast<float2*>(row) = make_float2(x[0] + x[2], x[1] + x[3]);
+        } else {
+          *reinterpret_cast<float2*>(row) = make_float2(x[0], x[1]);
+          *reinterpret_cast<float2*>(row + 8u * kDims) = make_float2(x[2], x[3]);
         }
-      }
-    }
-    if (!whole) {
-      // ---- join the unit's records: the CTA that arrives last ----------------
-      const uint32_t c0 = owner(unit0), c1 = owner(unit1 - 1u), parts = c1 - c0 + 1u;
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        last_arrival = atomicAdd(&p.counters[c0], 1u) == parts - 1u ? 1u : 0u;
-        if (last_arrival) p.counters[c0] = 0u;
       }
       __syncthreads();
-      if (last_arrival) {
-        __threadfence();
-        // a CTA's record of this unit is its second one only when the unit
-        // begins inside the CTA's range
-        const auto record = [&](uint32_t c) {
-          const bool second = c == c0 && total * c0 / ctas != unit0;
-          return p.records + static_cast<size_t>(c * 2u + (second ? 1u : 0u)) * record_floats(HD);
-        };
-        float* const weight = reinterpret_cast<float*>(smem);  // [head][part]
-        for (uint32_t h = warp; h < heads; h += WARPS) {
-          float mm = -INFINITY, zz = 0.f;
-          for (uint32_t j = lane; j < parts; j += 32u) mm = fmaxf(mm, __ldcg(record(c0 + j) + h));
-          mm = warp_max(mm);
-          const float base = mm == -INFINITY ? 0.f : mm;
-          for (uint32_t j = lane; j < parts; j += 32u) {
-            const float f = exp2f(__ldcg(record(c0 + j) + h) - base);
-            zz += f * __ldcg(record(c0 + j) + kHeadsMax + h);
-            weight[h * kMaxCtas + j] = f;
-          }
-          zz = warp_sum(zz);
-          __syncwarp();
-          for (uint32_t j = lane; j < parts; j += 32u) weight[h * kMaxCtas + j] /= zz;
-          if (p.lse && lane == 0u)
-            p.lse[static_cast<size_t>(u.b) * p.heads + head0 + h] = (mm - N::kShift + log2f(zz)) * kLn2;
+      for (uint32_t i = threadIdx.x; i < heads * (kDims / 4u); i += kThreads) {
+        const uint32_t h = i / (kDims / 4u), dp = i % (kDims / 4u) * 4u, d = pass * kDims + dp;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, join_m[w][h]);
+        const float base = mm == -INFINITY ? 0.f : mm;
+        float zz = 0.f;
+        float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          const float f = exp2f(join_m[w][h] - base);
+          const float4 x = *reinterpret_cast<const float4*>(join + (w * S::kHeads + h) * kDims + dp);
+          zz += join_z[w][h] * f;
+          oo.x += x.x * f;
+          oo.y += x.y * f;
+          oo.z += x.z * f;
+          oo.w += x.w * f;
         }
-        // the records' O come through shared memory, as many at a time as fit:
-        // all their 16-byte copies are in flight at once
-        constexpr uint32_t kWeights = kMaxCtas * kHeadsMax * 4, kEach = (S::kHeads * (HD / 4) + kThreads - 1u) / kThreads;
-        float* const stage = reinterpret_cast<float*>(smem + kWeights);
-        const uint32_t quads = heads * (HD / 4), fit = min(parts, (S::kSmem - kWeights) / (quads * 16u));
-        float4 oo[kEach];
-#pragma unroll
-        for (uint32_t k = 0; k < kEach; ++k) oo[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (uint32_t j0 = 0; j0 < parts; j0 += fit) {
-          const uint32_t n = min(fit, parts - j0);
-          __syncthreads();  // the weights are there; the copies before have been used
-          for (uint32_t j = 0; j < n; ++j) {
-            const float* from = record(c0 + j0 + j) + kRecHeader;
-            for (uint32_t i = threadIdx.x; i < quads; i += kThreads)
-              cp_async16(smem_u32(stage + (j * quads + i) * 4u), from + i * 4u, true);
+        if (whole) {
+          const float inv = 1.f / zz;
+          const size_t row = static_cast<size_t>(u.b) * p.heads + head0 + h;
+          store4(out + row * HD + d, make_float4(oo.x * inv, oo.y * inv, oo.z * inv, oo.w * inv));
+          if (p.lse && d == 0u) p.lse[row] = (mm - N::kShift + log2f(zz)) * kLn2;
+        } else {
+          store4(rec + kRecHeader + h * HD + d, oo);
+          if (d == 0u) {
+            rec[h] = mm;
+            rec[kHeadsMax + h] = zz;
           }
-          cp_commit();
-          cp_wait<0>();
-          __syncthreads();
-#pragma unroll
-          for (uint32_t k = 0; k < kEach; ++k) {
-            const uint32_t i = k * kThreads + threadIdx.x;
-            if (i < quads) {
-              const uint32_t h = i / (HD / 4);
-              for (uint32_t j = 0; j < n; ++j) {
-                const float f = weight[h * kMaxCtas + j0 + j];
-                const float4 x = *reinterpret_cast<const float4*>(stage + (j * quads + i) * 4u);
-                oo[k].x += x.x * f;
-                oo[k].y += x.y * f;
-                oo[k].z += x.z * f;
-                oo[k].w += x.w * f;
-              }
-            }
-          }
-        }
-#pragma unroll
-        for (uint32_t k = 0; k < kEach; ++k) {
-          const uint32_t i = k * kThreads + threadIdx.x;
-          if (i < quads)
-            store4(out + (static_cast<size_t>(u.b) * p.heads + head0 + i / (HD / 4)) * HD + i % (HD / 4) * 4u, oo[k]);
         }
       }
     }
-    __syncthreads();  // the ring is free again
-    first_segment = false;
-    t += e - a;
-    a = 0;
-    if (t < end && ++u.pr == per_seq) {
-      u.pr = 0;
-      do visible(p, sequence(p.c, ++u.b, nullptr), u);
-      while (u.tiles == 0u);
+    if (!whole && a == 0u && threadIdx.x == 0) {  // what the second launch has to know
+      Cut& cut = cut_of(p, blockIdx.x);
+      // the segments taken so far end at `at`, the last of them being this one or the next
+      const uint64_t unit0 = (more ? at - (next.e - next.a) : at) - e;
+      cut.parts = owner(unit0 + u.tiles - 1u) - blockIdx.x + 1u;
+      cut.second = segment ? 1u : 0u;
+      cut.b = u.b;
+      cut.head0 = head0;
+      cut.heads = heads;
     }
+    if (!more) break;
+    __syncthreads();  // join and its sums have been read; the next queries are seen by all
+    cur = next;
+    if (in_next)
+      in_next = false;
+    else
+      tile = cur.a + warp;
+    more = follow(cur, next);
+    if (!have) find(more);
+  }
+}
+
+// Joins the records of a cut unit: blockIdx.x is the CTA in whose range it
+// begins, blockIdx.y the head.  o = sum_j 2^(m_j - max m) o_j over
+// sum_j 2^(m_j - max m) z_j.
+template <typename T, typename Q, int HD>
+__global__ void __launch_bounds__(256) decode_join_kernel(const AttendParams p) {
+  using N = Num<T>;
+  constexpr uint32_t kQuads = HD / 4, kGroups = 256 / kQuads;
+  __shared__ float weight[kMaxCtas];
+  __shared__ float4 sums[kGroups][kQuads];
+  pdl_wait();
+  pdl_launch_dependents();
+  const Cut cut = cut_of(p, blockIdx.x);
+  const uint32_t h = blockIdx.y;
+  if (h >= cut.heads || cut.parts == 0u) return;
+  const auto record = [&](uint32_t j) {
+    return p.records + static_cast<size_t>((blockIdx.x + j) * 2u + (j == 0u ? cut.second : 0u)) * record_floats(HD);
+  };
+  const size_t row = static_cast<size_t>(cut.b) * p.heads + cut.head0 + h;
+  if (threadIdx.x < 32u) {
+    constexpr uint32_t kOwn = kMaxCtas / 32u;
+    float m[kOwn], z[kOwn], mm = -INFINITY, zz = 0.f;
+#pragma unroll
+    for (uint32_t k = 0; k < kOwn; ++k) {
+      const uint32_t j = k * 32u + threadIdx.x;
+      m[k] = j < cut.parts ? record(j)[h] : -INFINITY;
+      z[k] = j < cut.parts ? record(j)[kHeadsMax + h] : 0.f;
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < kOwn; ++k) mm = fmaxf(mm, m[k]);
+    mm = warp_max(mm);
+    const float base = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+    for (uint32_t k = 0; k < kOwn; ++k) {
+      m[k] = exp2f(m[k] - base);
+      zz += m[k] * z[k];
+    }
+    zz = warp_sum(zz);
+#pragma unroll
+    for (uint32_t k = 0; k < kOwn; ++k) weight[k * 32u + threadIdx.x] = m[k] / zz;
+    if (p.lse && threadIdx.x == 0u) p.lse[row] = (mm - N::kShift + log2f(zz)) * kLn2;
+  }
+  const uint32_t d = threadIdx.x % kQuads, group = threadIdx.x / kQuads;
+  constexpr uint32_t kAhead = 8;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f), x[kAhead];
+  const auto load = [&](uint32_t j0) {
+#pragma unroll
+    for (uint32_t k = 0; k < kAhead; ++k) {
+      const uint32_t j = j0 + k * kGroups;
+      x[k] = j < cut.parts ? *reinterpret_cast<const float4*>(record(j) + kRecHeader + h * HD + d * 4u) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  };
+  load(group);
+  __syncthreads();  // the weights are there
+  for (uint32_t j0 = group; j0 < cut.parts; j0 += kGroups * kAhead) {
+    if (j0 != group) load(j0);
+#pragma unroll
+    for (uint32_t k = 0; k < kAhead; ++k) {
+      const uint32_t j = j0 + k * kGroups;
+      const float f = j < cut.parts ? weight[j] : 0.f;
+      o.x += x[k].x * f;
+      o.y += x[k].y * f;
+      o.z += x[k].z * f;
+      o.w += x[k].w * f;
+    }
+  }
+  sums[group][d] = o;
+  __syncthreads();
+  if (group == 0u) {
+#pragma unroll
+    for (uint32_t k = 1; k < kGroups; ++k) {
+      const float4 x = sums[k][d];
+      o.x += x.x;
+      o.y += x.y;
+      o.z += x.z;
+      o.w += x.w;
+    }
+    store4(static_cast<Q*>(p.out) + row * HD + d * 4u, o);
   }
 }
 
@@ -490,7 +590,10 @@ cudaError_t launch(const AttendParams& p, cudaStream_t s) {
     sms_of[dev].store(sms, std::memory_order_release);
   }
   const uint32_t ctas = static_cast<uint32_t>(sms) < kMaxCtas ? static_cast<uint32_t>(sms) : kMaxCtas;
-  return launch_early(decode_kernel<T, Q, HD, WARPS, STAGES, PAIR>, dim3(ctas), dim3(WARPS * 32), smem, s, p);
+  e = launch_early(decode_kernel<T, Q, HD, WARPS, STAGES, PAIR>, dim3(ctas), dim3(WARPS * 32), smem, s, p);
+  if (e != cudaSuccess) return e;
+  const uint32_t heads = Shape<T, Q, HD, WARPS, STAGES, PAIR>::kHeads;
+  return launch_early(decode_join_kernel<T, Q, HD>, dim3(ctas, p.group < heads ? p.group : heads), dim3(256), 0, s, p);
 }
 
 template <typename T, typename Q, bool PAIR>

@@ -80,7 +80,9 @@ struct Cut {
   int32_t past;
   uint32_t firsts, low, high;
 };
-__device__ __forceinline__ Cut* p_cuts(const AttendParams& p) { return static_cast<Cut*>(p.cuts); }
+__device__ __forceinline__ Cut& cut_of(const AttendParams& p, uint32_t cta) {
+  return *reinterpret_cast<Cut*>(static_cast<uint8_t*>(p.cuts) + cta * kCutBytes);
+}
 
 // K and V as TMA sees them: (dimension, position in the page, head, page), or
 // head before position where that is the order of the strides.
@@ -393,7 +395,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
 
   pdl_wait();
   pdl_launch_dependents();  // the joining launch waits for this grid's end by itself
-  if (threadIdx.x == 0) p_cuts(p)[blockIdx.x].parts = 0u;
+  if (threadIdx.x == 0) cut_of(p, blockIdx.x).parts = 0u;
 
   // ---- the list of blocks and this CTA's range ------------------------------
   uint64_t total = 0;
@@ -720,7 +722,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
           }
         }
         if (a == 0u && threadIdx.x == 0u) {  // this unit begins here: what the second launch has to know of it
-          Cut& cut = p_cuts(p)[blockIdx.x];
+          Cut& cut = cut_of(p, blockIdx.x);
           cut.parts = static_cast<uint32_t>(((unit_last + 1u) * ctas - 1u) / total) - blockIdx.x + 1u;
           cut.second = first_segment ? 0u : 1u;
           cut.first_row = u.first_row;
@@ -1022,7 +1024,7 @@ __global__ void __launch_bounds__(256) prefill_join_kernel(const AttendParams p)
   __shared__ uint32_t bad_rows;
   pdl_wait();
   pdl_launch_dependents();
-  const Cut cut = p_cuts(p)[blockIdx.x];
+  const Cut cut = cut_of(p, blockIdx.x);
   const uint32_t y0 = blockIdx.y * kJoinRows;  // first row within the unit
   if (cut.parts == 0u || y0 >= cut.rows) return;
   if (threadIdx.x == 0) bad_rows = 0u;

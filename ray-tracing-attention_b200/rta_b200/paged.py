@@ -228,8 +228,8 @@ class PagedCache:
         if status == _lib.RTA_OK:
             return
         message = self._lib.rta_last_error().decode(errors="replace")
-        if word.value:  # after an expired wait the counters may hold anything: clear those too
-            (self.workspace if word.value & 1 else self.workspace[:4]).zero_()
+        if word.value:
+            self.workspace[:4].zero_()
         raise RtaError(status, message)
 
     def _map(self, map: PageMap | None) -> PageMap:
