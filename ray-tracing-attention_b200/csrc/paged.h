@@ -77,6 +77,7 @@ struct AppendParams {
   const void* v;
   uint64_t row_stride, head_stride;  // elements
   uint32_t* err;
+  uint32_t block_rows;  // set by the launch
 };
 cudaError_t launch_append(const AppendParams& p, int fmt, int in_fmt, cudaStream_t s);
 
@@ -86,7 +87,8 @@ struct MapArrays {
   int32_t* lengths;
 };
 struct PagesParams {
-  MapArrays map;  // updated in place (the caller has copied `map` to `out`)
+  MapArrays map;   // updated in place
+  MapArrays from;  // copied into it first, where refs is not null
   uint32_t slot_count, width, pages, page_size;
   uint8_t* k;
   uint8_t* v;
@@ -100,6 +102,7 @@ struct PagesParams {
   uint32_t* plan;  // scratch words: see pages.cu
 };
 size_t plan_bytes(uint32_t pages, uint32_t slots);
+bool plan_copies(uint32_t pages, uint32_t slots, uint32_t width);  // whether a plan copies a map of this size itself
 cudaError_t launch_map_copy(const MapArrays& from, const MapArrays& to, uint32_t pages, uint32_t slots,
                             uint32_t width, cudaStream_t s);
 cudaError_t launch_reserve(const PagesParams& p, cudaStream_t s);

@@ -136,9 +136,9 @@ bool same_map(const rta_page_map* a, const rta_page_map* b) {
   return a->refs == b->refs && a->table == b->table && a->lengths == b->lengths;
 }
 
-// Checks a bookkeeping call, fills its parameters, and copies map to out when
-// they are two maps.
-rta_status pages_params(const char* fn, const rta_page_pool* pool, const rta_page_map* map, const rta_page_map* out,
+// Checks a bookkeeping call, fills its parameters, and has map copied to out when
+// they are two maps: by the call's plan where it can, else by a launch.
+rta_status pages_params(const char* fn, bool plan, const rta_page_pool* pool, const rta_page_map* map, const rta_page_map* out,
                         uint32_t count, void* ws, size_t ws_bytes, cudaStream_t s, paged::PagesParams& p) {
   const char* why = bad_pool(pool);
   if (!why) why = bad_map(pool, map);
@@ -152,6 +152,7 @@ rta_status pages_params(const char* fn, const rta_page_pool* pool, const rta_pag
   if (why) return refuse(fn, why);
   const Workspace w(ws);
   p.map = {out->refs, out->table, out->lengths};
+  p.from = {nullptr, nullptr, nullptr};
   p.slot_count = map->slots;
   p.width = map->width;
   p.pages = pool->pages;
@@ -171,6 +172,10 @@ rta_status pages_params(const char* fn, const rta_page_pool* pool, const rta_pag
   p.err = w.err;
   p.plan = static_cast<uint32_t*>(w.body);
   if (same_map(map, out)) return RTA_OK;
+  if (plan && paged::plan_copies(pool->pages, map->slots, map->width)) {
+    p.from = {map->refs, map->table, map->lengths};
+    return RTA_OK;
+  }
   return status(paged::launch_map_copy({map->refs, map->table, map->lengths}, p.map, pool->pages, map->slots,
                                        map->width, s),
                 fn);
@@ -250,7 +255,7 @@ rta_status rta_pages_reserve(const rta_page_pool* pool, const rta_page_map* map,
   if (!counts || !batch) return refuse("rta_pages_reserve", "null counts or an empty batch");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   paged::PagesParams p;
-  const rta_status st = pages_params("rta_pages_reserve", pool, map, out, batch, workspace, workspace_bytes, s, p);
+  const rta_status st = pages_params("rta_pages_reserve", true, pool, map, out, batch, workspace, workspace_bytes, s, p);
   if (st != RTA_OK) return st;
   p.a = slots;
   p.b = counts;
@@ -263,7 +268,7 @@ rta_status rta_pages_fork(const rta_page_pool* pool, const rta_page_map* map, co
   if (!src || !dst || !count) return refuse("rta_pages_fork", "null src or dst, or nothing to fork");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   paged::PagesParams p;
-  const rta_status st = pages_params("rta_pages_fork", pool, map, out, count, workspace, workspace_bytes, s, p);
+  const rta_status st = pages_params("rta_pages_fork", true, pool, map, out, count, workspace, workspace_bytes, s, p);
   if (st != RTA_OK) return st;
   p.a = src;
   p.b = dst;
@@ -276,7 +281,7 @@ rta_status rta_pages_free(const rta_page_pool* pool, const rta_page_map* map, co
   if (!slots || !count) return refuse("rta_pages_free", "null slots or nothing to free");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   paged::PagesParams p;
-  const rta_status st = pages_params("rta_pages_free", pool, map, out, count, workspace, workspace_bytes, s, p);
+  const rta_status st = pages_params("rta_pages_free", false, pool, map, out, count, workspace, workspace_bytes, s, p);
   if (st != RTA_OK) return st;
   p.a = slots;
   return status(paged::launch_free(p, s), "rta_pages_free");
@@ -286,7 +291,7 @@ rta_status rta_pages_compact(const rta_page_pool* pool, const rta_page_map* map,
                              uint32_t* live, void* workspace, size_t workspace_bytes, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   paged::PagesParams p;
-  const rta_status st = pages_params("rta_pages_compact", pool, map, out, 0, workspace, workspace_bytes, s, p);
+  const rta_status st = pages_params("rta_pages_compact", true, pool, map, out, 0, workspace, workspace_bytes, s, p);
   if (st != RTA_OK) return st;
   p.live = live;
   return status(paged::launch_compact(p, s), "rta_pages_compact");

@@ -109,15 +109,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
   pdl_launch_dependents();
   if (threadIdx.x == 0) cut_of(p, blockIdx.x).parts = 0u;
 
-  // ---- the list of tiles: its length, and this CTA's range -----------------
-  uint64_t total = 0, own = 0, own_upto = 0;  // this thread's (last) sequence in the list
+  // ---- the list of units: its length, and this CTA's range ------------------
+  uint64_t tiles = 0, own = 0, own_upto = 0;  // this thread's (last) sequence in the list
+  uint32_t some = 0;                          // sequences that have anything to see
   for (uint32_t b0 = 0; b0 < p.c.batch; b0 += kThreads) {
     const uint32_t b = b0 + threadIdx.x;
     uint64_t mine = 0, sum;
     if (b < p.c.batch) {
       Unit u;
       visible(p, sequence(p.c, b, blockIdx.x == 0u ? p.err : nullptr), u);
-      mine = static_cast<uint64_t>(u.tiles) * per_seq;
+      mine = u.tiles;
       if (u.seen == 0u && b % gridDim.x == blockIdx.x) {  // nothing to see: zeros
         for (uint32_t i = 0; i < p.heads * HD; i += 4u)
           store4(out + static_cast<size_t>(b) * p.heads * HD + i, make_float4(0.f, 0.f, 0.f, 0.f));
@@ -125,42 +126,54 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
           for (uint32_t h = 0; h < p.heads; ++h) p.lse[static_cast<size_t>(b) * p.heads + h] = -INFINITY;
       }
     }
+    some += __syncthreads_count(mine != 0u);
     own = mine;
-    own_upto = total + block_scan(mine, scan_part, sum);
-    total += sum;
+    own_upto = tiles + block_scan(mine, scan_part, sum);
+    tiles += sum;
   }
-  if (total == 0u) return;
-  // at least a tile per warp for every CTA that takes part
-  const uint64_t want = (total + WARPS - 1u) / WARPS;
-  const uint64_t ctas = want < gridDim.x ? want : gridDim.x;
+  if (tiles == 0u) return;
+  tiles *= per_seq;
+  // Beginning and ending a unit costs a CTA about as much as some tiles (3.3 us
+  // measured, a tile of 16 KB 0.4 us): where the CTAs have many, each unit counts
+  // as four tiles per warp longer, in front (64 ragged sequences 209 -> 185 us,
+  // 100 windowed ones 244 -> 232 us; two per warp 187 and 236).  Where there are
+  // few, the units are cut evenly instead, one tile per warp.
+  const uint32_t entry = tiles / gridDim.x >= 4u * WARPS ? 4u * WARPS : 0u;
+  const uint64_t units = static_cast<uint64_t>(some) * per_seq, total = tiles + units * entry;
+  uint64_t ctas = (total + WARPS - 1u) / WARPS;
+  if (ctas > gridDim.x) ctas = gridDim.x;
+  if (!entry && units <= gridDim.x) ctas = min((ctas + units - 1u) / units, gridDim.x / units) * units;
   if (blockIdx.x >= ctas) return;
   const uint64_t begin = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1u) / ctas;
   const auto owner = [&](uint64_t t) { return static_cast<uint32_t>(((t + 1u) * ctas - 1u) / total); };
 
-  // ---- the unit that holds the first tile ----------------------------------
-  if (p.c.batch <= kThreads) {
-    if (own && begin < own_upto && begin >= own_upto - own) {
-      found_b = threadIdx.x;
-      found_at = begin - (own_upto - own);
-    }
-    __syncthreads();
-  } else {
+  // ---- the unit at its beginning --------------------------------------------
+  {
     uint64_t base = 0;
     for (uint32_t b0 = 0; b0 < p.c.batch; b0 += kThreads) {
       const uint32_t b = b0 + threadIdx.x;
-      uint64_t mine = 0, sum;
-      if (b < p.c.batch) {
-        Unit u;
-        visible(p, sequence(p.c, b, nullptr), u);
-        mine = static_cast<uint64_t>(u.tiles) * per_seq;
+      uint64_t mine = own, upto = own_upto, sum = tiles;
+      if (p.c.batch > kThreads) {  // otherwise the sums above are still these
+        mine = 0;
+        if (b < p.c.batch) {
+          Unit u;
+          visible(p, sequence(p.c, b, nullptr), u);
+          mine = u.tiles;
+        }
+        upto = block_scan(mine, scan_part, sum);
       }
-      const uint64_t upto = base + block_scan(mine, scan_part, sum);
-      if (mine && begin < upto && begin >= upto - mine) {
+      // sequences with anything to see before this one, for their entries
+      uint64_t sum_entries = 0;
+      const uint32_t before = entry ? static_cast<uint32_t>(block_scan(mine ? 1u : 0u, scan_part, sum_entries)) : 0u;
+      const uint64_t cost = mine ? (mine + entry) * per_seq : 0u;
+      const uint64_t last = p.c.batch > kThreads ? base + (upto + static_cast<uint64_t>(before) * entry) * per_seq
+                                                 : (upto + static_cast<uint64_t>(before) * entry) * per_seq;
+      if (mine && begin < last && begin >= last - cost) {
         found_b = b;
-        found_at = begin - (upto - mine);
+        found_at = begin - (last - cost);
       }
-      base += sum;
-      if (begin < base) break;
+      base += (sum + sum_entries * entry) * per_seq;
+      if (p.c.batch <= kThreads || begin < base) break;
     }
     __syncthreads();
   }
@@ -168,23 +181,29 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
   struct Segment {
     Unit u;
     uint32_t a, e;
+    uint64_t unit0;  // the unit's place in the list
   };
   uint64_t at = begin;  // place in the list behind the segments taken so far
-  const auto take = [&](Segment& s) {  // s.u is set: its tiles from s.a on that are this CTA's
-    s.e = static_cast<uint32_t>(min(static_cast<uint64_t>(s.u.tiles), s.a + (end - at)));
-    at += s.e - s.a;
+  // s.u is set, and its place `from` on is this CTA's; false: it holds no tile
+  const auto take = [&](Segment& s, uint32_t from) {
+    s.unit0 = at - from;
+    const uint32_t to = static_cast<uint32_t>(min(static_cast<uint64_t>(s.u.tiles + entry), from + (end - at)));
+    at += to - from;
+    s.a = from > entry ? from - entry : 0u;
+    s.e = to > entry ? to - entry : 0u;
+    return s.e > s.a;
   };
   const auto follow = [&](const Segment& s, Segment& next) {  // false: there is none
-    if (at >= end) return false;
     next.u = s.u;
-    if (++next.u.pr == per_seq) {
-      next.u.pr = 0;
-      do visible(p, sequence(p.c, ++next.u.b, nullptr), next.u);
-      while (next.u.tiles == 0u);
+    while (at < end) {
+      if (++next.u.pr == per_seq) {
+        next.u.pr = 0;
+        do visible(p, sequence(p.c, ++next.u.b, nullptr), next.u);
+        while (next.u.tiles == 0u);
+      }
+      if (take(next, 0u)) return true;
     }
-    next.a = 0;
-    take(next);
-    return true;
+    return false;
   };
   const auto first_head = [&](const Unit& u) { return u.pr / blocks * p.group + u.pr % blocks * S::kHeads; };
   const auto heads_of = [&](const Unit& u) { return min(S::kHeads, p.group - u.pr % blocks * S::kHeads); };
@@ -202,9 +221,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
   Segment cur, next;
   cur.u.b = found_b;
   visible(p, sequence(p.c, cur.u.b, nullptr), cur.u);
-  cur.u.pr = static_cast<uint32_t>(found_at / cur.u.tiles);
-  cur.a = static_cast<uint32_t>(found_at % cur.u.tiles);
-  take(cur);
+  cur.u.pr = static_cast<uint32_t>(found_at / (cur.u.tiles + entry));
+  if (!take(cur, static_cast<uint32_t>(found_at % (cur.u.tiles + entry)))) {
+    next = cur;
+    if (!follow(next, cur)) return;
+  }
   next = cur;
 
   // ---- this warp's tiles: warp, warp + WARPS, .. of every segment -----------
@@ -470,9 +491,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
     }
     if (!whole && a == 0u && threadIdx.x == 0) {  // what the second launch has to know
       Cut& cut = cut_of(p, blockIdx.x);
-      // the segments taken so far end at `at`, the last of them being this one or the next
-      const uint64_t unit0 = (more ? at - (next.e - next.a) : at) - e;
-      cut.parts = owner(unit0 + u.tiles - 1u) - blockIdx.x + 1u;
+      cut.parts = owner(cur.unit0 + entry + u.tiles - 1u) - blockIdx.x + 1u;
       cut.second = segment ? 1u : 0u;
       cut.b = u.b;
       cut.head0 = head0;

@@ -13,8 +13,9 @@ namespace paged {
 namespace {
 
 // ------------------------------------------------------------------ append
-// One warp per (new row, K/V head): K and V rows of head_dim elements, 16
-// bytes written per lane and step.
+// A block takes `block_rows` new rows: its warps find their places in the pool,
+// then every thread moves 16-byte pieces of the rows' K and V, one after the
+// other (neighbouring threads neighbouring pieces, whatever head_dim is).
 template <typename T, typename X>
 __device__ __forceinline__ uint4 convert8(const X* src);
 template <>
@@ -35,40 +36,51 @@ __device__ __forceinline__ uint4 convert8<__half, float>(const float* src) { ret
 template <>
 __device__ __forceinline__ uint4 convert8<__nv_bfloat16, float>(const float* src) { return round8<__nv_bfloat16>(src); }
 
+constexpr uint32_t kBlockRows = 64;  // at most
+
 template <typename T, typename X>
 __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
+  __shared__ uint64_t place[kBlockRows];
+  constexpr uint64_t kNowhere = ~0ull;
   pdl_wait();
   pdl_launch_dependents();
-  const uint32_t lane = threadIdx.x & 31u;
-  const uint64_t item = static_cast<uint64_t>(blockIdx.x) * 8u + (threadIdx.x >> 5);
-  if (item >= static_cast<uint64_t>(p.rows) * p.c.kv_heads) return;
-  const uint32_t row = static_cast<uint32_t>(item / p.c.kv_heads), kv = static_cast<uint32_t>(item % p.c.kv_heads);
-  // the sequence: how many of starts[1 .. batch] are <= row
-  uint32_t b = 0;
-  for (uint32_t i = 0; i < p.c.batch; i += 32u)
-    b += __popc(__ballot_sync(0xffffffffu, i + lane < p.c.batch && static_cast<uint32_t>(p.starts[i + lane + 1u]) <= row));
-  if (b >= p.c.batch) {
-    if (lane == 0u) atomicOr(p.err, RTA_DEVERR_SLOT);
-    return;
+  const uint32_t lane = threadIdx.x & 31u, row0 = blockIdx.x * p.block_rows;
+  const uint32_t rows = min(p.block_rows, p.rows - row0);
+  for (uint32_t r = threadIdx.x >> 5; r < rows; r += 8u) {
+    const uint32_t row = row0 + r;
+    // the sequence: how many of starts[1 .. batch] are <= row
+    uint32_t b = 0;
+    for (uint32_t i = 0; i < p.c.batch; i += 32u)
+      b += __popc(__ballot_sync(0xffffffffu, i + lane < p.c.batch && static_cast<uint32_t>(p.starts[i + lane + 1u]) <= row));
+    if (lane) continue;
+    uint64_t off = kNowhere;
+    if (b < p.c.batch) {
+      const Sequence s = sequence(p.c, b, p.err);
+      const uint32_t first = static_cast<uint32_t>(p.starts[b]), count = static_cast<uint32_t>(p.starts[b + 1u]) - first;
+      const int64_t at = static_cast<int64_t>(s.length) - count + (row - first);
+      if (at < 0 || at >= s.length)
+        atomicOr(p.err, RTA_DEVERR_SLOT);
+      else if (!locate(p.c, s.slot, static_cast<uint32_t>(at), off)) {
+        atomicOr(p.err, RTA_DEVERR_PAGE);
+        off = kNowhere;
+      }
+    } else {
+      atomicOr(p.err, RTA_DEVERR_SLOT);
+    }
+    place[r] = off;
   }
-  const Sequence s = sequence(p.c, b, lane == 0u ? p.err : nullptr);
-  const uint32_t new_rows = static_cast<uint32_t>(p.starts[b + 1u] - p.starts[b]);
-  const int64_t at = static_cast<int64_t>(s.length) - new_rows + (row - static_cast<uint32_t>(p.starts[b]));
-  uint64_t off = 0;
-  const bool inside = at >= 0 && at < s.length;
-  if (!inside || !locate(p.c, s.slot, static_cast<uint32_t>(at), off)) {
-    if (lane == 0u) atomicOr(p.err, inside ? RTA_DEVERR_PAGE : RTA_DEVERR_SLOT);
-    return;
-  }
-  off += kv * p.c.head_bytes;
-  const X* ks = static_cast<const X*>(p.k) + row * p.row_stride + kv * p.head_stride;
-  const X* vs = static_cast<const X*>(p.v) + row * p.row_stride + kv * p.head_stride;
-  uint8_t* kd = const_cast<uint8_t*>(p.c.k) + off;
-  uint8_t* vd = const_cast<uint8_t*>(p.c.v) + off;
-  for (uint32_t d = lane * 8u; d < p.c.head_dim; d += 256u) {
-    const uint4 a = convert8<T, X>(ks + d), c = convert8<T, X>(vs + d);
-    *reinterpret_cast<uint4*>(kd + d * 2u) = a;
-    *reinterpret_cast<uint4*>(vd + d * 2u) = c;
+  __syncthreads();
+  const uint32_t per_head = p.c.head_dim / 8u, per_row = 2u * p.c.kv_heads * per_head;  // pieces: K and V side by side
+  const uint32_t pieces = rows * per_row;
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < pieces; i += 256u) {
+    const uint32_t r = i / per_row, x = i % per_row, h = x / (2u * per_head), y = x % (2u * per_head);
+    const bool is_v = y >= per_head;
+    const uint32_t d = (is_v ? y - per_head : y) * 8u;
+    if (place[r] == kNowhere) continue;
+    const X* src = static_cast<const X*>(is_v ? p.v : p.k) + (row0 + r) * p.row_stride + h * p.head_stride + d;
+    uint8_t* dst = const_cast<uint8_t*>(is_v ? p.c.v : p.c.k) + place[r] + h * p.c.head_bytes + d * 2u;
+    *reinterpret_cast<uint4*>(dst) = convert8<T, X>(src);
   }
 }
 
@@ -116,6 +128,20 @@ __device__ uint32_t list_free(const int32_t* refs, uint32_t pages, uint32_t want
   return static_cast<uint32_t>(found < want ? found : want);
 }
 
+// A plan on another map's copy: where that is small, its block copies it itself
+// (a launch less); MapArrays.refs is null when there is nothing to copy.
+constexpr uint64_t kCopyWords = 32768;
+__device__ void copy_map(const PagesParams& p) {
+  if (!p.from.refs) return;
+  const uint64_t cells = static_cast<uint64_t>(p.slot_count) * p.width;
+#pragma unroll 8
+  for (uint64_t i = threadIdx.x; i < cells; i += kPlanThreads) p.map.table[i] = p.from.table[i];
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < p.pages; i += kPlanThreads) p.map.refs[i] = p.from.refs[i];
+  for (uint32_t i = threadIdx.x; i < p.slot_count; i += kPlanThreads) p.map.lengths[i] = p.from.lengths[i];
+  __syncthreads();
+}
+
 __global__ void map_copy_kernel(MapArrays from, MapArrays to, uint32_t pages, uint32_t slots, uint64_t cells) {
   pdl_wait();
   pdl_launch_dependents();
@@ -129,6 +155,7 @@ __global__ void map_copy_kernel(MapArrays from, MapArrays to, uint32_t pages, ui
 __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const PagesParams p) {
   pdl_wait();
   pdl_launch_dependents();
+  copy_map(p);
   __shared__ uint64_t part[32];
   const Plan plan(p.plan, p.pages, p.slot_count);
   uint64_t total = 0;
@@ -178,6 +205,7 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const PagesParams
 __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagesParams p) {
   pdl_wait();
   pdl_launch_dependents();
+  copy_map(p);
   __shared__ uint64_t part[32];
   __shared__ uint32_t fault;
   const Plan plan(p.plan, p.pages, p.slot_count);
@@ -242,6 +270,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagesPara
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagesParams p) {
   pdl_wait();
   pdl_launch_dependents();
+  copy_map(p);
   __shared__ uint64_t part[32];
   const Plan plan(p.plan, p.pages, p.slot_count);
   uint64_t mine = 0, live;
@@ -421,12 +450,15 @@ size_t plan_bytes(uint32_t pages, uint32_t slots) {
   return (kPlanHead + 4u * most) * 4u;
 }
 
-cudaError_t launch_append(const AppendParams& p, int fmt, int in_fmt, cudaStream_t s) {
-  const uint64_t items = static_cast<uint64_t>(p.rows) * p.c.kv_heads;
-  if (items == 0u) return cudaSuccess;
-  const uint64_t blocks = (items + 7u) / 8u;
-  if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
-  const dim3 grid(static_cast<uint32_t>(blocks));
+cudaError_t launch_append(const AppendParams& in, int fmt, int in_fmt, cudaStream_t s) {
+  if (in.rows == 0u) return cudaSuccess;
+  AppendParams p = in;
+  // about four pieces per thread, fewer while that leaves SMs idle
+  const uint32_t per_row = p.c.kv_heads * p.c.head_dim / 4u;
+  p.block_rows = per_row >= 1024u ? 1u : 1024u / per_row;
+  if (p.block_rows > kBlockRows) p.block_rows = kBlockRows;
+  while (p.block_rows > 1u && p.rows / p.block_rows < 296u) p.block_rows /= 2u;
+  const dim3 grid((p.rows + p.block_rows - 1u) / p.block_rows);
   if (fmt == kF16 && in_fmt == kF32)
     return launch_early(append_kernel<__half, float>, grid, dim3(256), 0, s, p);
   if (fmt == kF16)
@@ -436,6 +468,9 @@ cudaError_t launch_append(const AppendParams& p, int fmt, int in_fmt, cudaStream
   return launch_early(append_kernel<__nv_bfloat16, __nv_bfloat16>, grid, dim3(256), 0, s, p);
 }
 
+bool plan_copies(uint32_t pages, uint32_t slots, uint32_t width) {
+  return static_cast<uint64_t>(slots) * width + pages <= kCopyWords;
+}
 cudaError_t launch_map_copy(const MapArrays& from, const MapArrays& to, uint32_t pages, uint32_t slots,
                             uint32_t width, cudaStream_t s) {
   const uint64_t cells = static_cast<uint64_t>(slots) * width;
