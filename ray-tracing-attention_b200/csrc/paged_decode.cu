@@ -14,8 +14,8 @@
 // record per CTA, which a second launch joins, a CTA per head.
 //
 // The kernel is bound by HBM, so everything else has to stay out of the way of
-// the copies: each warp owns a ring of tiles that it fills by 16-byte copies
-// two tiles ahead, across the ends of units; the page of a tile is looked up
+// the copies: each warp owns a ring of tiles (of its dimensions) that it fills by
+// 16-byte copies two tiles ahead, across the ends of units; the page of a tile is looked up
 // one tile before its copies; the next unit's queries are copied while this
 // one's tiles are read.
 #include <atomic>
@@ -50,14 +50,22 @@ __device__ __forceinline__ Cut& cut_of(const AttendParams& p, uint32_t cta) {
 template <typename T, typename Q, int HD, int WARPS, int STAGES, bool PAIR>
 struct Shape {
   static constexpr uint32_t kHeads = PAIR ? 8 : 16;
-  static constexpr uint32_t kRow = HD * 2;             // bytes of one K or V row
+  // Warps that share a tile, each with 128 of its dimensions: its part of the
+  // scores, which the two exchange, and its part of the values.  (One warp for
+  // 256 dimensions, four per SM, was bound by its own instructions: 64 ragged
+  // sequences 205 us.)
+  static constexpr uint32_t kParts = HD == 256 ? 2 : 1;
+  static constexpr uint32_t kGroups = WARPS / kParts;  // tiles in work at a time
+  static constexpr uint32_t kWide = HD / kParts;       // dimensions of a warp
+  static constexpr uint32_t kRow = kWide * 2;          // bytes of one K or V row of a warp
   static constexpr uint32_t kChunks = kRow / 16;       // 16-byte chunks per row
   static constexpr uint32_t kStage = 2 * kTile * kRow; // K rows then V rows
   static constexpr uint32_t kRing = WARPS * STAGES * kStage;
   static constexpr uint32_t kQueries = kHeads * HD * sizeof(Q);  // one unit's
   // the warps' results are added a part of the dimensions at a time, in 16 KB
-  static constexpr uint32_t kPasses = WARPS * kHeads * HD * 4 / 16384 ? WARPS * kHeads * HD * 4 / 16384 : 1;
-  static constexpr uint32_t kJoin = WARPS * kHeads * (HD / kPasses) * 4;
+  static constexpr uint32_t kPasses = WARPS * kHeads * kWide * 4 / 16384 ? WARPS * kHeads * kWide * 4 / 16384 : 1;
+  static constexpr uint32_t kJoin = WARPS * kHeads * (kWide / kPasses) * 4;
+  static constexpr uint32_t kSwap = PAIR ? 4 : 8;      // scores per lane that two warps exchange
   static constexpr uint32_t kSmem = kRing + 2 * kQueries + kJoin;
 };
 
@@ -95,13 +103,14 @@ template <typename T, typename Q, int HD, int WARPS, int STAGES, bool PAIR>
 __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParams p) {
   using S = Shape<T, Q, HD, WARPS, STAGES, PAIR>;
   using N = Num<T>;
-  constexpr uint32_t kThreads = WARPS * 32, kSteps = HD / 16;
+  constexpr uint32_t kThreads = WARPS * 32, kSteps = S::kWide / 16, kParts = S::kParts, kGroups = S::kGroups;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t scan_part[WARPS];
   __shared__ uint32_t found_b;
   __shared__ uint64_t found_at;
   __shared__ float join_m[WARPS][S::kHeads], join_z[WARPS][S::kHeads];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t4 = lane & 3u;
+  const uint32_t group = warp / kParts, part = warp % kParts;
   const uint32_t blocks = (p.group + S::kHeads - 1u) / S::kHeads;  // head blocks per K/V head
   const uint32_t per_seq = p.c.kv_heads * blocks;
   Q* const out = static_cast<Q*>(p.out);
@@ -135,12 +144,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
   tiles *= per_seq;
   // Beginning and ending a unit costs a CTA about as much as some tiles (3.3 us
   // measured, a tile of 16 KB 0.4 us): where the CTAs have many, each unit counts
-  // as four tiles per warp longer, in front (64 ragged sequences 209 -> 185 us,
-  // 100 windowed ones 244 -> 232 us; two per warp 187 and 236).  Where there are
-  // few, the units are cut evenly instead, one tile per warp.
-  const uint32_t entry = tiles / gridDim.x >= 4u * WARPS ? 4u * WARPS : 0u;
+  // as four tiles per group of warps longer, in front (64 ragged sequences 209 -> 185 us,
+  // 100 windowed ones 244 -> 232 us; two per group 187 and 236).  Where there are
+  // few, the units are cut evenly instead, one tile per group.
+  const uint32_t entry = tiles / gridDim.x >= 4u * kGroups ? 4u * kGroups : 0u;
   const uint64_t units = static_cast<uint64_t>(some) * per_seq, total = tiles + units * entry;
-  uint64_t ctas = (total + WARPS - 1u) / WARPS;
+  uint64_t ctas = (total + kGroups - 1u) / kGroups;
   if (ctas > gridDim.x) ctas = gridDim.x;
   if (!entry && units <= gridDim.x) ctas = min((ctas + units - 1u) / units, gridDim.x / units) * units;
   if (blockIdx.x >= ctas) return;
@@ -228,13 +237,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
   }
   next = cur;
 
-  // ---- this warp's tiles: warp, warp + WARPS, .. of every segment -----------
+  // ---- this warp's tiles: group, group + groups, .. of every segment --------
   const uint32_t ring = smem_u32(smem) + warp * STAGES * S::kStage;
   uint32_t issued = 0, consumed = 0;  // tiles; tile n lies in stage n % STAGES
   // the next tile to issue: lane r < 16 holds the page of its position r and
   // the bytes inside the page
   bool in_next = false, have = false;
-  uint32_t tile = cur.a + warp;
+  uint32_t tile = cur.a + group;
   int32_t page = -1;
   uint32_t real = 0;
   uint64_t inside = 0;
@@ -244,7 +253,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
     const uint32_t pos = n < s.u.first ? n : n + s.u.skip;
     const uint32_t j = real ? page_of(p.c, pos) : 0u;
     page = real ? p.c.table[static_cast<size_t>(s.u.slot) * p.c.width + j] : 0;
-    inside = static_cast<uint64_t>(pos - j * p.c.page_size) * p.c.pos_bytes + static_cast<uint64_t>(s.u.pr / blocks) * p.c.head_bytes;
+    inside = static_cast<uint64_t>(pos - j * p.c.page_size) * p.c.pos_bytes + static_cast<uint64_t>(s.u.pr / blocks) * p.c.head_bytes +
+             part * S::kRow;
   };
   const auto find = [&](bool more) {  // the tile at or after `tile`, in this segment or the next
     have = false;
@@ -256,7 +266,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
       }
       if (!more) return;
       in_next = true;
-      tile = next.a + warp;
+      tile = next.a + group;
     }
     if (tile < next.e) {
       have = true;
@@ -281,7 +291,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
     }
     cp_commit();
     ++issued;
-    tile += WARPS;
+    tile += kGroups;
     find(more);
   };
 
@@ -301,7 +311,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
     // Query fragments (A operand: rows are heads, k is the dimension).
     uint32_t qa[kSteps][4];
     {
-      const Q* q0 = reinterpret_cast<const Q*>(smem + S::kRing + (segment & 1u) * S::kQueries) + g * HD + 2u * t4;
+      const Q* q0 = reinterpret_cast<const Q*>(smem + S::kRing + (segment & 1u) * S::kQueries) + g * HD + part * S::kWide + 2u * t4;
 #pragma unroll
       for (uint32_t kk = 0; kk < kSteps; ++kk)
 #pragma unroll
@@ -322,15 +332,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
         }
     }
 
-    float o[HD / 8][4];
+    float o[S::kWide / 8][4];
 #pragma unroll
-    for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    for (int j = 0; j < static_cast<int>(S::kWide / 8); ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     constexpr int kRows = PAIR ? 1 : 2;  // heads of this lane: g (and g + 8)
     float m[kRows], z[kRows];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) m[r] = -INFINITY, z[r] = 0.f;
 
-    for (uint32_t i = a + warp; i < e; i += WARPS) {
+    for (uint32_t i = a + group; i < e; i += kGroups) {
       while (have && issued < consumed + STAGES) issue(more);
       if (issued == consumed + STAGES)
         cp_wait<STAGES - 1>();
@@ -352,7 +362,35 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
         N::mma(sc[kk & 1u][0], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], f[0], f[1]);
         N::mma(sc[kk & 1u][1], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], f[2], f[3]);
       }
+      // whole scores: both accumulators, the query's two halves, both parts
       float pr[kRows][2][2], rescale[kRows];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            pr[r][c][x] = sc[0][c][2 * r + x] + sc[1][c][2 * r + x];
+            if (PAIR) pr[r][c][x] += sc[0][c][2 + x] + sc[1][c][2 + x];
+          }
+      if (kParts == 2) {
+        // two buffers taken in turn: the other warp has read one before this
+        // warp, a barrier later, writes it again
+        float* const swap = reinterpret_cast<float*>(smem + S::kRing + 2 * S::kQueries) +
+                            (consumed & 1u) * (WARPS * S::kSwap * 32u) + lane * 4u;
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+          store4(swap + (warp * kRows + r) * 128u, make_float4(pr[r][0][0], pr[r][0][1], pr[r][1][0], pr[r][1][1]));
+        asm volatile("bar.sync %0, 64;" ::"r"(1u + group) : "memory");
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          const float4 y = *reinterpret_cast<const float4*>(swap + ((warp ^ 1u) * kRows + r) * 128u);
+          pr[r][0][0] += y.x;
+          pr[r][0][1] += y.y;
+          pr[r][1][0] += y.z;
+          pr[r][1][1] += y.w;
+        }
+      }
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         float mx = -INFINITY;
@@ -360,9 +398,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            float s = sc[0][c][2 * r + x] + sc[1][c][2 * r + x];
-            if (PAIR) s += sc[0][c][2 + x] + sc[1][c][2 + x];  // the query's lower half
-            s *= p.scale_log2;
+            float s = pr[r][c][x] * p.scale_log2;
             if (i * kTile + c * 8u + 2u * t4 + x >= u.seen) s = -INFINITY;
             pr[r][c][x] = s;
             mx = fmaxf(mx, s);
@@ -387,7 +423,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
       if (!PAIR) moved |= rescale[kRows - 1] != 1.f;
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-        for (int j = 0; j < HD / 8; ++j) {
+        for (int j = 0; j < static_cast<int>(S::kWide / 8); ++j) {
           o[j][0] *= rescale[0];
           o[j][1] *= rescale[0];
           o[j][2] *= rescale[kRows - 1];
@@ -411,7 +447,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
         }
       }
 #pragma unroll
-      for (uint32_t j = 0; j < HD / 8u; j += 2u) {
+      for (uint32_t j = 0; j < S::kWide / 8u; j += 2u) {
         uint32_t f[4];
         const uint32_t r = (lane & 7u) + (((lane >> 3) & 1u) << 3), c = j + (lane >> 4);
         ldsm4_t(st + (kTile + r) * S::kRow + ((c ^ (r & 7u)) << 4), f);
@@ -439,12 +475,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
     const bool whole = a == 0u && e == u.tiles;
     float* const rec = p.records + static_cast<size_t>(blockIdx.x * 2u + (segment ? 1u : 0u)) * record_floats(HD);
     float* const join = reinterpret_cast<float*>(smem + S::kRing + 2 * S::kQueries);  // [warp][head][dimensions of a pass]
-    constexpr uint32_t kDims = HD / S::kPasses;
+    constexpr uint32_t kDims = S::kWide / S::kPasses;  // of each part
     cp_commit();
     cp_wait<0>();  // the next unit's queries, and its first tiles, are there
 #pragma unroll
     for (uint32_t pass = 0; pass < S::kPasses; ++pass) {
-      if (pass) __syncthreads();
+      if (pass || kParts == 2) __syncthreads();  // the sums before, or the exchanges, have been read
 #pragma unroll
       for (uint32_t j = 0; j < kDims / 8u; ++j) {
         const float(&x)[4] = o[pass * (kDims / 8u) + j];
@@ -457,18 +493,19 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
         }
       }
       __syncthreads();
-      for (uint32_t i = threadIdx.x; i < heads * (kDims / 4u); i += kThreads) {
-        const uint32_t h = i / (kDims / 4u), dp = i % (kDims / 4u) * 4u, d = pass * kDims + dp;
+      for (uint32_t i = threadIdx.x; i < kParts * heads * (kDims / 4u); i += kThreads) {
+        const uint32_t hp = i / (kDims / 4u), h = hp / kParts, of = hp % kParts, dp = i % (kDims / 4u) * 4u;
+        const uint32_t d = of * S::kWide + pass * kDims + dp;
         float mm = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, join_m[w][h]);
+        for (uint32_t w = 0; w < WARPS; w += kParts) mm = fmaxf(mm, join_m[w][h]);
         const float base = mm == -INFINITY ? 0.f : mm;
         float zz = 0.f;
         float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
+        for (uint32_t w = 0; w < WARPS; w += kParts) {
           const float f = exp2f(join_m[w][h] - base);
-          const float4 x = *reinterpret_cast<const float4*>(join + (w * S::kHeads + h) * kDims + dp);
+          const float4 x = *reinterpret_cast<const float4*>(join + ((w + of) * S::kHeads + h) * kDims + dp);
           zz += join_z[w][h] * f;
           oo.x += x.x * f;
           oo.y += x.y * f;
@@ -503,7 +540,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParam
     if (in_next)
       in_next = false;
     else
-      tile = cur.a + warp;
+      tile = cur.a + group;
     more = follow(cur, next);
     if (!have) find(more);
   }
@@ -620,7 +657,7 @@ cudaError_t by_dim(const AttendParams& p, cudaStream_t s) {
   switch (p.c.head_dim) {
     case 64: return launch<T, Q, 64, 8, 6, PAIR>(p, s);
     case 128: return launch<T, Q, 128, 8, 3, PAIR>(p, s);
-    default: return launch<T, Q, 256, 4, 3, PAIR>(p, s);
+    default: return launch<T, Q, 256, 8, 3, PAIR>(p, s);
   }
 }
 
