@@ -867,21 +867,22 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
       if (lane == 0) arrive(&full[told % kStages]);
       ++told;
     };
-    // Table entry of position `block * 128 + row0 + lane + 32 x`, kNone where
-    // nothing is visible; resolved to an offset a block later, when it is here.
-    constexpr int32_t kNone = INT32_MIN;
+    // Table entry of position `block * 128 + row0 + lane + 32 x`, 0 where there is
+    // none; resolved to an offset a block later, when it is here.
     const auto look = [&](uint32_t block, uint32_t x) -> int32_t {
       const uint32_t l = lane + 32u * x, at = block * kKeys + row0 + l;
-      if (l >= mine || at >= u.seen) return kNone;
+      if (l >= mine || at >= u.seen) return 0;
       const uint32_t pos = at < u.firsts ? at : at + u.skip;
       return p.c.table[static_cast<size_t>(u.slot) * p.c.width + page_of(p.c, pos)];
     };
     const auto resolve = [&](uint32_t block, uint32_t x, int32_t page) -> uint64_t {
+      const uint32_t l = lane + 32u * x, at = block * kKeys + row0 + l;
+      if (l >= mine || at >= u.seen) return ~0ull;
       if (static_cast<uint32_t>(page) >= p.c.pages) {
-        if (page != kNone) atomicOr(p.err, RTA_DEVERR_PAGE);
+        atomicOr(p.err, RTA_DEVERR_PAGE);
         return ~0ull;
       }
-      const uint32_t at = block * kKeys + row0 + lane + 32u * x, pos = at < u.firsts ? at : at + u.skip;
+      const uint32_t pos = at < u.firsts ? at : at + u.skip;
       return static_cast<uint64_t>(page) * p.c.page_bytes + static_cast<uint64_t>(pos - page_of(p.c, pos) * p.c.page_size) * p.c.pos_bytes +
              static_cast<uint64_t>(u.kv) * p.c.head_bytes;
     };
@@ -962,7 +963,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
       const uint32_t whole = maps.box ? min(e, max(a, u.seen / kKeys)) : a;
       int32_t kp = box_page(a), np = box_page(a + 1u), vp = 0;  // pages of this K block, the next, and the V block
       uint64_t k0 = 0, k1 = 0, v0 = 0, v1 = 0;
-      int32_t n0 = kNone, n1 = kNone;
+      int32_t n0 = 0, n1 = 0;
       if (whole < a + 2u) {
         n0 = look(whole, 0);
         n1 = look(whole, 1);

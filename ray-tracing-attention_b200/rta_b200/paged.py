@@ -112,6 +112,12 @@ class PagedCache:
         rows, heads, _ = q.shape
         return rows, heads, fmt, q.stride(0) if rows > 1 else 0, q.stride(1) if heads > 1 else 0
 
+    @staticmethod
+    def _reach(window: int, sinks: int):
+        if window < 0 or sinks < 0:
+            raise ValueError("window and sinks are not negative")
+        return min(window, 0xffffffff), min(sinks, 0xffffffff)
+
     def _out(self, q: torch.Tensor, out: torch.Tensor | None, lse: bool):
         if out is None:
             out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=self.device)
@@ -127,6 +133,7 @@ class PagedCache:
         visible, scale: 1 / sqrt(head_dim) unless given.  Returns out, or (out, lse) with lse=True."""
         rows, heads, fmt, row, head = self._q(q)
         out, l = self._out(q, out, lse)
+        window, sinks = self._reach(window, sinks)
         m = self._map(map)
         if rows:
             check(self._lib.rta_paged_decode(
@@ -142,6 +149,7 @@ class PagedCache:
         q [rows, heads, head_dim] are sequence b's, its last ones.  The rest as in decode; q in the cache's type."""
         rows, heads, fmt, row, head = self._q(q)
         out, l = self._out(q, out, lse)
+        window, sinks = self._reach(window, sinks)
         m = self._map(map)
         batch = _ints(starts, "starts", self.device).shape[0] - 1
         if rows:

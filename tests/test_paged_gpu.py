@@ -68,6 +68,10 @@ def get(cache, pool, layer, slot, n, map=None):
     return pool[layer, at, :, p % cache.page_size]
 
 
+def ints(*x):
+    return torch.tensor(list(x), dtype=torch.int32, device="cuda")
+
+
 def attend(q, k, v, t, window, sinks, scale, u_w, u_out, tiny):
     """64-bit attention of rows q [m, heads, dim] at positions t over k, v [n, kv_heads, dim]: out, lse, and the bound
     of the module's docstring."""
@@ -253,6 +257,126 @@ def test_growing_scores(paged):
     near(one, want[-1:], bound[-1:], "decode")
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [(torch.float16, 8, 2, 128), (torch.bfloat16, 8, 2, 256),
+                                                      (torch.float16, 4, 4, 256), (torch.bfloat16, 8, 4, 64)])
+@pytest.mark.parametrize("top", [-400.0, 6.0, 60.0, 900.0])
+def test_scores_that_move_far(paged, dtype, heads, kv_heads, dim, top):
+    """Scores that rise (or fall) by `top` along the sequence, from the first position on: the reference of the
+    prefill moves, the maximum of the decode moves, weights reach both ends of their range."""
+    n = 700
+    cache = build(paged, [n], kv_heads, dim, 32, dtype)
+    size = math.sqrt(abs(top))
+    ramp = torch.linspace(0, 1, n, device="cuda")[:, None, None].expand(n, kv_heads, dim) * size
+    ramp = ramp + torch.randn(n, kv_heads, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(5)) * 0.01
+    put(cache, cache.k, 0, 0, 0, ramp.to(dtype))
+    q = torch.full((n, heads, dim), size * math.copysign(1.0, top), device="cuda").to(dtype)
+    out, lse = cache.prefill(q, ints(0, n), scale=1 / dim, lse=True)
+    cache.check()
+    k, v = get(cache, cache.k, 0, 0, n), get(cache, cache.v, 0, 0, n)
+    want, want_lse, bound, lse_bound = attend(q, k, v, torch.arange(n, device="cuda"), 0, 0, 1 / dim, U_ONE[dtype],
+                                              U_OUT[dtype], TINY[dtype])
+    near(out, want, bound, "prefill")
+    near(lse, want_lse, lse_bound, "lse")
+    near(cache.decode(q[-1:], scale=1 / dim), want[-1:], bound[-1:], "decode")
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.11, 1e-6, 3.0])
+@pytest.mark.parametrize("dtype,dim,page", [(torch.float16, 256, 16), (torch.bfloat16, 128, 64)])
+def test_prefill_scales(paged, scale, dtype, dim, page):
+    parts = [(40, 100), (0, 7)]
+    lengths, new = [a + b for a, b in parts], [b for _, b in parts]
+    cache = build(paged, lengths, 2, dim, page, dtype)
+    starts = ints(0, *np.cumsum(new))
+    q = torch.randn(sum(new), 6, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(3)).to(dtype)
+    out = cache.prefill(q, starts, scale=scale)
+    cache.check()
+    row = 0
+    for b, (n, m) in enumerate(zip(lengths, new)):
+        want, _, bound, _ = attend(q[row:row + m], get(cache, cache.k, 0, b, n), get(cache, cache.v, 0, b, n),
+                                   torch.arange(n - m, n, device="cuda"), 0, 0, scale, U_ONE[dtype], U_OUT[dtype],
+                                   TINY[dtype])
+        near(out[row:row + m], want, bound, f"sequence {b}")
+        row += m
+
+
+@pytest.mark.parametrize("batch,new,past,window,sinks", [(600, 5, 60, 0, 0), (450, 90, 10, 20, 3), (2, 1, 2 ** 14, 0, 0)])
+def test_prefill_many(paged, batch, new, past, window, sinks):
+    """More sequences than a block has threads, and units that are cut over many blocks."""
+    rng = np.random.default_rng(batch)
+    parts = [(int(rng.integers(0, past + 1)) if batch > 2 else past, int(rng.integers(0, new + 1)) if batch > 2 else 1)
+             for _ in range(batch)]
+    lengths, news = [a + b for a, b in parts], [b for _, b in parts]
+    cache = build(paged, lengths, 2, 128, 32, torch.bfloat16, seed=batch)
+    starts = ints(0, *np.cumsum(news))
+    q = torch.randn(sum(news), 8, 128, device="cuda", generator=torch.Generator("cuda").manual_seed(4)).bfloat16()
+    out = cache.prefill(q, starts, window=window, sinks=sinks)
+    cache.check()
+    for b in sorted({0, 1, batch // 2, batch - 1, int(np.argmax(lengths)), int(np.argmax(news))}):
+        n, m, row = lengths[b], news[b], sum(news[:b])
+        want, _, bound, _ = attend(q[row:row + m], get(cache, cache.k, 0, b, n), get(cache, cache.v, 0, b, n),
+                                   torch.arange(n - m, n, device="cuda"), window, sinks, 128 ** -0.5, 2.0 ** -8,
+                                   2.0 ** -8, 1e-37)
+        near(out[row:row + m], want, bound, f"sequence {b}")
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "one head", "one page", "padded"])
+def test_pool_layouts(paged, layout):
+    """Views with other strides: K and V in one tensor, dimensions of extent one, rows wider than head_dim."""
+    kv_heads, page, pages, dim = (1 if layout == "one head" else 2), 64, (1 if layout == "one page" else 9), 128
+    if layout == "interleaved":
+        both = torch.randn(2, pages, 2, page, kv_heads, dim, device="cuda").half()
+        k, v = both[:, :, 0].transpose(2, 3), both[:, :, 1].transpose(2, 3)
+    elif layout == "padded":
+        k, v = (torch.randn(2, pages, kv_heads, page, dim + 8, device="cuda").half()[..., :dim] for _ in range(2))
+    else:
+        k, v = (torch.randn(2, pages, kv_heads, page, dim, device="cuda").half() for _ in range(2))
+    n = min(64, pages * page) if pages == 1 else 500
+    need = -(-n // page)
+    table = torch.full((1, 8), -1, dtype=torch.int32, device="cuda")
+    table[0, :need] = torch.randperm(pages, device="cuda")[:need].to(torch.int32)
+    refs = torch.zeros(pages, dtype=torch.int32, device="cuda")
+    refs[table[0, :need].long()] = 1
+    cache = paged.PagedCache(k, v, paged.PageMap(refs, table, ints(n)))
+    q = torch.randn(n, 4 * kv_heads, dim, device="cuda").half()
+    out = cache.prefill(q, ints(0, n), layer=1)
+    cache.check()
+    want, _, bound, _ = attend(q, get(cache, k, 1, 0, n), get(cache, v, 1, 0, n), torch.arange(n, device="cuda"), 0, 0,
+                               128 ** -0.5, 2.0 ** -11, 2.0 ** -11, 2.0 ** -24)
+    near(out, want, bound, "prefill")
+    near(cache.decode(q[-1:], layer=1), want[-1:], bound[-1:], "decode")
+
+
+def test_reach_past_every_length(paged):
+    """Windows and sinks larger than any sequence, up to the largest number, change nothing."""
+    cache = build(paged, [300], 2, 64, 16, torch.float16)
+    q = torch.randn(300, 4, 64, device="cuda").half()
+    plain, one = cache.prefill(q, ints(0, 300)), cache.decode(q[-1:])
+    for window, sinks in ((300, 0), (2 ** 31 + 5, 2 ** 32 - 1), (2 ** 40, 1), (7, 2 ** 32 - 1), (1, 300)):
+        assert torch.equal(cache.prefill(q, ints(0, 300), window=window, sinks=sinks), plain)
+        assert torch.equal(cache.decode(q[-1:], window=window, sinks=sinks), one)
+    with pytest.raises(ValueError):
+        cache.decode(q[-1:], window=-1)
+
+
+def test_bad_pages_are_read_as_zeros(paged):
+    """Table entries outside the pool, where blocks come by TMA and where rows are copied: flagged, and nothing else."""
+    from rta_b200._lib import RtaError
+    for page in (32, 16):
+        cache = build(paged, [400, 400], 2, 128, page, torch.bfloat16)
+        q = torch.randn(400, 4, 128, device="cuda").bfloat16()
+        good = cache.prefill(q, ints(0, 400), slots=ints(1))
+        for entry in (-1, 10 ** 6, -2 ** 31, cache.pages):
+            cache.map.table[0, 3] = entry
+            cache.prefill(q, ints(0, 400))
+            with pytest.raises(RtaError, match="word 4$"):
+                cache.check()
+            cache.decode(q[-1:])
+            with pytest.raises(RtaError, match="word 4$"):
+                cache.check()
+        assert torch.equal(cache.prefill(q, ints(0, 400), slots=ints(1)), good)
+        cache.check()
+
+
 @pytest.mark.parametrize("dtype,heads,kv_heads,dim,window,sinks", [
     (torch.float16, 16, 4, 256, 0, 0), (torch.bfloat16, 8, 2, 128, 0, 0), (torch.bfloat16, 8, 8, 64, 40, 3),
     (torch.float16, 8, 2, 128, 100, 0)])
@@ -392,10 +516,6 @@ class Model:
         assert m.refs.tolist() == self.refs
         assert m.lengths.tolist() == self.lengths
         assert m.table.tolist() == [row + [-1] * (self.width - len(row)) for row in self.table]
-
-
-def ints(*x):
-    return torch.tensor(list(x), dtype=torch.int32, device="cuda")
 
 
 @pytest.mark.parametrize("page,order,slots,pages,width", [(16, "heads", 12, 200, 20), (5, "positions", 9, 97, 30),
@@ -604,3 +724,15 @@ def test_refusals(paged):
         with pytest.raises(ValueError):
             call()
     assert cache.decode(q[:0]).shape == (0, 4, 64)  # nothing to do
+
+
+@pytest.mark.parametrize("prompt,samples,tokens", [(700, 6, 24), (33, 3, 40), (256, 2, 5)])
+def test_serving_example(paged, prompt, samples, tokens):
+    """Prefill in chunks, fork, decode as a graph, free, compact, decode on: the states of the model without a cache.
+    bf16 activations through three layers: each rounds to 2^-9, and so do its projections, its weights and its result,
+    about ten roundings a layer that add up like independent ones: 2^-9 sqrt(30) = 1.1e-2; 3e-2 is asked for."""
+    from rta_b200.examples.paged_serving import serve
+    said, worst, live, used, pages = serve(prompt, samples, tokens)
+    assert said.shape == (samples - samples // 2, 2 * tokens)
+    assert worst < 3e-2
+    assert live <= used <= pages
