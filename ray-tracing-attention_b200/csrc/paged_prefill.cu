@@ -130,10 +130,6 @@ __device__ __forceinline__ void set_tile(const AttendParams& p, Unit& u, uint32_
   u.seen = seen_by(p, u, R1 - 1u);
   u.blocks = blocks_of(u.seen);
 }
-// What a unit costs: its blocks, and about as much as kEntry of them to fill
-// and to empty the pipeline (a segment of the list that holds only a unit's
-// entry holds nothing).
-constexpr uint32_t kEntry = 2;
 template <int HD>
 __device__ __forceinline__ void next_unit(const AttendParams& p, Unit& u) {
   if (u.tile + 1u < u.tiles) {
@@ -147,15 +143,15 @@ __device__ __forceinline__ void next_unit(const AttendParams& p, Unit& u) {
   }
   set_tile<HD>(p, u, 0u);
 }
-// Cost of all tiles of a sequence (one K/V head), by the whole warp: a lane
+// Blocks of all tiles of a sequence (one K/V head), by the whole warp: a lane
 // adds a short sequence's itself, the warp shares a long one's.
 template <int HD>
-__device__ uint64_t sequence_cost(const AttendParams& p, Unit u) {
+__device__ uint64_t sequence_blocks(const AttendParams& p, Unit u) {
   uint64_t sum = 0;
   if (u.tiles <= 4u)
     for (uint32_t i = 0; i < u.tiles; ++i) {
       set_tile<HD>(p, u, i);
-      sum += u.blocks + kEntry;
+      sum += u.blocks;
     }
   uint32_t longs = __ballot_sync(0xffffffffu, u.tiles > 4u);
   while (longs) {
@@ -168,7 +164,7 @@ __device__ uint64_t sequence_cost(const AttendParams& p, Unit u) {
     uint64_t part = 0;
     for (uint32_t i = threadIdx.x & 31u; i < v.tiles; i += 32u) {
       set_tile<HD>(p, v, i);
-      part += v.blocks + kEntry;
+      part += v.blocks;
     }
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
@@ -181,21 +177,21 @@ __device__ uint64_t sequence_cost(const AttendParams& p, Unit u) {
 template <int HD>
 struct Walk {
   Unit u;
-  uint64_t unit0, left;  // the unit's place in the list; what is left of the range
-  uint32_t at, a, e;     // place in the unit
+  uint64_t unit0, left;     // the unit's place in the list; what is left of the range
+  uint32_t entry, at, a, e;  // what a unit costs besides its blocks; place in the unit
   __device__ __forceinline__ bool step(const AttendParams& p) {
     while (left) {
-      uint32_t cost = u.blocks + kEntry;
+      uint32_t cost = u.blocks + entry;
       if (at == cost) {
         unit0 += cost;
         at = 0;
         next_unit<HD>(p, u);
-        cost = u.blocks + kEntry;
+        cost = u.blocks + entry;
       }
       const uint32_t take = static_cast<uint32_t>(min(left, static_cast<uint64_t>(cost - at)));
-      a = at > kEntry ? at - kEntry : 0u;
+      a = at > entry ? at - entry : 0u;
       at += take;
-      e = at > kEntry ? at - kEntry : 0u;
+      e = at > entry ? at - entry : 0u;
       left -= take;
       if (e > a) return true;
     }
@@ -356,6 +352,10 @@ template <typename T>
 struct Room {
   static constexpr float value = Num<T>::kBf16 ? 1.152921504606846976e18f : 16384.f;  // 2^60, 2^14
 };
+// See the list of units: kEntry blocks for a unit's beginning and end where there
+// are kFew blocks or more per CTA, else at least kLeast blocks per CTA.
+constexpr uint32_t kEntry = 2, kFew = 4, kLeast = 2;
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const AttendParams p, const __grid_constant__ Maps maps) {
   using S = Shape<HD>;
@@ -397,68 +397,72 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
   pdl_launch_dependents();  // the joining launch waits for this grid's end by itself
   if (threadIdx.x == 0) cut_of(p, blockIdx.x).parts = 0u;
 
-  // ---- the list of blocks and this CTA's range ------------------------------
-  uint64_t total = 0;
+  // ---- the list of units and this CTA's range --------------------------------
+  uint64_t blocks = 0, tiles = 0, own = 0, own_upto = 0, own_tiles_upto = 0;  // own: this thread's (last) sequence
+  uint32_t own_tiles = 0;
   for (uint32_t b0 = 0; b0 < p.c.batch; b0 += S::kThreads) {
     const uint32_t b = b0 + threadIdx.x;
     Unit u;
     u.tiles = 0;
     if (b < p.c.batch) load_sequence<HD>(p, b, u, blockIdx.x == 0u ? p.err : nullptr);
     uint64_t sum;
-    block_scan(sequence_cost<HD>(p, u) * p.c.kv_heads, scan_part, sum);
-    total += sum;
+    own = sequence_blocks<HD>(p, u);
+    own_upto = blocks + block_scan(own, scan_part, sum);
+    blocks += sum;
+    own_tiles = u.tiles;
+    own_tiles_upto = tiles + block_scan(own_tiles, scan_part, sum);
+    tiles += sum;
   }
-  if (total == 0u) return;
-  const uint64_t want = (total + kEntry + 1u) / (kEntry + 2u);  // at least about two blocks per CTA
-  const uint64_t ctas = want < gridDim.x ? want : gridDim.x;
+  if (tiles == 0u) return;
+  // Filling and emptying the pipeline costs a unit about as much as kEntry
+  // blocks: where the CTAs have several blocks each, a unit counts as that much
+  // longer, in front.  Where there are few, the units are cut evenly instead.
+  const uint64_t units = tiles * p.c.kv_heads;
+  const uint32_t entry = blocks * p.c.kv_heads >= static_cast<uint64_t>(kFew) * gridDim.x ? kEntry : 0u;
+  const uint64_t total = blocks * p.c.kv_heads + units * entry;
+  uint64_t ctas = entry ? total : (total + kLeast - 1u) / kLeast;
+  if (ctas > gridDim.x) ctas = gridDim.x;
+  if (!entry && units <= gridDim.x) ctas = min((ctas + units - 1u) / units, gridDim.x / units) * units;
   if (blockIdx.x >= ctas) return;
   const uint64_t begin = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1u) / ctas;
   {
-    uint64_t base = 0;
+    uint64_t before = 0, before_tiles = 0;
     for (uint32_t b0 = 0; b0 < p.c.batch; b0 += S::kThreads) {
-      const uint32_t b = b0 + threadIdx.x;
-      Unit u;
-      u.tiles = 0;
-      if (b < p.c.batch) load_sequence<HD>(p, b, u, nullptr);
-      uint64_t sum;
-      const uint64_t mine = sequence_cost<HD>(p, u) * p.c.kv_heads;
-      const uint64_t upto = base + block_scan(mine, scan_part, sum);
-      if (mine && begin < upto && begin >= upto - mine) {
-        found_b = b;
-        found_at = begin - (upto - mine);
+      if (p.c.batch > S::kThreads) {  // otherwise the sums above are still these
+        const uint32_t b = b0 + threadIdx.x;
+        Unit u;
+        u.tiles = 0;
+        if (b < p.c.batch) load_sequence<HD>(p, b, u, nullptr);
+        uint64_t sum;
+        own = sequence_blocks<HD>(p, u);
+        own_upto = before + block_scan(own, scan_part, sum);
+        before += sum;
+        own_tiles = u.tiles;
+        own_tiles_upto = before_tiles + block_scan(own_tiles, scan_part, sum);
+        before_tiles += sum;
       }
-      base += sum;
-      if (begin < base) break;
+      const uint64_t upto = (own_upto + own_tiles_upto * entry) * p.c.kv_heads, per_kv = own + own_tiles * entry;
+      if (own_tiles && begin < upto && begin >= upto - per_kv * p.c.kv_heads) {
+        const uint64_t at = begin - (upto - per_kv * p.c.kv_heads);
+        found_b = b0 + threadIdx.x;
+        found_kv = static_cast<uint32_t>(at / per_kv);
+        found_at = at % per_kv;
+      }
+      if (p.c.batch <= S::kThreads || begin < (before + before_tiles * entry) * p.c.kv_heads) break;
     }
     __syncthreads();
   }
   Unit first;
   load_sequence<HD>(p, found_b, first, nullptr);
-  first.kv = 0;
-  if (warp == 0) {
-    // the K/V head, then the tile whose blocks hold the offset
+  first.kv = found_kv;
+  if (warp == 0) {  // the tile that holds the offset
     uint64_t off = found_at;
-    const Unit all = first;
-    uint64_t per_kv = 0;
     for (uint32_t i0 = 0; i0 < first.tiles; i0 += 32u) {
-      Unit v = all;
+      Unit v = first;
       uint64_t n = 0;
       if (i0 + lane < first.tiles) {
         set_tile<HD>(p, v, i0 + lane);
-        n = v.blocks + kEntry;
-      }
-#pragma unroll
-      for (int d = 16; d >= 1; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
-      per_kv += n;
-    }
-    const uint32_t kv = static_cast<uint32_t>(off / per_kv);
-    off -= kv * per_kv;
-    for (uint32_t i0 = 0; i0 < first.tiles; i0 += 32u) {
-      Unit v = all;
-      uint64_t n = 0;
-      if (i0 + lane < first.tiles) {
-        set_tile<HD>(p, v, i0 + lane);
-        n = v.blocks + kEntry;
+        n = v.blocks + entry;
       }
       uint64_t upto = n;
 #pragma unroll
@@ -469,11 +473,10 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
       const uint32_t hit = __ballot_sync(0xffffffffu, off < upto);
       if (hit) {
         const int at = __ffs(hit) - 1;
-        const uint64_t before = __shfl_sync(0xffffffffu, upto - n, at);
+        const uint64_t past = __shfl_sync(0xffffffffu, upto - n, at);
         if (lane == 0) {
           found_tile = i0 + at;
-          found_at = off - before;
-          found_kv = kv;
+          found_at = off - past;
         }
         break;
       }
@@ -489,10 +492,10 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
   __syncthreads();
   tc_after();
   const uint32_t tmem = tmem_base;
-  first.kv = found_kv;
   set_tile<HD>(p, first, found_tile);
   Walk<HD> walk;
   walk.u = first;
+  walk.entry = entry;
   walk.at = static_cast<uint32_t>(found_at);
   walk.unit0 = begin - walk.at;
   walk.left = end - begin;
@@ -550,7 +553,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     while (more && ok) {
       const Unit u = walk.u;
       const uint32_t a = walk.a, e = walk.e;
-      const uint64_t unit_last = walk.unit0 + u.blocks + kEntry - 1u;  // the unit's last place in the list
+      const uint64_t unit_last = walk.unit0 + u.blocks + walk.entry - 1u;  // the unit's last place in the list
       const uint32_t rows = lane_rows(u, L), n = lane_blocks(u, L, a, e);
       const uint32_t R = u.tile * S::kRows + L * kLaneRows + r;
       const bool real = r < rows;
