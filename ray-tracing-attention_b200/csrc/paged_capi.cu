@@ -57,6 +57,13 @@ const char* bad_workspace(const rta_page_pool* p, const rta_page_map* m, const v
 
 size_t element(int format) { return format == RTA_F32 ? 4u : 2u; }
 
+// x / d = (umulhi(x, mul) + x) >> shift for x < 2^31: mul = floor(2^32 (2^shift - d) / d) + 1, shift = ceil(log2 d)
+void divide(uint32_t d, uint32_t& mul, uint32_t& shift) {
+  shift = 0;
+  while ((1u << shift) < d) ++shift;
+  mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1u);
+}
+
 paged::View view(const rta_page_pool* p, const rta_page_map* m, uint32_t layer, const int32_t* slots, uint32_t batch) {
   paged::View v;
   v.k = static_cast<const uint8_t*>(p->k) + layer * p->layer_stride * 2u;
@@ -71,10 +78,7 @@ paged::View view(const rta_page_pool* p, const rta_page_map* m, uint32_t layer, 
   v.width = m->width;
   v.pages = p->pages;
   v.page_size = p->page_size;
-  // x / d = (umulhi(x, mul) + x) >> shift for x < 2^31: mul = floor(2^32 (2^shift - d) / d) + 1, shift = ceil(log2 d)
-  v.div_shift = 0;
-  while ((1u << v.div_shift) < p->page_size) ++v.div_shift;
-  v.div_mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << v.div_shift) - p->page_size)) / p->page_size + 1u);
+  divide(p->page_size, v.div_mul, v.div_shift);
   v.batch = batch;
   v.kv_heads = p->kv_heads;
   v.head_dim = p->head_dim;

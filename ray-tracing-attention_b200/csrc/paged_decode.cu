@@ -36,8 +36,9 @@ __host__ __device__ constexpr uint32_t record_floats(uint32_t hd) { return kRecH
 // A unit that begins in a CTA's range and ends in another's: at most one per CTA.
 struct Cut {
   uint32_t parts;   // CTAs that hold a part of it, from this one on; 0: no such unit
+  uint32_t heads;
   uint32_t second;  // this CTA's record of it is its second (the others': their first)
-  uint32_t b, head0, heads;
+  uint32_t b, head0;
 };
 __device__ __forceinline__ Cut& cut_of(const AttendParams& p, uint32_t cta) {
   return *reinterpret_cast<Cut*>(static_cast<uint8_t*>(p.cuts) + cta * kCutBytes);

@@ -75,8 +75,9 @@ constexpr uint32_t kTmemO = 256;  // tensor-memory column of O (S buffers at 0 a
 // A unit that begins in a CTA's range and ends in another's: at most one per CTA.
 struct Cut {
   uint32_t parts;   // CTAs that hold a part of it, from this one on; 0: no such unit
+  uint32_t rows;
   uint32_t second;  // this CTA's record of it is its second (the others': their first)
-  uint32_t first_row, R0, rows, kv, slot;
+  uint32_t first_row, R0, kv, slot;
   int32_t past;
   uint32_t firsts, low, high;
 };
@@ -101,15 +102,13 @@ struct Unit {
 
 template <int HD>
 __device__ __forceinline__ void load_sequence(const AttendParams& p, uint32_t b, Unit& u, uint32_t* err) {
+  const Sequence s = sequence(p.c, b, err);  // (its loads and those of the rows run side by side)
   const uint32_t count = new_rows(p, b, u.first_row, err);
   u.b = b;
   u.rows = count * p.group;
   u.tiles = (u.rows + Shape<HD>::kRows - 1u) / Shape<HD>::kRows;
-  if (count) {
-    const Sequence s = sequence(p.c, b, err);
-    u.slot = s.slot;
-    u.past = static_cast<int32_t>(s.length) - static_cast<int32_t>(count);
-  }
+  u.slot = s.slot;
+  u.past = static_cast<int32_t>(s.length) - static_cast<int32_t>(count);
 }
 // Last visible position + 1, numbered without the gap, of rows up to R.
 __device__ __forceinline__ uint32_t seen_by(const AttendParams& p, const Unit& u, uint32_t R) {
@@ -364,7 +363,8 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t scan_part[S::kThreads / 32];
   __shared__ uint64_t found_at;
-  __shared__ uint32_t found_b, found_kv, found_tile, tmem_base, stop_word, never;
+  __shared__ Unit found_unit;
+  __shared__ uint32_t found_kv, found_tile, tmem_base, stop_word, never;
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~uintptr_t{1023});
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
   uint64_t* const full = bars;                 // [stages] producers -> MMA
@@ -394,22 +394,21 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
   }
 
   pdl_wait();
-  pdl_launch_dependents();  // the joining launch waits for this grid's end by itself
-  if (threadIdx.x == 0) cut_of(p, blockIdx.x).parts = 0u;
+  if (threadIdx.x == 0) *reinterpret_cast<uint2*>(&cut_of(p, blockIdx.x)) = make_uint2(0u, 0u);
 
   // ---- the list of units and this CTA's range --------------------------------
   uint64_t blocks = 0, tiles = 0, own = 0, own_upto = 0, own_tiles_upto = 0;  // own: this thread's (last) sequence
   uint32_t own_tiles = 0;
+  Unit seq;
   for (uint32_t b0 = 0; b0 < p.c.batch; b0 += S::kThreads) {
     const uint32_t b = b0 + threadIdx.x;
-    Unit u;
-    u.tiles = 0;
-    if (b < p.c.batch) load_sequence<HD>(p, b, u, blockIdx.x == 0u ? p.err : nullptr);
+    seq.tiles = 0;
+    if (b < p.c.batch) load_sequence<HD>(p, b, seq, blockIdx.x == 0u ? p.err : nullptr);
     uint64_t sum;
-    own = sequence_blocks<HD>(p, u);
+    own = sequence_blocks<HD>(p, seq);
     own_upto = blocks + block_scan(own, scan_part, sum);
     blocks += sum;
-    own_tiles = u.tiles;
+    own_tiles = seq.tiles;
     own_tiles_upto = tiles + block_scan(own_tiles, scan_part, sum);
     tiles += sum;
   }
@@ -430,21 +429,20 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     for (uint32_t b0 = 0; b0 < p.c.batch; b0 += S::kThreads) {
       if (p.c.batch > S::kThreads) {  // otherwise the sums above are still these
         const uint32_t b = b0 + threadIdx.x;
-        Unit u;
-        u.tiles = 0;
-        if (b < p.c.batch) load_sequence<HD>(p, b, u, nullptr);
+        seq.tiles = 0;
+        if (b < p.c.batch) load_sequence<HD>(p, b, seq, nullptr);
         uint64_t sum;
-        own = sequence_blocks<HD>(p, u);
+        own = sequence_blocks<HD>(p, seq);
         own_upto = before + block_scan(own, scan_part, sum);
         before += sum;
-        own_tiles = u.tiles;
+        own_tiles = seq.tiles;
         own_tiles_upto = before_tiles + block_scan(own_tiles, scan_part, sum);
         before_tiles += sum;
       }
       const uint64_t upto = (own_upto + own_tiles_upto * entry) * p.c.kv_heads, per_kv = own + own_tiles * entry;
       if (own_tiles && begin < upto && begin >= upto - per_kv * p.c.kv_heads) {
         const uint64_t at = begin - (upto - per_kv * p.c.kv_heads);
-        found_b = b0 + threadIdx.x;
+        found_unit = seq;
         found_kv = static_cast<uint32_t>(at / per_kv);
         found_at = at % per_kv;
       }
@@ -452,8 +450,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     }
     __syncthreads();
   }
-  Unit first;
-  load_sequence<HD>(p, found_b, first, nullptr);
+  Unit first = found_unit;
   first.kv = found_kv;
   if (warp == 0) {  // the tile that holds the offset
     uint64_t off = found_at;
@@ -1017,21 +1014,27 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
 }
 
 // Joins the records of cut units: blockIdx.x is the CTA in whose range the unit
-// begins, blockIdx.y sixteen of its rows.  O = sum_j 2^(m_j - max m) O_j over
-// sum_j 2^(m_j - max m) z_j.
-constexpr uint32_t kJoinRows = 16;
+// begins, blockIdx.y some of its rows.  O = sum_j 2^(m_j - max m) O_j over
+// sum_j 2^(m_j - max m) z_j.  It is bound by latency: every possible piece has a
+// CTA of its own (CTAs that share out the pieces: 25 us for a ragged batch where
+// this takes 7), and a row's O is on its way while its weights are worked out.
+template <int HD>
+constexpr uint32_t join_rows() { return 2048u / HD; }  // a thread for eight dimensions of a row
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) prefill_join_kernel(const AttendParams p) {
   using S = Shape<HD>;
   using N = Num<T>;
-  __shared__ float weight[kMaxCtas][kJoinRows];
+  constexpr uint32_t kRows = join_rows<HD>();
+  constexpr uint32_t kPer = 256 / kRows;      // threads that work out a row's weights
+  constexpr uint32_t kOwn = kMaxCtas / kPer;  // parts of each
+  constexpr uint32_t kAhead = 4;
+  __shared__ float weight[kMaxCtas][kRows];
   __shared__ uint32_t bad_rows;
   pdl_wait();
   pdl_launch_dependents();
   const Cut cut = cut_of(p, blockIdx.x);
-  const uint32_t y0 = blockIdx.y * kJoinRows;  // first row within the unit
+  const uint32_t y0 = blockIdx.y * kRows;  // first row within the unit
   if (cut.parts == 0u || y0 >= cut.rows) return;
-  if (threadIdx.x == 0) bad_rows = 0u;
   const uint32_t L = y0 / kLaneRows, r0 = y0 % kLaneRows;
   const auto record = [&](uint32_t j) {
     return p.records + (static_cast<size_t>((blockIdx.x + j) * 2u + (j == 0u ? cut.second : 0u)) * S::kLanes + L) * S::kRecord;
@@ -1042,48 +1045,70 @@ __global__ void __launch_bounds__(256) prefill_join_kernel(const AttendParams p)
     head = cut.kv * p.group + R % p.group;
     t = cut.past + static_cast<int32_t>(R / p.group);
   };
-  {  // weights: sixteen threads per row
-    const uint32_t x = threadIdx.x / 16u, k = threadIdx.x % 16u;
-    float mm = -INFINITY, zz = 0.f;
-    for (uint32_t j = k; j < cut.parts; j += 16u) mm = fmaxf(mm, record(j)[r0 + x]);
+  const uint32_t x = threadIdx.x % kRows, d8 = threadIdx.x / kRows;  // eight dimensions of a row
+  float4 lo[kAhead], hi[kAhead];
+  const auto load = [&](uint32_t j0) {
 #pragma unroll
-    for (int d = 8; d >= 1; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
-    const float base = mm == -INFINITY ? 0.f : mm;
-    for (uint32_t j = k; j < cut.parts; j += 16u) {
-      const float f = ex2(record(j)[r0 + x] - base);
-      if (f != 0.f) zz += f * record(j)[kLaneRows + r0 + x];
+    for (uint32_t j = 0; j < kAhead; ++j)
+      if (j0 + j < cut.parts) {
+        const float4* o = reinterpret_cast<const float4*>(record(j0 + j) + 2 * kLaneRows) + 2u * d8 * kLaneRows + r0 + x;
+        lo[j] = __ldcg(o);
+        hi[j] = __ldcg(o + kLaneRows);
+      }
+  };
+  load(0u);
+  if (threadIdx.x == 0) bad_rows = 0u;
+  {
+    const uint32_t wx = threadIdx.x / kPer, k = threadIdx.x % kPer;
+    float m[kOwn], z[kOwn], mm = -INFINITY, zz = 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i < kOwn; ++i) {
+      const uint32_t j = i * kPer + k;
+      m[i] = j < cut.parts ? record(j)[r0 + wx] : -INFINITY;
+      z[i] = j < cut.parts ? record(j)[kLaneRows + r0 + wx] : 0.f;
     }
 #pragma unroll
-    for (int d = 8; d >= 1; d >>= 1) zz += __shfl_xor_sync(0xffffffffu, zz, d);
+    for (uint32_t i = 0; i < kOwn; ++i) mm = fmaxf(mm, m[i]);
+#pragma unroll
+    for (int d = kPer / 2; d >= 1; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+    const float base = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+    for (uint32_t i = 0; i < kOwn; ++i) {
+      m[i] = ex2(m[i] - base);
+      if (m[i] != 0.f) zz += m[i] * z[i];
+    }
+#pragma unroll
+    for (int d = kPer / 2; d >= 1; d >>= 1) zz += __shfl_xor_sync(0xffffffffu, zz, d);
     const float inv = 1.f / zz;
-    for (uint32_t j = k; j < cut.parts; j += 16u) weight[j][x] = ex2(record(j)[r0 + x] - base) * inv;
-    if (p.lse && k == 0u && y0 + x < cut.rows) {
+#pragma unroll
+    for (uint32_t i = 0; i < kOwn; ++i)
+      if (i * kPer + k < cut.parts) weight[i * kPer + k][wx] = m[i] * inv;
+    if (p.lse && k == 0u && y0 + wx < cut.rows) {
       uint32_t row, head;
       int32_t t;
-      place(y0 + x, row, head, t);
+      place(y0 + wx, row, head, t);
       p.lse[static_cast<size_t>(row) * p.heads + head] = t < 0 ? -INFINITY : (mm + log2f(zz)) * kLn2;
     }
   }
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < kJoinRows * (HD / 8); i += 256u) {
-    const uint32_t x = i % kJoinRows, d8 = i / kJoinRows;  // eight dimensions of a row
-    if (y0 + x >= cut.rows) continue;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-#pragma unroll 4
-    for (uint32_t j = 0; j < cut.parts; ++j) {
-      const float f = weight[j][x];
-      if (f == 0.f) continue;  // an empty part has no O
-      const float4* o = reinterpret_cast<const float4*>(record(j) + 2 * kLaneRows) + 2u * d8 * kLaneRows + r0 + x;
-      const float4 u = __ldcg(o), v = __ldcg(o + kLaneRows);
-      a.x += f * u.x;
-      a.y += f * u.y;
-      a.z += f * u.z;
-      a.w += f * u.w;
-      b.x += f * v.x;
-      b.y += f * v.y;
-      b.z += f * v.z;
-      b.w += f * v.w;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+  for (uint32_t j0 = 0; j0 < cut.parts; j0 += kAhead) {
+    if (j0) load(j0);
+#pragma unroll
+    for (uint32_t j = 0; j < kAhead; ++j) {
+      const float f = j0 + j < cut.parts ? weight[j0 + j][x] : 0.f;
+      if (f == 0.f) continue;  // an empty part has no O: what was loaded is not used
+      a.x += f * lo[j].x;
+      a.y += f * lo[j].y;
+      a.z += f * lo[j].z;
+      a.w += f * lo[j].w;
+      b.x += f * hi[j].x;
+      b.y += f * hi[j].y;
+      b.z += f * hi[j].z;
+      b.w += f * hi[j].w;
     }
+  }
+  if (y0 + x < cut.rows) {
     uint32_t row, head;
     int32_t t;
     place(y0 + x, row, head, t);
@@ -1096,11 +1121,11 @@ __global__ void __launch_bounds__(256) prefill_join_kernel(const AttendParams p)
     *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (static_cast<size_t>(row) * p.heads + head) * HD + d8 * 8u) = w;
   }
   __syncthreads();
-  for (uint32_t x = threadIdx.x >> 5; x < kJoinRows; x += 8u) {  // see row_alone
-    if (!(bad_rows >> x & 1u)) continue;
+  for (uint32_t bx = threadIdx.x >> 5; bx < kRows; bx += 8u) {  // see row_alone
+    if (!(bad_rows >> bx & 1u)) continue;
     uint32_t row, head;
     int32_t t;
-    place(y0 + x, row, head, t);
+    place(y0 + bx, row, head, t);
     if (spoiled<T, HD>(p, cut.slot, cut.kv, cut.firsts, cut.low, cut.high, static_cast<uint32_t>(t)))
       row_alone<T, HD>(p, cut.slot, cut.kv, head, row, static_cast<uint32_t>(t));
   }
@@ -1180,7 +1205,7 @@ cudaError_t launch(const AttendParams& p, cudaStream_t s) {
   q.align = maps.box ? maps.box : 1u;
   e = launch_early(prefill_kernel<T, HD>, dim3(ctas), dim3(Shape<HD>::kThreads), Shape<HD>::kSmem, s, q, maps);
   if (e != cudaSuccess) return e;
-  return launch_early(prefill_join_kernel<T, HD>, dim3(ctas, Shape<HD>::kRows / kJoinRows), dim3(256), 0, s, q);
+  return launch_early(prefill_join_kernel<T, HD>, dim3(ctas, Shape<HD>::kRows / join_rows<HD>()), dim3(256), 0, s, q);
 }
 template <typename T>
 cudaError_t by_dim(const AttendParams& p, cudaStream_t s) {
