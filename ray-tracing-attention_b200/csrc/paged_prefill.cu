@@ -286,6 +286,12 @@ __device__ __forceinline__ void store32(void* at, const uint32_t* v) {  // 32 by
 __device__ __forceinline__ void arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ void arrive(uint64_t* bar, uint32_t count) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void cp_arrive(uint64_t* bar) {  // once this thread's copies so far have landed
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -317,15 +323,6 @@ __device__ __forceinline__ void tma4(uint32_t dst, const CUtensorMap* map, int32
           dst),
       "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
-}
-// Whether a phase has ended, without waiting (mbar_try_wait may suspend the thread).
-__device__ __forceinline__ bool phase_ended(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0,1,0,p; }"
-               : "=r"(done)
-               : "r"(smem_u32(bar)), "r"(parity)
-               : "memory");
-  return done != 0;
 }
 // Bounded wait of a whole warp; false (for all its lanes) ends the role.
 // Inline to the end: a kernel that moves registers between its warps cannot
@@ -379,7 +376,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
 
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < kStages; ++i) {
-      mbar_init(&full[i], S::kProducers);
+      mbar_init(&full[i], S::kProducers * 32u);
       mbar_init(&empty[i], 1);
     }
     for (uint32_t i = 0; i < 2u; ++i) {
@@ -753,7 +750,11 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     const uint32_t q0 = smem_u32(smem), ring = q0 + S::kRing;
     uint32_t st = 0, it[2] = {0, 0}, segs[2] = {0, 0};  // stages consumed, blocks and segments of each lane
     bool ok = true;
-    const auto wait_stage = [&](uint32_t x) { return warp_wait(&full[x % kStages], x / kStages & 1u, p.err, stop); };
+    const auto wait_stage = [&](uint32_t x) {
+      const bool here = warp_wait(&full[x % kStages], x / kStages & 1u, p.err, stop);
+      fence_async();  // rows copied by the producers' threads are read by the MMA's proxy
+      return here;
+    };
     const uint64_t high = desc(0u, 16u), high_v = desc(0u, kSub);
     const uint32_t id_s = idesc<T>(kKeys, false) | (p.scale_log2 < 0.f ? 1u << 13 : 0u);
     // S (+)= Q K^T over the dimensions of one stage
@@ -858,15 +859,9 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     constexpr uint32_t kOwn = S::kOwn;
     const uint32_t w = warp - S::kSoftmaxWarps - 1u, row0 = w * kOwn, mine = min(kOwn, kKeys - row0);
     const uint32_t ring = smem_u32(smem) + S::kRing;
-    uint32_t st = 0, told = 0;  // stages issued, and made known to the MMA warp
+    uint32_t st = 0;  // stages issued
     bool ok = true;
     const Unit& u = walk.u;
-    const auto tell = [&]() {
-      fence_async();
-      __syncwarp();
-      if (lane == 0) arrive(&full[told % kStages]);
-      ++told;
-    };
     // Table entry of position `block * 128 + row0 + lane + 32 x`, 0 where there is
     // none; resolved to an offset a block later, when it is here.
     const auto look = [&](uint32_t block, uint32_t x) -> int32_t {
@@ -886,27 +881,18 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
       return static_cast<uint64_t>(page) * p.c.page_bytes + static_cast<uint64_t>(pos - page_of(p.c, pos) * p.c.page_size) * p.c.pos_bytes +
              static_cast<uint64_t>(u.kv) * p.c.head_bytes;
     };
-    const auto flush = [&]() {
-      cp_wait<0>();
-      while (told < st) tell();
-    };
-    // waits until the next stage is free
-    const auto next_stage = [&]() {
-      const uint32_t s = st % kStages, par = (st / kStages & 1u) ^ 1u;
-      if (!__all_sync(0xffffffffu, phase_ended(&empty[s], par))) {
-        flush();  // the MMA warp must know of every stage issued while this warp waits
-        ok = warp_wait(&empty[s], par, p.err, stop);
-      }
+    const auto next_stage = [&]() {  // waits until the next stage is free
+      const uint32_t s = st % kStages;
+      ok = warp_wait(&empty[s], (st / kStages & 1u) ^ 1u, p.err, stop);
       return s;
     };
     // one stage by TMA: lane i of the first producer brings box i, of `page`
     const uint32_t boxes = maps.box ? kKeys / maps.box : 0u;
     const auto bring = [&](const CUtensorMap* map, int32_t page, uint32_t block, uint32_t half) {
-      flush();
       const uint32_t s = next_stage();
       if (!ok) return;
       if (w == 0u) {
-        if (lane == 0) mbar_expect_tx(&full[s], S::kStage);
+        if (lane == 0) mbar_expect_tx(&full[s], S::kStage);  // arrives, as 31 others do here, and 32 of each other warp
         __syncwarp();
         if (lane < boxes) {
           const uint32_t at = block * kKeys + lane * maps.box, pos = at < u.firsts ? at : at + u.skip;
@@ -922,10 +908,9 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
             tma4(dst + x * kSub, map, static_cast<int32_t>(half * 128u + x * 64u), maps.heads_first ? kv : y,
                  maps.heads_first ? y : kv, page, &full[s]);
         }
-      } else if (lane == 0) {
-        arrive(&full[s]);
       }
-      told = ++st;
+      if (lane == 0) arrive(&full[s], w == 0u ? 31u : 32u);
+      ++st;
     };
     const auto box_page = [&](uint32_t block) -> int32_t {
       const uint32_t at = block * kKeys + lane * maps.box;
@@ -950,12 +935,8 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
           for (uint32_t y = 0; y < S::kSubs; ++y) cp_async16(to + y * kSub, src + y * 128u, o != ~0ull);
         }
       }
-      cp_commit();
+      cp_arrive(&full[s]);  // when this thread's copies have landed
       ++st;
-      if (st - told > 2u) {
-        cp_wait<2>();
-        tell();
-      }
     };
     while (ok && walk.step(p)) {
       const uint32_t a = walk.a, e = walk.e;
@@ -996,15 +977,13 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
         np = box_page(j + 2u);
       }
     }
-    cp_wait<0>();
-    if (ok)
-      while (told < st) tell();
-    else {
+    if (!ok) {
       *stop = 1u;
       if (w == 0u)  // boxes still on their way have landed before the CTA exits (bounded)
         for (uint32_t x = st > kStages ? st - kStages : 0u; x < st; ++x)
           (void)warp_wait(&full[x % kStages], x / kStages & 1u, nullptr, &never);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   tc_before();
   __syncthreads();
