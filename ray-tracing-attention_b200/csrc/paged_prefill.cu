@@ -294,8 +294,8 @@ __device__ __forceinline__ void cp_arrive(uint64_t* bar) {  // once this thread'
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  float y;  // volatile: exponentials, sums and conversions stay in turn as written (3 percent of a ragged batch)
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if one of them is
