@@ -52,7 +52,6 @@ struct AttendParams {
   uint32_t rows;           // prefill: rows of the call
   uint32_t heads, group;   // query heads, query heads per K/V head
   float scale_log2;        // scale * log2(e): the softmax runs in base 2
-  float scale;
   uint32_t window, sinks;
   uint32_t align;  // prefill: reads begin at multiples of this many positions
   void* out;

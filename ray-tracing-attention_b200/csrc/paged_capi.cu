@@ -121,7 +121,6 @@ const char* attend_params(const rta_page_pool* pool, const rta_page_map* map, ui
   p.q_head = q_head;
   p.heads = heads;
   p.group = heads / pool->kv_heads;
-  p.scale = scale;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.window = window;
   p.sinks = sinks;
