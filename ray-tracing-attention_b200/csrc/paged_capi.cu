@@ -113,7 +113,7 @@ const char* attend_params(const rta_page_pool* pool, const rta_page_map* map, ui
   if (!aligned(q, 16) || q_row % unit || q_head % unit) return "q's rows must be 16-byte aligned";
   if (!aligned(out, 16)) return "out must be 16-byte aligned";
   if (lse && !aligned(lse, 4)) return "lse must be 4-byte aligned";
-  if (!std::isfinite(scale)) return "scale must be finite";
+  if (!std::isfinite(scale * 1.4426950408889634f)) return "scale (and scale * log2 e) must be finite";
   const Workspace w(ws);
   p.c = view(pool, map, layer, slots, batch);
   p.q = q;

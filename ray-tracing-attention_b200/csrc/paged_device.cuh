@@ -144,7 +144,8 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* part, uint6
 }
 
 // Rows first .. of the call that belong to sequence b: starts[b], and how many.
-// Offsets that do not ascend inside 0 .. rows are flagged and give no rows.
+// Offsets that do not ascend inside 0 .. rows are flagged and give no rows; rows
+// that belong to no sequence are flagged.
 __device__ __forceinline__ uint32_t new_rows(const AttendParams& p, uint32_t b, uint32_t& first, uint32_t* err) {
   const int32_t a = p.starts[b], e = p.starts[b + 1u];
   first = 0u;
@@ -152,6 +153,8 @@ __device__ __forceinline__ uint32_t new_rows(const AttendParams& p, uint32_t b, 
     if (err) atomicOr(err, RTA_DEVERR_SLOT);
     return 0u;
   }
+  if (err && ((b == 0u && a != 0) || (b + 1u == p.c.batch && static_cast<uint32_t>(e) != p.rows)))
+    atomicOr(err, RTA_DEVERR_SLOT);
   first = static_cast<uint32_t>(a);
   return static_cast<uint32_t>(e - a);
 }

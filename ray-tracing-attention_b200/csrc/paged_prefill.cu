@@ -1184,7 +1184,7 @@ cudaError_t launch(const AttendParams& p, cudaStream_t s) {
     sms_of[dev].store(sms, std::memory_order_release);
   }
   const uint32_t ctas = static_cast<uint32_t>(sms) < kMaxCtas ? static_cast<uint32_t>(sms) : kMaxCtas;
-  Maps maps;
+  Maps maps = {};
   AttendParams q = p;
   encode<T>(p, maps);
   q.align = maps.box ? maps.box : 1u;

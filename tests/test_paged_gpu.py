@@ -299,6 +299,28 @@ def test_prefill_scales(paged, scale, dtype, dim, page):
         row += m
 
 
+@pytest.mark.parametrize("page,order", [(128, "heads"), (256, "positions"), (96, "heads"), (224, "positions"),
+                                        (65536, "heads")])
+@pytest.mark.parametrize("dim,window,sinks", [(64, 0, 0), (128, 100, 33), (256, 200, 7)])
+def test_prefill_page_sizes(paged, page, order, dim, window, sinks):
+    """Pages that hold one box, several, or more than a block, with reads that begin inside a page."""
+    parts = [(300, 260), (0, 129)] if page < 65536 else [(100, 60)]
+    lengths, new = [a + b for a, b in parts], [b for _, b in parts]
+    cache = build(paged, lengths, 2 if page < 65536 else 1, dim, page, torch.bfloat16, order, stale=math.nan, spare=1)
+    heads = 4 * cache.kv_heads
+    starts = ints(0, *np.cumsum(new))
+    q = torch.randn(sum(new), heads, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(3)).bfloat16()
+    out = cache.prefill(q, starts, window=window, sinks=sinks)
+    cache.check()
+    row = 0
+    for b, (n, m) in enumerate(zip(lengths, new)):
+        want, _, bound, _ = attend(q[row:row + m], get(cache, cache.k, 0, b, n), get(cache, cache.v, 0, b, n),
+                                   torch.arange(n - m, n, device="cuda"), window, sinks, dim ** -0.5, 2.0 ** -8,
+                                   2.0 ** -8, 1e-37)
+        near(out[row:row + m], want, bound, f"sequence {b}")
+        row += m
+
+
 @pytest.mark.parametrize("batch,new,past,window,sinks", [(600, 5, 60, 0, 0), (450, 90, 10, 20, 3), (2, 1, 2 ** 14, 0, 0)])
 def test_prefill_many(paged, batch, new, past, window, sinks):
     """More sequences than a block has threads, and units that are cut over many blocks."""
@@ -620,6 +642,8 @@ def test_device_checks(paged):
     q = torch.randn(2, 2, 64, device="cuda").half()
     flagged(16, cache.decode, q, slots=ints(0, 7))
     flagged(16, cache.prefill, q, ints(0, 3))                     # past the rows
+    flagged(16, cache.prefill, q, ints(0, 1))                     # a row that no sequence owns
+    flagged(16, cache.prefill, q, ints(1, 2))
     flagged(16, cache.append, q[:, :1], q[:, :1], ints(0, 1))     # a row that no sequence owns
     table = cache.map.table.clone()
     cache.map.table[0, 1] = 99
