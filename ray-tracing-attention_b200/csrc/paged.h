@@ -28,8 +28,9 @@ inline cudaError_t launch_early(void (*kernel)(P...), dim3 grid, dim3 block, siz
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
-// CTAs of an attention launch at most (one per SM): bounds the split records.
-constexpr uint32_t kMaxCtas = 160;
+// CTAs of an attention launch at most (one per SM in the prefill, up to two in
+// the decode): bounds the split records.
+constexpr uint32_t kMaxCtas = 160, kMaxDecodeCtas = 320;
 
 // Where position p of a sequence lives.  page_size is any number, so p /
 // page_size is a multiply and a shift (exact for p < 2^31).

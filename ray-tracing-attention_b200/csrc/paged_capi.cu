@@ -42,7 +42,7 @@ const char* bad_map(const rta_page_pool* p, const rta_page_map* m) {
 
 // Workspace: error word and padding, the descriptions of cut units, then either
 // their records (an attention call) or the plan of a bookkeeping call.
-constexpr size_t kErr = 256, kCuts = (paged::kMaxCtas * paged::kCutBytes + 255u) / 256u * 256u, kBody = kErr + kCuts;
+constexpr size_t kErr = 256, kCuts = (paged::kMaxDecodeCtas * paged::kCutBytes + 255u) / 256u * 256u, kBody = kErr + kCuts;
 size_t workspace_bytes_of(const rta_page_pool* p, const rta_page_map* m) {
   size_t body = paged::decode_record_bytes();
   if (paged::prefill_record_bytes() > body) body = paged::prefill_record_bytes();

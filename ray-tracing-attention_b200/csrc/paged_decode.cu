@@ -66,8 +66,12 @@ struct Shape {
   static constexpr uint32_t kStage = 2 * kTile * kRow; // K rows then V rows
   static constexpr uint32_t kRing = WARPS * STAGES * kStage;
   static constexpr uint32_t kQueries = kHeads * HD * sizeof(Q);  // one unit's
-  // the warps' results are added a part of the dimensions at a time, in 16 KB
-  static constexpr uint32_t kPasses = WARPS * kHeads * kWide * 4 / 16384 ? WARPS * kHeads * kWide * 4 / 16384 : 1;
+  // two CTAs of four warps share an SM (one's units begin and end under the
+  // other's copies), or one of eight with 256 dimensions (its rings fill the SM)
+  static constexpr uint32_t kPerSm = WARPS == 4 ? 2 : 1;
+  // the warps' results are added a part of the dimensions at a time
+  static constexpr uint32_t kRoom = kPerSm == 2 ? 8192 : 16384;
+  static constexpr uint32_t kPasses = WARPS * kHeads * kWide * 4 / kRoom ? WARPS * kHeads * kWide * 4 / kRoom : 1;
   static constexpr uint32_t kJoin = WARPS * kHeads * (kWide / kPasses) * 4;
   static constexpr uint32_t kSwap = PAIR ? 4 : 8;      // scores per lane that two warps exchange
   static constexpr uint32_t kSmem = kRing + 2 * kQueries + kJoin;
@@ -104,7 +108,7 @@ __device__ __forceinline__ void store4(__nv_bfloat16* dst, float4 v) {
 }
 
 template <typename T, typename Q, int HD, int WARPS, int STAGES, bool PAIR>
-__global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(WARPS * 32, Shape<T, Q, HD, WARPS, STAGES, PAIR>::kPerSm) decode_kernel(const AttendParams p) {
   using S = Shape<T, Q, HD, WARPS, STAGES, PAIR>;
   using N = Num<T>;
   constexpr uint32_t kThreads = WARPS * 32, kSteps = S::kWide / 16, kParts = S::kParts, kGroups = S::kGroups;
@@ -557,7 +561,7 @@ template <typename T, typename Q, int HD>
 __global__ void __launch_bounds__(256) decode_join_kernel(const AttendParams p) {
   using N = Num<T>;
   constexpr uint32_t kQuads = HD / 4, kGroups = 256 / kQuads;
-  __shared__ float weight[kMaxCtas];
+  __shared__ float weight[kMaxDecodeCtas];
   __shared__ float4 sums[kGroups][kQuads];
   pdl_wait();
   pdl_launch_dependents();
@@ -569,7 +573,7 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const AttendParams p) 
   };
   const size_t row = static_cast<size_t>(cut.b) * p.heads + cut.head0 + h;
   if (threadIdx.x < 32u) {
-    constexpr uint32_t kOwn = kMaxCtas / 32u;
+    constexpr uint32_t kOwn = kMaxDecodeCtas / 32u;
     float m[kOwn], z[kOwn], mm = -INFINITY, zz = 0.f;
 #pragma unroll
     for (uint32_t k = 0; k < kOwn; ++k) {
@@ -649,25 +653,41 @@ cudaError_t launch(const AttendParams& p, cudaStream_t s) {
     if (sms <= 0) return cudaErrorInvalidDevice;
     sms_of[dev].store(sms, std::memory_order_release);
   }
-  const uint32_t ctas = static_cast<uint32_t>(sms) < kMaxCtas ? static_cast<uint32_t>(sms) : kMaxCtas;
+  const uint32_t most = static_cast<uint32_t>(sms) * Shape<T, Q, HD, WARPS, STAGES, PAIR>::kPerSm;
+  const uint32_t ctas = most < kMaxDecodeCtas ? most : kMaxDecodeCtas;
   e = launch_early(decode_kernel<T, Q, HD, WARPS, STAGES, PAIR>, dim3(ctas), dim3(WARPS * 32), smem, s, p);
   if (e != cudaSuccess) return e;
   const uint32_t heads = Shape<T, Q, HD, WARPS, STAGES, PAIR>::kHeads;
   return launch_early(decode_join_kernel<T, Q, HD>, dim3(ctas, p.group < heads ? p.group : heads), dim3(256), 0, s, p);
 }
 
+// Two CTAs of four warps per SM where units are short or many for each SM: of 32
+// / 8 heads x 128, 512 sequences of up to 300 positions take 86 us instead of
+// 122, 100 of them 27 instead of 33, while 160 of up to 4000 take 233 instead of
+// 223 and 100 windowed ones 248 instead of 240 (one CTA's rings are deeper).
+// Lengths are device data: what the table and the window allow stands for them.
+constexpr uint64_t kManyUnits = 8, kShort = 1024;
 template <typename T, typename Q, bool PAIR>
 cudaError_t by_dim(const AttendParams& p, cudaStream_t s) {
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  const uint32_t heads = PAIR ? 8u : 16u, blocks = (p.group + heads - 1u) / heads;
+  const uint64_t units = static_cast<uint64_t>(p.c.batch) * p.c.kv_heads * blocks;
+  uint64_t reach = static_cast<uint64_t>(p.c.width) * p.c.page_size;
+  if (p.window && static_cast<uint64_t>(p.window) + p.sinks < reach) reach = static_cast<uint64_t>(p.window) + p.sinks;
+  const bool many = units >= (reach <= kShort ? 1u : kManyUnits) * static_cast<uint64_t>(sms);
   switch (p.c.head_dim) {
-    case 64: return launch<T, Q, 64, 8, 6, PAIR>(p, s);
-    case 128: return launch<T, Q, 128, 8, 3, PAIR>(p, s);
+    case 64: return many ? launch<T, Q, 64, 4, 6, PAIR>(p, s) : launch<T, Q, 64, 8, 6, PAIR>(p, s);
+    case 128: return many ? launch<T, Q, 128, 4, 3, PAIR>(p, s) : launch<T, Q, 128, 8, 3, PAIR>(p, s);
     default: return launch<T, Q, 256, 8, 3, PAIR>(p, s);
   }
 }
 
 }  // namespace
 
-size_t decode_record_bytes() { return static_cast<size_t>(kMaxCtas) * 2u * record_floats(256) * 4u; }
+size_t decode_record_bytes() { return static_cast<size_t>(kMaxDecodeCtas) * 2u * record_floats(256) * 4u; }
 
 // Up to eight query heads per K/V head, and fp32 queries: paired rows.  More
 // 16-bit heads: sixteen per unit (fewer passes over K and V).
