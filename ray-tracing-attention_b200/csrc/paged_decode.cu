@@ -151,11 +151,13 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, Q, HD, WARPS, STAGES, PAI
   if (tiles == 0u) return;
   tiles *= per_seq;
   // Beginning and ending a unit costs a CTA about as much as some tiles (3.3 us
-  // measured, a tile of 16 KB 0.4 us): where the CTAs have many, each unit counts
-  // as four tiles per group of warps longer, in front (64 ragged sequences 209 -> 185 us,
-  // 100 windowed ones 244 -> 232 us; two per group 187 and 236).  Where there are
-  // few, the units are cut evenly instead, one tile per group.
-  const uint32_t entry = tiles / gridDim.x >= 4u * kGroups ? 4u * kGroups : 0u;
+  // measured, a tile of 16 KB 0.4 us), so each unit counts as that much longer,
+  // in front: four tiles per group of warps where the CTAs have a tile per group
+  // or more (64 ragged sequences 209 -> 185 us, 100 windowed ones 244 -> 232 us,
+  // 37 of up to 300 positions 33 -> 16 us), two where they have less (ten of up to
+  // 300 positions 21 -> 12 us), none for one sequence alone, whose units are
+  // alike and are cut evenly, a tile per group.
+  const uint32_t entry = tiles / gridDim.x >= kGroups ? 4u * kGroups : some > 1u ? 2u * kGroups : 0u;
   const uint64_t units = static_cast<uint64_t>(some) * per_seq, total = tiles + units * entry;
   uint64_t ctas = (total + kGroups - 1u) / kGroups;
   if (ctas > gridDim.x) ctas = gridDim.x;

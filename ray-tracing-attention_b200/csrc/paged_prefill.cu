@@ -355,7 +355,7 @@ struct Room {
   static constexpr float value = Num<T>::kBf16 ? 1.152921504606846976e18f : 16384.f;  // 2^60, 2^14
 };
 // See the list of units: kEntry blocks for a unit's beginning and end where there
-// are kFew blocks or more per CTA, else at least kLeast blocks per CTA.
+// are kFew blocks or more per CTA; without entries at least kLeast blocks per CTA.
 constexpr uint32_t kEntry = 2, kFew = 4, kLeast = 2;
 
 template <typename T, int HD>
@@ -418,9 +418,11 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
   if (tiles == 0u) return;
   // Filling and emptying the pipeline costs a unit about as much as kEntry
   // blocks: where the CTAs have several blocks each, a unit counts as that much
-  // longer, in front.  Where there are few, the units are cut evenly instead.
+  // longer, in front.  Where they have few it counts one block longer (four
+  // prompts of up to 200 rows 39 -> 32 us), or none where there are two units a
+  // K/V head at most, which are alike and are cut evenly.
   const uint64_t units = tiles * p.c.kv_heads;
-  const uint32_t entry = blocks * p.c.kv_heads >= static_cast<uint64_t>(kFew) * gridDim.x ? kEntry : 0u;
+  const uint32_t entry = blocks * p.c.kv_heads >= static_cast<uint64_t>(kFew) * gridDim.x ? kEntry : tiles > 2u ? 1u : 0u;
   const uint64_t total = blocks * p.c.kv_heads + units * entry;
   uint64_t ctas = entry ? total : (total + kLeast - 1u) / kLeast;
   if (ctas > gridDim.x) ctas = gridDim.x;
