@@ -33,6 +33,11 @@ const char* bad_pool(const rta_page_pool* p) {
   if (!aligned(p->k, 16) || !aligned(p->v, 16)) return "k and v must be 16-byte aligned";
   return nullptr;
 }
+const char* bad_batch(const rta_page_map* m, const int32_t* slots, uint32_t batch) {
+  if (batch == 0 || batch > (slots ? 0x7fffffffu : m->slots))
+    return "batch is at least 1, at most the slots without a slot list, and below 2^31";
+  return nullptr;
+}
 const char* bad_map(const rta_page_pool* p, const rta_page_map* m) {
   if (!m || !m->refs || !m->table || !m->lengths) return "null map";
   if (!m->slots || m->slots > 0x7fffffffu || !m->width) return "slots and width are at least 1";
@@ -103,7 +108,7 @@ const char* attend_params(const rta_page_pool* pool, const rta_page_map* map, ui
   if (!why) why = bad_workspace(pool, map, ws, ws_bytes);
   if (why) return why;
   if (layer >= pool->layers) return "no such layer";
-  if (batch == 0 || (!slots && batch > map->slots)) return "batch is at least 1, and at most the slots without a slot list";
+  if (const char* bad = bad_batch(map, slots, batch)) return bad;
   if (!q || !out) return "null q or out";
   if (heads == 0 || heads % pool->kv_heads || heads / pool->kv_heads > 128u)
     return "heads is a multiple of kv_heads, at most 128 query heads per K/V head";
@@ -229,8 +234,7 @@ rta_status rta_paged_append(const rta_page_pool* pool, const rta_page_map* map, 
   if (!why) why = bad_map(pool, map);
   if (!why) why = bad_workspace(pool, map, workspace, workspace_bytes);
   if (!why && layer >= pool->layers) why = "no such layer";
-  if (!why && (batch == 0 || (!slots && batch > map->slots)))
-    why = "batch is at least 1, and at most the slots without a slot list";
+  if (!why) why = bad_batch(map, slots, batch);
   if (!why && (!starts || !k || !v)) why = "null argument";
   if (!why && format != pool->format && format != RTA_F32) why = "the rows are fp32 or in the pool's format";
   if (!why) {

@@ -92,6 +92,15 @@ def _gpu():
     return torch.cuda.is_available()
 
 
+@pytest.mark.parametrize("slots", [None, BASE])
+def test_a_batch_past_31_bits_is_refused(slots):
+    """The kernels count sequences in 32 bits, some hundred at a time."""
+    if _gpu():
+        pytest.skip("made-up addresses: calls that are not refused must not reach a device")
+    status = calls(_lib.load(), pool(), pmap(), slots=slots, batch=0xffffffff)
+    assert {name for name in ROWS if status[name] == _lib.RTA_E_ARG} == ROWS
+
+
 def test_refusals_name_the_call():
     lib = _lib.load()
     assert lib.rta_paged_decode(None, None, 0, None, 1, None, 1, 4, 0, 0, 1.0, 0, 0, None, None, None, 0, None) == 1
