@@ -370,7 +370,7 @@ RTA_API rta_status rta_paged_append(const rta_page_pool* pool, const rta_page_ma
  *
  * reserve: slots[i]'s sequence grows by counts[i] >= 0 positions; the pages it
  * lacks are the lowest free ones, taken in the order of the call.  Slots are
- * distinct. */
+ * distinct; one that is named twice is flagged. */
 RTA_API rta_status rta_pages_reserve(const rta_page_pool* pool, const rta_page_map* map, const rta_page_map* out,
                                      const int32_t* slots, const int32_t* counts, uint32_t batch, void* workspace,
                                      size_t workspace_bytes, void* stream);

@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const PagesParams
   copy_map(p);
   __shared__ uint64_t part[32];
   const Plan plan(p.plan, p.pages, p.slot_count);
+  constexpr uint32_t kUnclaimed = 0xffffffffu;
   uint64_t total = 0;
   bool bad = false;
   for (uint32_t i0 = 0; i0 < p.count; i0 += kPlanThreads) {
@@ -170,37 +171,44 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const PagesParams
     uint64_t need = 0, sum;
     if (i < p.count) {
       const int32_t slot = p.a ? p.a[i] : static_cast<int32_t>(i), add = p.b[i];
+      plan.dst[i] = kUnclaimed;
       if (slot < 0 || static_cast<uint32_t>(slot) >= p.slot_count || add < 0) {
         bad = true;
       } else {
+        // a slot list may name a slot twice: the length is taken by one of them
         const int64_t n = p.map.lengths[slot];
-        if (n < 0 || n + add > static_cast<int64_t>(p.width) * p.page_size)
+        if (n < 0 || n + add > static_cast<int64_t>(p.width) * p.page_size ||
+            (p.a && atomicCAS(&p.map.lengths[slot], static_cast<int32_t>(n), -1) != n)) {
           bad = true;
-        else
+        } else {
+          plan.dst[i] = static_cast<uint32_t>(n);
           need = (n + add + p.page_size - 1) / p.page_size - (n + p.page_size - 1) / p.page_size;
+        }
       }
     }
     const uint64_t first = total + block_scan(need, part, sum) - need;
     if (i < p.count) plan.src[i] = static_cast<uint32_t>(first);
     total += sum;
   }
-  if (__syncthreads_or(bad ? 1 : 0)) {
-    if (threadIdx.x == 0) atomicOr(p.err, RTA_DEVERR_SLOT);
-    return;
-  }
-  if (total > p.pages || list_free(p.map.refs, p.pages, static_cast<uint32_t>(total), plan.list, part) < total) {
-    if (threadIdx.x == 0) atomicOr(p.err, RTA_DEVERR_POOL);
+  uint32_t wrong = __syncthreads_or(bad ? 1 : 0) ? RTA_DEVERR_SLOT : 0u;
+  if (!wrong && (total > p.pages ||
+                 list_free(p.map.refs, p.pages, static_cast<uint32_t>(total), plan.list, part) < total))
+    wrong = RTA_DEVERR_POOL;
+  if (wrong) {  // give the lengths back
+    if (p.a)
+      for (uint32_t i = threadIdx.x; i < p.count; i += kPlanThreads)
+        if (plan.dst[i] != kUnclaimed) p.map.lengths[p.a[i]] = static_cast<int32_t>(plan.dst[i]);
+    if (threadIdx.x == 0) atomicOr(p.err, wrong);
     return;
   }
   for (uint32_t k = threadIdx.x; k < total; k += kPlanThreads) p.map.refs[plan.list[k]] = 1;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   for (uint32_t i = warp; i < p.count; i += kPlanThreads / 32u) {
     const uint32_t slot = p.a ? p.a[i] : i;
-    const uint32_t n = p.map.lengths[slot], grown = n + p.b[i];
+    const uint32_t n = plan.dst[i], grown = n + p.b[i];
     const uint32_t have = (n + p.page_size - 1u) / p.page_size, need = (grown + p.page_size - 1u) / p.page_size;
     for (uint32_t j = have + lane; j < need; j += 32u)
       p.map.table[static_cast<size_t>(slot) * p.width + j] = static_cast<int32_t>(plan.list[plan.src[i] + j - have]);
-    __syncwarp();
     if (lane == 0u) p.map.lengths[slot] = static_cast<int32_t>(grown);
   }
 }

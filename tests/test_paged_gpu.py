@@ -659,6 +659,23 @@ def test_device_checks(paged):
     near(cache.decode(q[:1]), want, bound, "after the flags")
 
 
+@pytest.mark.parametrize("slots,counts", [((0, 0), (4, 4)), ((1, 2, 1), (20, 0, 20)), (tuple([2] * 1500), tuple([1] * 1500))])
+def test_reserve_of_a_slot_twice(paged, slots, counts):
+    """A slot named twice is flagged whatever its sums, and the call changes nothing."""
+    from rta_b200._lib import RtaError
+    cache = paged.PagedCache.create(1, 1600, 4, 1, 64, 1600, 32, torch.float16)
+    cache.reserve(ints(10, 5, 0))
+    before = cache.map.clone()
+    cache.reserve(ints(*counts), ints(*slots))
+    with pytest.raises(RtaError, match="word 16$"):
+        cache.check()
+    for a, b in ((before.refs, cache.map.refs), (before.table, cache.map.table), (before.lengths, cache.map.lengths)):
+        assert torch.equal(a, b)
+    cache.reserve(ints(1, 2), ints(2, 0))
+    cache.check()
+    assert cache.map.lengths[:4].tolist() == [12, 5, 1, 0] and cache.map.refs.sum().item() == 3 + 2 + 1
+
+
 def test_rows_before_the_sequence(paged):
     """More new rows than positions: the rows before position 0 see nothing."""
     cache = build(paged, [5], 2, 128, 16, torch.bfloat16, stale=math.nan)
