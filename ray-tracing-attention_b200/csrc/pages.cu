@@ -7,10 +7,12 @@
 // launch over the whole device moves the data.  The moves of a plan have
 // disjoint sources and destinations, so they run in any order.
 //
-// The moves are bound by HBM (compacting 1.85 GB of reads and writes takes 317
-// us, 5.8 TB/s; pieces of 4 KB per warp keep eight loads in flight per lane), the
-// plans by the latency of one block (9 - 15 us over some thousand pages), appended
-// rows by HBM when they are many (17,000 rows of 8 x 128 in 36 us with reserve).
+// The moves are bound by HBM (freeing half of 64 sequences and compacting, 1.85 GB
+// of reads and writes, takes 310 us with its plan; pages of 64 to 128 positions are
+// copied at 6.3 TB/s; pieces of 4 KB per warp keep eight loads in flight per lane,
+// 2 and 8 KB were slower), the plans by the latency of one block (9 - 15 us over
+// some thousand pages), appended rows by HBM when they are many (17,000 rows of
+// 8 x 128 in 36 us with reserve).
 #include "paged_device.cuh"
 
 namespace rta {
@@ -454,7 +456,16 @@ __global__ void __launch_bounds__(256) free_kernel(const PagesParams p) {
   }
 }
 
-constexpr uint32_t kMoveBlocks = 148 * 6;
+// Blocks of a move: a warp per piece, at most eight rounds of the four blocks
+// that an SM holds.  Compacting 1.85 GB took 341 us with a round and a half, 326
+// with four, 310 with eight, 305 with sixteen, forking 0.21 GB 49, 44, 44, 45 us;
+// a block without work costs 0.8 ns, so a call that can move little launches few.
+uint32_t move_blocks(const PagesParams& p, uint64_t most_moves) {
+  const uint64_t pieces = (p.page_size * p.row_bytes + kPiece - 1u) / kPiece;
+  const uint64_t blocks = (most_moves * p.layers * 2u * p.kv_heads * pieces + 7u) / 8u;
+  constexpr uint64_t kLeast = 148, kMost = 148 * 32;
+  return static_cast<uint32_t>(blocks < kLeast ? kLeast : blocks > kMost ? kMost : blocks);
+}
 
 }  // namespace
 
@@ -498,7 +509,7 @@ cudaError_t launch_reserve(const PagesParams& p, cudaStream_t s) {
 cudaError_t launch_fork(const PagesParams& p, cudaStream_t s) {
   const cudaError_t e = launch_early(fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p);
   if (e != cudaSuccess) return e;
-  return launch_early(move_kernel<kMoveFork>, dim3(kMoveBlocks), dim3(256), 0, s, p);
+  return launch_early(move_kernel<kMoveFork>, dim3(move_blocks(p, p.count)), dim3(256), 0, s, p);
 }
 cudaError_t launch_free(const PagesParams& p, cudaStream_t s) {
   return launch_early(free_kernel, dim3(p.count), dim3(256), 0, s, p);
@@ -506,12 +517,12 @@ cudaError_t launch_free(const PagesParams& p, cudaStream_t s) {
 cudaError_t launch_compact(const PagesParams& p, cudaStream_t s) {
   const cudaError_t e = launch_early(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p);
   if (e != cudaSuccess) return e;
-  return launch_early(move_kernel<kMoveCompact>, dim3(kMoveBlocks), dim3(256), 0, s, p);
+  return launch_early(move_kernel<kMoveCompact>, dim3(move_blocks(p, p.pages / 2u)), dim3(256), 0, s, p);
 }
 cudaError_t launch_copy(const PagesParams& p, cudaStream_t s) {
   const cudaError_t e = launch_early(copy_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p);
   if (e != cudaSuccess) return e;
-  return launch_early(move_kernel<kMoveCopy>, dim3(kMoveBlocks), dim3(256), 0, s, p);
+  return launch_early(move_kernel<kMoveCopy>, dim3(move_blocks(p, p.count)), dim3(256), 0, s, p);
 }
 
 }  // namespace paged
