@@ -10,14 +10,14 @@
 // row's own; they are numbered without the gap, u < firsts ? u : u + skip.
 //
 // Mathematics.  One pass over the blocks, in base 2: S = Q K^T, w = 2^(scale_log2
-// S - m), O += w V, z += sum w, with a reference m per row.  m is the maximum of
-// the first positions the row sees, and stays while a block's weights add up to
-// less than Room: a row's result is O / z whatever m is, so m only has to keep
-// the weights in range, and the maximum of later blocks is not looked for (a
-// pass over S is bounded by its exponentials and conversions).  Otherwise the
-// block is weighed again with its own maximum and O and z are scaled.  w enters
-// the second product rounded to the cache's type (its one rounding; the sum
-// takes w itself).
+// S - m + shift), O += w V, z += sum w, with a reference m per row.  m is the
+// maximum of the first positions the row sees, and stays while a block's weights
+// add up to a number within Range: a row's result is O / z whatever m is, so m
+// only has to keep the weights where their type is exact, and the maximum of
+// later blocks is not looked for (a pass over S is bounded by its exponentials
+// and conversions).  Otherwise, above the range or below it, the block is weighed
+// again with its own maximum and O and z are scaled.  w enters the second product
+// rounded to the cache's type (its one rounding; the sum takes w itself).
 //
 // Work: the blocks of all units form one list, cut evenly over the CTAs (one
 // per SM) whatever the lengths are; a lane of a unit that is cut leaves a
@@ -348,11 +348,26 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32
   }
 }
 
-// A block's weights may add up to this much (each is then below it) before the
-// row takes a new reference: fp16 weights end at 2^16, bf16 ones have fp32's range.
+// Where a block's weights may lie.  The reference weighs 2^shift; a row takes
+// the block's maximum for its new one when the weights add up to `most` or more
+// (each is below it), or to less than `least`.
+//   fp16: weights end at 65504, are exact to 2^-12 from 2^-14 on and vanish below
+//   2^-25.  shift 8 leaves 128 positions as heavy as the reference below the end,
+//   and keeps positions 15 nats under it exact; `least` is 128 times 2^-14.  A
+//   first token that scores far above all others and holds nearly nothing is
+//   common, and then those others are the result: with shift 0 and no `least` the
+//   values of 3000 positions 18 nats below it came out 15 percent off, 120 of them
+//   73, now 0.02 and 0.1.  Scores that spread by three nats take new references
+//   more often so (8192 rows of 256-dimension heads 580 -> 700 us; one nat: 520).
+//   bf16 has fp32's exponents.
 template <typename T>
-struct Room {
-  static constexpr float value = Num<T>::kBf16 ? 1.152921504606846976e18f : 16384.f;  // 2^60, 2^14
+struct Range {
+  static constexpr float shift = Num<T>::kBf16 ? 0.f : 8.f;
+  static constexpr float most = Num<T>::kBf16 ? 1.152921504606846976e18f : 65504.f;  // 2^60
+  static constexpr float least = Num<T>::kBf16 ? 0.f : 0.0078125f;                   // 2^-7
+  // a block that adds less than this of the sum so far is below what a result of
+  // its type can show, and its reference would make O and z outgrow fp32
+  static constexpr float nothing = 8.8817841970012523e-16f;  // 2^-50
 };
 // See the list of units: kEntry blocks for a unit's beginning and end where there
 // are kFew blocks or more per CTA; without entries at least kLeast blocks per CTA.
@@ -616,7 +631,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
         }
         float sum;
         for (bool again = false;;) {
-          const float base = m == -INFINITY ? 0.f : -m;
+          const float base = m == -INFINITY ? 0.f : Range<T>::shift - m;
           float zs[4][2] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
           tc_ld32(tmem_s, s[0]);
 #pragma unroll
@@ -635,15 +650,15 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
             }
           }
           sum = ((zs[0][0] + zs[0][1]) + (zs[1][0] + zs[1][1])) + ((zs[2][0] + zs[2][1]) + (zs[3][0] + zs[3][1]));
-          const bool over = !(sum < Room<T>::value);
-          if (again || !__any_sync(0xffffffffu, over)) break;
+          const bool outside = !(sum < Range<T>::most) || (sum < Range<T>::least && sum > z * Range<T>::nothing);
+          if (again || !__any_sync(0xffffffffu, outside)) break;
           const float x = largest(kKeys);
-          if (over) m = x;
+          if (outside) m = x;
           again = true;
         }
         if (!(m < INFINITY)) sum = NAN;  // a NaN or +inf score: the row has no weights
-        const bool rise = m != before;
-        const float factor = rise ? ex2(before - m) : 1.f;  // before = -inf: 0
+        const bool moved = m != before;
+        const float factor = moved ? ex2(before - m) : 1.f;  // before = -inf: 0
         z = z * factor + sum;
         tc_st32(tmem_s, w);  // the weights take the place of the scores
         tc_st32(tmem_s + 32, w + 32);
@@ -651,7 +666,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
           // O holds the blocks before this one
           // (two lanes: S of this block was computed after O of the one before)
           if (kLanes == 1 && !(ok = warp_wait(&o_done[L], (it - 1u) & 1u, p.err, stop))) break;
-          if (__any_sync(0xffffffffu, rise)) {
+          if (__any_sync(0xffffffffu, moved)) {
             tc_after();
 #pragma unroll 1
             for (uint32_t c = 0; c < HD; c += 32u) {
@@ -708,7 +723,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
           }
         }
         bad = !(odd[0] + odd[1] == 0.f);
-        if (real && p.lse) p.lse[at] = t < 0 ? -INFINITY : (m + log2f(z)) * kLn2;
+        if (real && p.lse) p.lse[at] = t < 0 ? -INFINITY : (m - Range<T>::shift + log2f(z)) * kLn2;
       } else if (rows) {
         float* const rec = p.records + (static_cast<size_t>(blockIdx.x * 2u + (first_segment ? 0u : 1u)) * kLanes + L) * S::kRecord;
         rec[r] = m;
@@ -1074,7 +1089,7 @@ __global__ void __launch_bounds__(256) prefill_join_kernel(const AttendParams p)
       uint32_t row, head;
       int32_t t;
       place(y0 + wx, row, head, t);
-      p.lse[static_cast<size_t>(row) * p.heads + head] = t < 0 ? -INFINITY : (mm + log2f(zz)) * kLn2;
+      p.lse[static_cast<size_t>(row) * p.heads + head] = t < 0 ? -INFINITY : (mm - Range<T>::shift + log2f(zz)) * kLn2;
     }
   }
   __syncthreads();

@@ -1,0 +1,79 @@
+"""GPU tests of the paged attentions at the ends of their numbers, against 64 bits.
+
+The bound is the one of test_paged_gpu.py -- |out - exact| <= A (2e + 2 u_w + 2^-20 + n 2^-28) + |exact| u_o -- where a
+weight keeps its relative rounding u_w as long as it is not far below the largest of the positions that are weighed
+together: 128 in the prefill, whose fp16 weights are multiples of 2^-32 of that largest one, 16 in the decode, whose
+fp16 pairs are multiples of 2^-39 of it.  A rounding is a quarter of a multiple in the mean, so positions 2^-34 or 2^-41
+max |v| are added.
+"""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+from test_paged_gpu import TINY, U_ONE, U_OUT, U_PAIR, attend, build, get, ints, near, put  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def paged():
+    from rta_b200 import paged as module
+    torch.cuda.init()
+    return module
+
+
+def sink(paged, dtype, n, kv_heads, dim, gap, spread, seed=0):
+    """A cache of one sequence whose position 0 scores `gap` above the others (they spread around 0) and holds zeros,
+    and a query row for it; scale 1."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    cache = build(paged, [n], kv_heads, dim, 16, dtype, seed=seed)
+    k = torch.zeros(n, kv_heads, dim, device="cuda")
+    k[:, :, 1] = torch.randn(n, kv_heads, device="cuda", generator=g) * spread
+    k[0] = 0
+    k[0, :, 0] = gap
+    v = torch.randn(n, kv_heads, dim, device="cuda", generator=g) + 8
+    v[0] = 0
+    put(cache, cache.k, 0, 0, 0, k.to(dtype))
+    put(cache, cache.v, 0, 0, 0, v.to(dtype))
+    q = torch.zeros(dim, device="cuda")
+    q[:2] = 1
+    return cache, q
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [(torch.float16, 8, 2, 128), (torch.float16, 4, 1, 256),
+                                                      (torch.float16, 4, 4, 64), (torch.bfloat16, 8, 2, 128)])
+@pytest.mark.parametrize("n", [120, 3000, 20000])
+@pytest.mark.parametrize("gap,spread", [(10.0, 0.5), (15.0, 0.0), (16.5, 0.5), (18.0, 0.0), (21.0, 1.0), (25.0, 0.0)])
+def test_prefill_behind_a_sink(paged, dtype, heads, kv_heads, dim, n, gap, spread):
+    """A first position that takes nearly all the weight and holds zeros: the result is what all the others add up to."""
+    cache, one = sink(paged, dtype, n, kv_heads, dim, gap, spread)
+    rows = min(n, 150)
+    q = one.to(dtype).expand(rows, heads, dim).contiguous()
+    out, lse = cache.prefill(q, ints(0, rows), scale=1.0, lse=True)
+    cache.check()
+    k, v = get(cache, cache.k, 0, 0, n), get(cache, cache.v, 0, 0, n)
+    want, want_lse, bound, lse_bound = attend(q, k, v, torch.arange(n - rows, n, device="cuda"), 0, 0, 1.0,
+                                              U_ONE[dtype], U_OUT[dtype], TINY[dtype])
+    held = 128 * 2.0 ** -34 * v.abs().max().item()
+    near(out, want, bound + held, "rows")
+    near(lse, want_lse, lse_bound, "lse")
+
+
+def test_prefill_of_sinks_along_the_way(paged):
+    """Positions of far larger scores now and then, with a window that loses sight of them: references rise and fall."""
+    n, dtype, dim = 2600, torch.float16, 128
+    cache, one = sink(paged, dtype, n, 2, dim, 14.0, 1.0)
+    k, v = get(cache, cache.k, 0, 0, n), get(cache, cache.v, 0, 0, n)
+    k[700::611, :, 0], v[700::611] = 17.0, 0.0
+    put(cache, cache.k, 0, 0, 0, k)
+    put(cache, cache.v, 0, 0, 0, v)
+    q = one.to(dtype).expand(n, 8, dim).contiguous()
+    for window, sinks in ((0, 0), (300, 2), (150, 0)):
+        out, lse = cache.prefill(q, ints(0, n), window=window, sinks=sinks, scale=1.0, lse=True)
+        cache.check()
+        want, want_lse, bound, lse_bound = attend(q, k, v, torch.arange(n, device="cuda"), window, sinks, 1.0,
+                                                  U_ONE[dtype], U_OUT[dtype], TINY[dtype])
+        # each position of a large score is weighed with the others of its block
+        near(out, want, bound + 128 * 2.0 ** -34 * v.abs().max().item() * 5, f"window {window}")
+        near(lse, want_lse, lse_bound, f"window {window}, lse")
