@@ -2,10 +2,12 @@
 // cache: o = sum_p softmax_p(scale q . k_p) v_p over the positions the token
 // sees (all, or a window and the first tokens).
 //
-// One pass over K and V with a running maximum m and sum z per head: a tile of
-// 16 positions gives scores s, m' = max(m, s), o' = o 2^(m - m') + sum
+// One pass over K and V with a reference m and a sum z per head: a tile of 16
+// positions gives scores s, a reference m' >= s, o' = o 2^(m - m') + sum
 // 2^(s - m') v, z' likewise; partial results (m, z, o) of the same head add up
-// the same way, so the positions are cut anywhere.
+// the same way, so the positions are cut anywhere.  m' is max(m, s), but with
+// fp16 weights a tile far below m takes its own maximum (see Num), and o and z
+// grow by 2^(m - m').
 //
 // Work: the tiles of all (sequence, K/V head, head block) units form one list;
 // every CTA takes an equal contiguous range of it, whatever the lengths are
@@ -346,9 +348,9 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, Q, HD, WARPS, STAGES, PAI
 #pragma unroll
     for (int j = 0; j < static_cast<int>(S::kWide / 8); ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     constexpr int kRows = PAIR ? 1 : 2;  // heads of this lane: g (and g + 8)
-    float m[kRows], z[kRows];
+    float m[kRows], z[kRows], top[kRows];  // top: the largest score so far
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) m[r] = -INFINITY, z[r] = 0.f;
+    for (int r = 0; r < kRows; ++r) m[r] = top[r] = -INFINITY, z[r] = 0.f;
 
     for (uint32_t i = a + group; i < e; i += kGroups) {
       while (have && issued < consumed + STAGES) issue(more);
@@ -415,7 +417,11 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, Q, HD, WARPS, STAGES, PAI
           }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = fmaxf(m[r], mx);
+        float mn = fmaxf(m[r], mx);
+        if (!N::kBf16) {
+          top[r] = fmaxf(top[r], mx);
+          if (mx < m[r] - N::kFar && mx > top[r] - N::kNothing) mn = mx;
+        }
         const float base = mn == -INFINITY ? 0.f : mn;
         rescale[r] = m[r] == mn ? 1.f : exp2f(m[r] - base);
         float sum = 0.f;

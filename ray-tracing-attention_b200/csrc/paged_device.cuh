@@ -78,9 +78,15 @@ template <typename T>
 struct Num;
 template <>
 struct Num<__half> {
-  // exp2(score - max) is scaled by 2^10: fp16 weights far below the largest
-  // stay clear of the subnormals, the sum carries the same factor.
-  static constexpr float kShift = 10.f;
+  // The decode's weights are pairs (hi, lo) of exp2(score - reference) 2^kShift,
+  // the sum carries the same factor: a pair is exact to 2^-22 from 2^-3 on and a
+  // multiple of 2^-24 below, and ends at 2^16.  A tile whose largest score is more
+  // than kFar below the reference takes its own as the new one, unless it is
+  // kNothing below the largest of all (a part of 2^-56 or less, and o and z stay
+  // within fp32 for 2^31 positions).  Behind a first token of zeros that takes all
+  // but e^-18 of the weight, 120 positions came out 3.5e-4 off with shift 10 and
+  // no kFar (fp32 results), now 1e-5.
+  static constexpr float kShift = 15.f, kFar = 12.f, kNothing = 56.f;
   static constexpr bool kBf16 = false;
   static __device__ __forceinline__ __half from(float x) { return __float2half_rn(x); }
   static __device__ __forceinline__ float to(__half x) { return __half2float(x); }
@@ -101,7 +107,7 @@ struct Num<__half> {
 };
 template <>
 struct Num<__nv_bfloat16> {
-  static constexpr float kShift = 0.f;  // bf16 has fp32's exponents
+  static constexpr float kShift = 0.f, kFar = 0.f, kNothing = 0.f;  // bf16 has fp32's exponents
   static constexpr bool kBf16 = true;
   static __device__ __forceinline__ __nv_bfloat16 from(float x) { return __float2bfloat16_rn(x); }
   static __device__ __forceinline__ float to(__nv_bfloat16 x) { return __bfloat162float(x); }

@@ -77,3 +77,39 @@ def test_prefill_of_sinks_along_the_way(paged):
         # each position of a large score is weighed with the others of its block
         near(out, want, bound + 128 * 2.0 ** -34 * v.abs().max().item() * 5, f"window {window}")
         near(lse, want_lse, lse_bound, f"window {window}, lse")
+
+
+@pytest.mark.parametrize("q32,heads,kv_heads,dim", [(True, 8, 2, 128), (True, 16, 4, 256), (False, 24, 2, 64),
+                                                    (False, 4, 4, 256)])
+@pytest.mark.parametrize("n", [20, 3000, 20000])
+@pytest.mark.parametrize("gap,spread", [(10.0, 0.5), (14.3, 0.0), (16.3, 0.0), (17.1, 0.0), (18.0, 0.5), (21.2, 0.0),
+                                        (25.0, 1.0)])
+def test_decode_behind_a_sink(paged, q32, heads, kv_heads, dim, n, gap, spread):
+    """The same for one token, whose weights enter as pairs."""
+    cache, one = sink(paged, torch.float16, n, kv_heads, dim, gap, spread)
+    dtype = torch.float32 if q32 else torch.float16
+    q = one.to(dtype).expand(1, heads, dim).contiguous()
+    out, lse = cache.decode(q, scale=1.0, lse=True)
+    cache.check()
+    k, v = get(cache, cache.k, 0, 0, n), get(cache, cache.v, 0, 0, n)
+    want, want_lse, bound, lse_bound = attend(q, k, v, torch.tensor([n - 1], device="cuda"), 0, 0, 1.0,
+                                              U_PAIR[torch.float16], U_OUT[dtype], TINY[dtype])
+    near(out, want, bound + 16 * 2.0 ** -41 * v.abs().max().item(), "token")
+    near(lse, want_lse, lse_bound, "lse")
+
+
+def test_decode_of_scores_that_jump(paged):
+    """Large scores at some positions, small ones between them, both with values: maxima rise and fall tile by tile."""
+    n, dim = 4000, 128
+    cache = build(paged, [n], 2, dim, 16, torch.float16)
+    k = torch.zeros(n, 2, dim, device="cuda")
+    k[:, :, 0] = torch.randn(n, 2, device="cuda", generator=torch.Generator("cuda").manual_seed(7)) * 12
+    put(cache, cache.k, 0, 0, 0, k.half())
+    q = torch.zeros(1, 16, dim, device="cuda")
+    q[:, :, 0] = 1
+    out, lse = cache.decode(q, scale=1.0, lse=True)
+    want, want_lse, bound, lse_bound = attend(q, get(cache, cache.k, 0, 0, n), get(cache, cache.v, 0, 0, n),
+                                              torch.tensor([n - 1], device="cuda"), 0, 0, 1.0, U_PAIR[torch.float16],
+                                              U_OUT[torch.float32], TINY[torch.float32])
+    near(out, want, bound, "token")
+    near(lse, want_lse, lse_bound, "lse")
