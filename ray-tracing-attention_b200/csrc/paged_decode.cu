@@ -51,7 +51,10 @@ __device__ __forceinline__ Cut& cut_of(const AttendParams& p, uint32_t cta) {
 
 // PAIR: rows g and g + 8 of the MMA are the two 16-bit halves of head g's
 // operand (x = T(x) + T(x - T(x))), so weights, and fp32 queries, enter with
-// about twice the bits of T at no extra MMA; up to 8 heads per unit.
+// about twice the bits of T at no extra MMA; up to 8 heads per unit.  fp32
+// queries are scaled first, by the power of two that puts a warp's largest of a
+// head at 2^14 to 2^15 (their scores by its inverse): both halves are then within
+// fp16's range whatever the queries' size is, with 22 bits down to 2^-18 of it.
 // Otherwise 16 heads per unit and the weights' lower half is a second MMA.
 template <typename T, typename Q, int HD, int WARPS, int STAGES, bool PAIR>
 struct Shape {
@@ -322,13 +325,30 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, Q, HD, WARPS, STAGES, PAI
 
     // Query fragments (A operand: rows are heads, k is the dimension).
     uint32_t qa[kSteps][4];
+    float back = 1.f;  // undoes the scaling of fp32 queries
     {
       const Q* q0 = reinterpret_cast<const Q*>(smem + S::kRing + (segment & 1u) * S::kQueries) + g * HD + part * S::kWide + 2u * t4;
+      float up = 1.f;
+      if (sizeof(Q) == 4) {
+        float big = 0.f;
+#pragma unroll
+        for (uint32_t x = 0; x < 2u * kSteps; ++x) {
+          const float2 y = two(q0 + x * 8u);
+          big = fmaxf(big, fmaxf(fabsf(y.x), fabsf(y.y)));
+        }
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        const uint32_t e = __float_as_uint(big) >> 23;  // 127 + floor(log2); 255: an infinity, left as it is
+        const uint32_t f = e == 255u ? 127u : min(127u + 14u + 127u - e, 253u);
+        up = __uint_as_float(f << 23);
+        back = __uint_as_float((254u - f) << 23);
+      }
 #pragma unroll
       for (uint32_t kk = 0; kk < kSteps; ++kk)
 #pragma unroll
         for (uint32_t h = 0; h < 2u; ++h) {
-          const float2 x = two(q0 + kk * 16u + h * 8u);
+          float2 x = two(q0 + kk * 16u + h * 8u);
+          if (sizeof(Q) == 4) x = make_float2(x.x * up, x.y * up);
           qa[kk][2u * h] = N::pack(x.x, x.y);
           if (PAIR) {
             if (sizeof(Q) == 4) {
@@ -384,6 +404,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, Q, HD, WARPS, STAGES, PAI
           for (int x = 0; x < 2; ++x) {
             pr[r][c][x] = sc[0][c][2 * r + x] + sc[1][c][2 * r + x];
             if (PAIR) pr[r][c][x] += sc[0][c][2 + x] + sc[1][c][2 + x];
+            if (sizeof(Q) == 4) pr[r][c][x] *= back;
           }
       if (kParts == 2) {
         // two buffers taken in turn: the other warp has read one before this

@@ -113,3 +113,22 @@ def test_decode_of_scores_that_jump(paged):
                                               U_OUT[torch.float32], TINY[torch.float32])
     near(out, want, bound, "token")
     near(lse, want_lse, lse_bound, "lse")
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 4, 256), (6, 2, 128), (24, 2, 64)])
+@pytest.mark.parametrize("size", [1e-35, 1e-20, 1e-6, 2.0 ** -7, 1.0, 1e4, 7e4, 1e6, 1e30])
+def test_decode_queries_of_any_size(paged, heads, kv_heads, dim, size):
+    """fp32 queries past both ends of fp16's range, the scale making up for it; each head of another size."""
+    lengths = [700, 3]
+    cache = build(paged, lengths, kv_heads, dim, 16, torch.float16)
+    q = torch.randn(2, heads, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) * size
+    q[:, ::2] *= 2.0 ** -9  # smaller by another factor, exactly
+    q[1, 1] = 0
+    scale = dim ** -0.5 / size
+    out = cache.decode(q, scale=scale)
+    cache.check()
+    for b, n in enumerate(lengths):
+        want, _, bound, _ = attend(q[b:b + 1], get(cache, cache.k, 0, b, n), get(cache, cache.v, 0, b, n),
+                                   torch.tensor([n - 1], device="cuda"), 0, 0, scale, U_PAIR[torch.float16],
+                                   U_OUT[torch.float32], 1e-37)
+        near(out[b:b + 1], want, bound, f"sequence {b}")
