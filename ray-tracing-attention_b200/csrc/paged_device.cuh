@@ -107,7 +107,9 @@ struct Num<__half> {
 };
 template <>
 struct Num<__nv_bfloat16> {
-  static constexpr float kShift = 0.f, kFar = 0.f, kNothing = 0.f;  // bf16 has fp32's exponents
+  // bf16 has fp32's exponents, and so have its values: weights of 2^-44 at most
+  // leave room for the sum of 2^31 of the largest.
+  static constexpr float kShift = -44.f, kFar = 0.f, kNothing = 0.f;
   static constexpr bool kBf16 = true;
   static __device__ __forceinline__ __nv_bfloat16 from(float x) { return __float2bfloat16_rn(x); }
   static __device__ __forceinline__ float to(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -224,7 +226,7 @@ __device__ void row_alone(const AttendParams& p, uint32_t slot, uint32_t kv, uin
     s = warp_sum(s) * p.scale_log2;
     const float mn = fmaxf(m, s);
     const float base = mn == -INFINITY ? 0.f : mn;
-    const float f = m == mn ? 1.f : exp2f(m - base), w = exp2f(s - base);
+    const float f = m == mn ? 1.f : exp2f(m - base), w = exp2f(s - (base - Num<T>::kShift));
     z = z * f + w;
 #pragma unroll
     for (int i = 0; i < E; ++i) o[i] = o[i] * f + w * v[i];
@@ -234,7 +236,7 @@ __device__ void row_alone(const AttendParams& p, uint32_t slot, uint32_t kv, uin
   T* out = static_cast<T*>(p.out) + at * HD + lane * E;
 #pragma unroll
   for (int i = 0; i < E; ++i) out[i] = Num<T>::from(o[i] / z);
-  if (p.lse && lane == 0u) p.lse[at] = (m + log2f(z)) * kLn2;
+  if (p.lse && lane == 0u) p.lse[at] = (m - Num<T>::kShift + log2f(z)) * kLn2;
 }
 
 }  // namespace paged

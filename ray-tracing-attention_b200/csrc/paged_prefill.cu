@@ -359,12 +359,16 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32
 //   values of 3000 positions 18 nats below it came out 15 percent off, 120 of them
 //   73, now 0.02 and 0.1.  Scores that spread by three nats take new references
 //   more often so (8192 rows of 256-dimension heads 580 -> 700 us; one nat: 520).
-//   bf16 has fp32's exponents.
+//   bf16 has fp32's exponents, and so have its values: 2^24 blocks (2^31
+//   positions) below 2^-24 add up to less than 1, so O stays below the largest
+//   value.  A later block may weigh 2^30 times the reference (2^20 made ragged
+//   prompts 234 instead of 220 us where scores spread by five nats), and what lies
+//   2^72 below it vanishes.
 template <typename T>
 struct Range {
-  static constexpr float shift = Num<T>::kBf16 ? 0.f : 8.f;
-  static constexpr float most = Num<T>::kBf16 ? 1.152921504606846976e18f : 65504.f;  // 2^60
-  static constexpr float least = Num<T>::kBf16 ? 0.f : 0.0078125f;                   // 2^-7
+  static constexpr float shift = Num<T>::kBf16 ? -54.f : 8.f;
+  static constexpr float most = Num<T>::kBf16 ? 5.9604644775390625e-8f : 65504.f;  // 2^-24
+  static constexpr float least = Num<T>::kBf16 ? 0.f : 0.0078125f;                 // 2^-7
   // a block that adds less than this of the sum so far is below what a result of
   // its type can show, and its reference would make O and z outgrow fp32
   static constexpr float nothing = 8.8817841970012523e-16f;  // 2^-50

@@ -132,3 +132,44 @@ def test_decode_queries_of_any_size(paged, heads, kv_heads, dim, size):
                                    torch.tensor([n - 1], device="cuda"), 0, 0, scale, U_PAIR[torch.float16],
                                    U_OUT[torch.float32], 1e-37)
         near(out[b:b + 1], want, bound, f"sequence {b}")
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (4, 1, 256), (40, 2, 64)])
+@pytest.mark.parametrize("top", [0.0, 12.0, 35.0, 80.0])
+def test_values_near_the_largest(paged, heads, kv_heads, dim, top):
+    """bf16 values of 3e38 and scores that rise by `top`: the mean of finite values is finite."""
+    n, dtype = 900, torch.bfloat16
+    cache = build(paged, [n], kv_heads, dim, 32, dtype)
+    k = torch.zeros(n, kv_heads, dim, device="cuda")
+    k[:, :, 0] = torch.linspace(0, top, n, device="cuda")[:, None]
+    put(cache, cache.k, 0, 0, 0, k.to(dtype))
+    put(cache, cache.v, 0, 0, 0, torch.full((n, kv_heads, dim), 3e38, device="cuda").to(dtype))
+    q = torch.zeros(n, heads, dim, device="cuda", dtype=dtype)
+    q[:, :, 0] = 1
+    out, lse = cache.prefill(q, ints(0, n), scale=1.0, lse=True)
+    cache.check()
+    want, want_lse, bound, lse_bound = attend(q, get(cache, cache.k, 0, 0, n), get(cache, cache.v, 0, 0, n),
+                                              torch.arange(n, device="cuda"), 0, 0, 1.0, U_ONE[dtype], U_OUT[dtype],
+                                              TINY[dtype])
+    near(out, want, bound, "prefill")
+    near(lse, want_lse, lse_bound, "lse")
+    one, lse = cache.decode(q[-1:], scale=1.0, lse=True)
+    near(one, want[-1:], bound[-1:], "decode")
+    near(lse, want_lse[-1:], lse_bound[-1:], "lse of decode")
+
+
+def test_values_near_the_largest_beside_nan(paged):
+    """The same for rows that are computed by themselves: the last position, which they do not see, holds NaN."""
+    n, dtype, dim = 300, torch.bfloat16, 128
+    cache = build(paged, [n], 2, dim, 32, dtype)
+    v = torch.full((n, 2, dim), 3e38, device="cuda").to(dtype)
+    put(cache, cache.v, 0, 0, 0, v)
+    q = torch.randn(n, 8, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(3)).to(dtype)
+    put(cache, cache.v, 0, 0, n - 1, torch.full((1, 2, dim), math.nan, device="cuda", dtype=dtype))
+    out, lse = cache.prefill(q, ints(0, n), lse=True)
+    cache.check()
+    want, want_lse, bound, lse_bound = attend(q, get(cache, cache.k, 0, 0, n), v, torch.arange(n, device="cuda"), 0, 0,
+                                              dim ** -0.5, U_ONE[dtype], U_OUT[dtype], TINY[dtype])
+    near(out[:-1], want[:-1], bound[:-1], "rows")
+    near(lse, want_lse, lse_bound, "lse")
+    assert torch.isnan(out[-1]).all()
