@@ -540,8 +540,9 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     const uint32_t L = warp >> 2, quarter = warp & 3u, r = quarter * 32u + lane;
     const uint32_t lane_addr = quarter * 32u << 16, tmem_o = tmem + lane_addr + kTmemO + L * HD;
     const uint32_t q_smem = smem_u32(smem) + L * S::kQ;
-    // 0: all weights equal; a negative one: the MMA negates the queries
-    const float scale = p.scale_log2 == 0.f ? 1e-30f : fabsf(p.scale_log2);
+    // 0: all weights equal (the smallest number, since -inf times it is still -inf);
+    // a negative one: the MMA negates the queries
+    const float scale = p.scale_log2 == 0.f ? 1.4e-45f : fabsf(p.scale_log2);
     uint32_t it = 0;  // blocks of this lane
     bool ok = true, first_segment = true;
     // the queries of a lane, a row at a time, 16 bytes per thread

@@ -173,3 +173,16 @@ def test_values_near_the_largest_beside_nan(paged):
     near(out[:-1], want[:-1], bound[:-1], "rows")
     near(lse, want_lse, lse_bound, "lse")
     assert torch.isnan(out[-1]).all()
+
+
+def test_a_scale_of_zero_weighs_all_alike(paged):
+    """Products of 1e32 times a scale of zero are zero."""
+    n, dim, dtype = 200, 64, torch.bfloat16
+    cache = build(paged, [n], 2, dim, 32, dtype)
+    put(cache, cache.k, 0, 0, 0, (torch.randn(n, 2, dim, device="cuda") * 1e16).to(dtype))
+    q = (torch.randn(n, 4, dim, device="cuda") * 1e16).to(dtype)
+    out = cache.prefill(q, ints(0, n), scale=0.0)
+    cache.check()
+    want, _, bound, _ = attend(q, get(cache, cache.k, 0, 0, n), get(cache, cache.v, 0, 0, n),
+                               torch.arange(n, device="cuda"), 0, 0, 0.0, U_ONE[dtype], U_OUT[dtype], TINY[dtype])
+    near(out, want, bound, "rows")
