@@ -21,7 +21,9 @@
 //
 // Work: the blocks of all units form one list, cut evenly over the CTAs (one
 // per SM) whatever the lengths are; a lane of a unit that is cut leaves a
-// record (m, z, O) per CTA, which a second launch joins in order, many CTAs to a unit.
+// record (m, z, O) per CTA, which a second launch joins in order, many CTAs to a
+// unit.  That launch also computes rows by themselves (see row_alone) that are not
+// finite beside values they do not see: nobody waits for them there.
 //
 // Roles (all waits bounded):
 //   softmax    four warps per lane, a thread per row: load Q, take S from
@@ -78,7 +80,9 @@ struct Shape {
 
 constexpr uint32_t kTmemO = 256;  // tensor-memory column of O (S buffers at 0 and 128)
 
-// A unit that begins in a CTA's range and ends in another's: at most one per CTA.
+// What the second launch has to know of a CTA: the unit that begins in its range
+// and ends in another's (at most one), and whether units that it wrote by itself,
+// which follow one another, have rows that are not finite.
 struct Cut {
   uint32_t parts;   // CTAs that hold a part of it, from this one on; 0: no such unit
   uint32_t rows;
@@ -86,7 +90,10 @@ struct Cut {
   uint32_t first_row, R0, kv, slot;
   int32_t past;
   uint32_t firsts, low, high;
+  uint32_t bad;                           // units from the first whole one to the last with such a row; 0: none
+  uint32_t whole_b, whole_kv, whole_tile;  // the first whole one
 };
+static_assert(sizeof(Cut) <= kCutBytes, "a description's room in the workspace");
 __device__ __forceinline__ Cut& cut_of(const AttendParams& p, uint32_t cta) {
   return *reinterpret_cast<Cut*>(static_cast<uint8_t*>(p.cuts) + cta * kCutBytes);
 }
@@ -416,7 +423,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
   }
 
   pdl_wait();
-  if (threadIdx.x == 0) *reinterpret_cast<uint2*>(&cut_of(p, blockIdx.x)) = make_uint2(0u, 0u);
+  if (threadIdx.x == 0) cut_of(p, blockIdx.x).parts = cut_of(p, blockIdx.x).bad = 0u;
 
   // ---- the list of units and this CTA's range --------------------------------
   uint64_t blocks = 0, tiles = 0, own = 0, own_upto = 0, own_tiles_upto = 0;  // own: this thread's (last) sequence
@@ -544,6 +551,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     // a negative one: the MMA negates the queries
     const float scale = p.scale_log2 == 0.f ? 1.4e-45f : fabsf(p.scale_log2);
     uint32_t it = 0;  // blocks of this lane
+    uint32_t wholes = 0;  // units this CTA wrote by itself
     bool ok = true, first_segment = true;
     // the queries of a lane, a row at a time, 16 bytes per thread
     const auto load_queries = [&](const Unit& v) {
@@ -761,12 +769,17 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
           cut.high = u.seen + u.skip;
         }
       }
-      uint32_t again = __ballot_sync(0xffffffffu, bad && real && t >= 0);
-      while (again) {  // see row_alone
-        const int x = __ffs(again) - 1;
-        again &= again - 1u;
-        const uint32_t tx = __shfl_sync(0xffffffffu, t, x), hx = __shfl_sync(0xffffffffu, head, x), rx = __shfl_sync(0xffffffffu, row, x);
-        if (spoiled<T, HD>(p, u.slot, u.kv, u.firsts, u.firsts + u.skip, u.seen + u.skip, tx)) row_alone<T, HD>(p, u.slot, u.kv, hx, rx, tx);
+      if (whole) {
+        Cut& cut = cut_of(p, blockIdx.x);
+        if (wholes == 0u && threadIdx.x == 0u) {
+          cut.whole_b = u.b;
+          cut.whole_kv = u.kv;
+          cut.whole_tile = u.tile;
+        }
+        ++wholes;
+        // (the second launch looks at them: alone, a row of a long history takes
+        // longer than the other warps' waits are bounded by)
+        if (__any_sync(0xffffffffu, bad && real && t >= 0) && lane == 0) atomicMax(&cut.bad, wholes);
       }
       first_segment = false;
     }
@@ -1020,6 +1033,35 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
+// Rows of a CTA's whole units that are not finite, by row_alone: a warp per row.
+template <typename T, int HD>
+__device__ __forceinline__ void look_again(const AttendParams& p, const volatile Cut& cut, uint32_t units) {
+  using S = Shape<HD>;
+  const uint32_t lane = threadIdx.x & 31u;
+  Unit u;
+  load_sequence<HD>(p, cut.whole_b, u, nullptr);
+  u.kv = cut.whole_kv;
+  set_tile<HD>(p, u, cut.whole_tile);
+  for (uint32_t k = 0;;) {
+    const uint32_t R0 = u.tile * S::kRows, rows = min(S::kRows, u.rows - R0);
+    for (uint32_t y = blockIdx.y * 8u + (threadIdx.x >> 5); y < rows; y += gridDim.y * 8u) {
+      const uint32_t i = (R0 + y) / p.group, row = u.first_row + i, head = u.kv * p.group + (R0 + y) % p.group;
+      const int32_t t = u.past + static_cast<int32_t>(i);
+      if (t < 0) continue;
+      float o[HD / 32];
+      load_dims<T, HD>(static_cast<const T*>(p.out) + (static_cast<size_t>(row) * p.heads + head) * HD, lane, o);
+      bool bad = false;
+#pragma unroll
+      for (int x = 0; x < HD / 32; ++x) bad |= !isfinite(o[x]);
+      if (__any_sync(0xffffffffu, bad) &&
+          spoiled<T, HD>(p, u.slot, u.kv, u.firsts, u.firsts + u.skip, u.seen + u.skip, static_cast<uint32_t>(t)))
+        row_alone<T, HD>(p, u.slot, u.kv, head, row, static_cast<uint32_t>(t));
+    }
+    if (++k == units) return;
+    next_unit<HD>(p, u);
+  }
+}
+
 // Joins the records of cut units: blockIdx.x is the CTA in whose range the unit
 // begins, blockIdx.y some of its rows.  O = sum_j 2^(m_j - max m) O_j over
 // sum_j 2^(m_j - max m) z_j.  It is bound by latency: every possible piece has a
@@ -1028,7 +1070,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) prefill_kernel(const A
 template <int HD>
 constexpr uint32_t join_rows() { return 2048u / HD; }  // a thread for eight dimensions of a row
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) prefill_join_kernel(const AttendParams p) {
+__device__ __forceinline__ void join_cut(const AttendParams& p, const Cut& cut) {
   using S = Shape<HD>;
   using N = Num<T>;
   constexpr uint32_t kRows = join_rows<HD>();
@@ -1037,9 +1079,6 @@ __global__ void __launch_bounds__(256) prefill_join_kernel(const AttendParams p)
   constexpr uint32_t kAhead = 4;
   __shared__ float weight[kMaxCtas][kRows];
   __shared__ uint32_t bad_rows;
-  pdl_wait();
-  pdl_launch_dependents();
-  const Cut cut = cut_of(p, blockIdx.x);
   const uint32_t y0 = blockIdx.y * kRows;  // first row within the unit
   if (cut.parts == 0u || y0 >= cut.rows) return;
   const uint32_t L = y0 / kLaneRows, r0 = y0 % kLaneRows;
@@ -1136,6 +1175,17 @@ __global__ void __launch_bounds__(256) prefill_join_kernel(const AttendParams p)
     if (spoiled<T, HD>(p, cut.slot, cut.kv, cut.firsts, cut.low, cut.high, static_cast<uint32_t>(t)))
       row_alone<T, HD>(p, cut.slot, cut.kv, head, row, static_cast<uint32_t>(t));
   }
+}
+
+// (Two blocks per SM: 128 registers.  The compiler's own 64 or 80 spilled what is
+// on its way: 64 rows over 2048 positions 33 us instead of 20.)
+template <typename T, int HD>
+__global__ void __launch_bounds__(256, 2) prefill_join_kernel(const AttendParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const Cut cut = cut_of(p, blockIdx.x);
+  join_cut<T, HD>(p, cut);
+  if (cut.bad) look_again<T, HD>(p, *const_cast<volatile Cut*>(&cut_of(p, blockIdx.x)), cut.bad);
 }
 
 // Tensor maps of the call's layer, if pages hold whole boxes of at least 32
