@@ -366,7 +366,8 @@ RTA_API rta_status rta_paged_append(const rta_page_pool* pool, const rta_page_ma
 
 /* Bookkeeping.  Each call reads `map` and leaves the result in `out`, which is
  * `map` itself or a map of the same slots and width with arrays of its own.
- * A call whose check fails on the device changes nothing (out = map).
+ * A call whose check fails on the device changes nothing (out = map); the one
+ * exception is a bad page that free meets.
  *
  * reserve: slots[i]'s sequence grows by counts[i] >= 0 positions; the pages it
  * lacks are the lowest free ones, taken in the order of the call.  Slots are
@@ -381,7 +382,10 @@ RTA_API rta_status rta_pages_fork(const rta_page_pool* pool, const rta_page_map*
                                   const int32_t* src, const int32_t* dst, uint32_t count, void* workspace,
                                   size_t workspace_bytes, void* stream);
 /* free: refs - 1 for every page of the slots, their table entries -1, their
- * lengths 0.  (A page without references is flagged and left at 0.) */
+ * lengths 0.  A slot named twice is freed once; a bad slot or length is flagged
+ * and frees none of the call's.  (A page without references is flagged and left
+ * at 0, a table entry outside the pool is flagged; the sequence is freed all the
+ * same, so that its slot can be used again.) */
 RTA_API rta_status rta_pages_free(const rta_page_pool* pool, const rta_page_map* map, const rta_page_map* out,
                                   const int32_t* slots, uint32_t count, void* workspace, size_t workspace_bytes,
                                   void* stream);

@@ -436,34 +436,43 @@ __global__ void __launch_bounds__(256) move_kernel(const PagesParams p) {
   }
 }
 
+// Every block looks over all of the call's slots before it frees its own, so none
+// is freed where one is bad: a bad slot or length is not written by any block, and
+// a length that another block has set to 0 already is a good one.
+constexpr uint32_t kFreeBlocks = 592;  // at most, four per SM
 __global__ void __launch_bounds__(256) free_kernel(const PagesParams p) {
   pdl_wait();
   pdl_launch_dependents();
   __shared__ int32_t length;
-  const int32_t slot = p.a[blockIdx.x];
-  if (slot < 0 || static_cast<uint32_t>(slot) >= p.slot_count) {
-    if (threadIdx.x == 0) atomicOr(p.err, RTA_DEVERR_SLOT);
+  bool bad = false;
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < p.count; i += blockDim.x) {
+    const int32_t slot = p.a[i];
+    const bool real = slot >= 0 && static_cast<uint32_t>(slot) < p.slot_count;
+    const int32_t n = real ? p.map.lengths[slot] : -1;
+    bad |= n < 0 || static_cast<uint32_t>(n) > p.width * p.page_size;
+  }
+  if (__syncthreads_or(bad)) {
+    if (blockIdx.x == 0u && threadIdx.x == 0) atomicOr(p.err, RTA_DEVERR_SLOT);
     return;
   }
-  if (threadIdx.x == 0) length = atomicExch(&p.map.lengths[slot], 0);  // a slot named twice is freed once
-  __syncthreads();
-  const int32_t n = length;
-  if (n <= 0) {
-    if (n < 0 && threadIdx.x == 0) atomicOr(p.err, RTA_DEVERR_SLOT);
-    return;
-  }
-  uint32_t held = (static_cast<uint32_t>(n) + p.page_size - 1u) / p.page_size;
-  if (held > p.width) held = p.width;
-  for (uint32_t j = threadIdx.x; j < held; j += blockDim.x) {
-    int32_t* cell = p.map.table + static_cast<size_t>(slot) * p.width + j;
-    const int32_t page = *cell;
-    *cell = -1;
-    if (static_cast<uint32_t>(page) >= p.pages) {
-      atomicOr(p.err, RTA_DEVERR_PAGE);
-    } else if (atomicSub(&p.map.refs[page], 1) <= 0) {
-      atomicAdd(&p.map.refs[page], 1);
-      atomicOr(p.err, RTA_DEVERR_PAGE);
+  for (uint32_t i = blockIdx.x; i < p.count; i += gridDim.x) {
+    const int32_t slot = p.a[i];
+    if (threadIdx.x == 0) length = atomicExch(&p.map.lengths[slot], 0);  // a slot named twice is freed once
+    __syncthreads();
+    const uint32_t held = (static_cast<uint32_t>(length) + p.page_size - 1u) / p.page_size;
+    for (uint32_t j = threadIdx.x; j < held; j += blockDim.x) {
+      int32_t* cell = p.map.table + static_cast<size_t>(slot) * p.width + j;
+      const int32_t page = *cell;
+      *cell = -1;
+      if (static_cast<uint32_t>(page) >= p.pages) {
+        atomicOr(p.err, RTA_DEVERR_PAGE);
+      } else if (atomicSub(&p.map.refs[page], 1) <= 0) {
+        atomicAdd(&p.map.refs[page], 1);
+        atomicOr(p.err, RTA_DEVERR_PAGE);
+      }
     }
+    __syncthreads();  // length has been read
   }
 }
 
@@ -523,7 +532,7 @@ cudaError_t launch_fork(const PagesParams& p, cudaStream_t s) {
   return launch_early(move_kernel<kMoveFork>, dim3(move_blocks(p, p.count)), dim3(256), 0, s, p);
 }
 cudaError_t launch_free(const PagesParams& p, cudaStream_t s) {
-  return launch_early(free_kernel, dim3(p.count), dim3(256), 0, s, p);
+  return launch_early(free_kernel, dim3(p.count < kFreeBlocks ? p.count : kFreeBlocks), dim3(256), 0, s, p);
 }
 cudaError_t launch_compact(const PagesParams& p, cudaStream_t s) {
   const cudaError_t e = launch_early(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p);

@@ -1,0 +1,77 @@
+"""GPU tests: a bookkeeping call of the paged cache that finds something wrong changes nothing."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+from test_paged_gpu import Model, ints  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def paged():
+    from rta_b200 import paged as module
+    torch.cuda.init()
+    return module
+
+
+def flagged(cache, bits, call):
+    """The call raises `bits` and leaves the map and the pools as they were; so it does into another map."""
+    from rta_b200._lib import RtaError
+    before, k, v = cache.map.clone(), cache.k.clone(), cache.v.clone()
+    other = cache.map.clone()
+    other.table.fill_(77)
+    for into in (None, other):
+        got = call(into)
+        with pytest.raises(RtaError, match=f"word {bits}$"):
+            cache.check()
+        for m in {cache.map, got}:
+            assert torch.equal(m.refs, before.refs) and torch.equal(m.table, before.table)
+            assert torch.equal(m.lengths, before.lengths)
+        assert torch.equal(cache.k, k) and torch.equal(cache.v, v)
+
+
+def small(paged, lengths=(10, 5, 8, 0, 0), pages=12, layers=2, slots=None, width=8):
+    """Pages of four positions, each filled with its own number."""
+    cache = paged.PagedCache.create(layers, pages, 4, 1, 64, slots or len(lengths), 4 * width, torch.float16)
+    for pool, sign in ((cache.k, 1), (cache.v, -1)):
+        pool.copy_((torch.arange(pages, device="cuda") * sign).view(1, -1, 1, 1, 1).expand_as(pool))
+    cache.reserve(ints(*lengths))
+    cache.check()
+    return cache
+
+
+@pytest.mark.parametrize("slots", [(0, 9), (9, 0), (0, 1, -1), (2, 5, 0, 1), (1, 2 ** 31 - 1)])
+def test_free_with_a_bad_slot_frees_none(paged, slots):
+    cache = small(paged)
+    flagged(cache, 16, lambda out: cache.free(ints(*slots), out=out))
+    model = Model(cache)
+    cache.free(ints(0, 1))
+    model.free([0, 1])
+    cache.check()
+    model.same(cache.map)
+
+
+@pytest.mark.parametrize("length", [-1, -2 ** 31, 33, 2 ** 31 - 1])
+def test_free_with_a_bad_length_frees_none(paged, length):
+    cache = small(paged)
+    cache.map.lengths[1] = length
+    flagged(cache, 16, lambda out: cache.free(ints(0, 1, 2), out=out))
+    flagged(cache, 16, lambda out: cache.free(ints(1), out=out))
+
+
+def test_free_of_many(paged):
+    """More slots than a block has threads, and than blocks are launched; one bad one among them, then none."""
+    slots, pages = 3000, 3100
+    cache = paged.PagedCache.create(1, pages, 4, 1, 64, slots, 8, torch.float16)
+    cache.reserve(ints(*[1 + i % 4 if i % 5 else 0 for i in range(slots)]))
+    cache.check()
+    for bad in (0, 1700, slots - 1):
+        which = list(range(slots))
+        which[bad] = slots
+        flagged(cache, 16, lambda out: cache.free(ints(*which), out=out))
+    model = Model(cache)
+    which = list(range(0, slots, 2)) + [4, 6]  # named twice: freed once
+    cache.free(ints(*which))
+    model.free(which)
+    cache.check()
+    model.same(cache.map)
