@@ -377,7 +377,9 @@ RTA_API rta_status rta_pages_reserve(const rta_page_pool* pool, const rta_page_m
                                      size_t workspace_bytes, void* stream);
 /* fork: the empty slot dst[i] becomes a copy of src[i]: full pages are shared
  * (refs + 1), the positions of a partly filled last page are copied, in every
- * layer, to the lowest free page.  dst are distinct and none of them a src. */
+ * layer, to the lowest free page.  dst are distinct and none of them a src; a
+ * source whose entries name a page outside the pool or one without references is
+ * flagged. */
 RTA_API rta_status rta_pages_fork(const rta_page_pool* pool, const rta_page_map* map, const rta_page_map* out,
                                   const int32_t* src, const int32_t* dst, uint32_t count, void* workspace,
                                   size_t workspace_bytes, void* stream);

@@ -226,8 +226,26 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const PagesParams
   }
 }
 
-// Claims the destinations, ranks the partly filled last pages, takes a page
-// for each; the launch after it shares the full pages and copies the rest.
+// Whether the first `held` entries of a row name pages of the pool that are in
+// use, by a warp.
+__device__ bool row_good(const PagesParams& p, const int32_t* row, uint32_t held) {
+  constexpr uint32_t kMany = 8;  // entries per lane and step
+  bool good = true;
+  for (uint32_t j0 = threadIdx.x & 31u; j0 < held; j0 += 32u * kMany) {
+    int32_t page[kMany], refs[kMany];
+#pragma unroll
+    for (uint32_t k = 0; k < kMany; ++k) page[k] = j0 + k * 32u < held ? row[j0 + k * 32u] : row[j0];
+#pragma unroll
+    for (uint32_t k = 0; k < kMany; ++k) refs[k] = static_cast<uint32_t>(page[k]) < p.pages ? p.map.refs[page[k]] : 0;
+#pragma unroll
+    for (uint32_t k = 0; k < kMany; ++k) good &= refs[k] > 0;
+  }
+  return __all_sync(0xffffffffu, good);
+}
+
+// Claims the destinations, looks at the sources' pages, ranks the partly filled
+// last ones, takes a page for each; the launch after it shares the full pages and
+// copies the rest.
 __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagesParams p) {
   pdl_wait();
   pdl_launch_dependents();
@@ -259,9 +277,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagesPara
       } else {
         const uint32_t rest = static_cast<uint32_t>(n) % p.page_size;
         if (rest) {
-          const int32_t page = p.map.table[static_cast<size_t>(src) * p.width + static_cast<uint32_t>(n) / p.page_size];
-          if (static_cast<uint32_t>(page) >= p.pages) atomicOr(&fault, RTA_DEVERR_PAGE);
-          plan.src[i] = static_cast<uint32_t>(page);
+          plan.src[i] = static_cast<uint32_t>(p.map.table[static_cast<size_t>(src) * p.width + static_cast<uint32_t>(n) / p.page_size]);
           need = 1u;
         }
         plan.held[i] = rest;
@@ -270,6 +286,14 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagesPara
     const uint64_t first = total + block_scan(need, part, sum) - need;
     if (i < p.count) plan.dst[i] = static_cast<uint32_t>(first);
     total += sum;
+  }
+  __syncthreads();
+  if (!fault) {  // every source is a sequence
+    __syncthreads();
+    for (uint32_t i = threadIdx.x >> 5; i < p.count; i += kPlanThreads / 32u) {
+      const uint32_t src = p.a[i], held = (static_cast<uint32_t>(p.map.lengths[src]) + p.page_size - 1u) / p.page_size;
+      if (!row_good(p, p.map.table + static_cast<size_t>(src) * p.width, held)) atomicOr(&fault, RTA_DEVERR_PAGE);
+    }
   }
   __syncthreads();
   uint32_t wrong = fault;
@@ -370,7 +394,7 @@ __global__ void __launch_bounds__(256) move_kernel(const PagesParams p) {
   const uint64_t me = static_cast<uint64_t>(blockIdx.x) * 8u + (threadIdx.x >> 5);
   const uint32_t moves = *plan.moves;
   if (KIND == kMoveFork) {
-    for (uint64_t i = me; i < moves; i += warps) {  // share the full pages, end the row
+    for (uint64_t i = me; i < moves; i += warps) {  // share the full pages (the plan has looked at them), end the row
       const uint32_t src = p.a[i], dst = p.b[i], rest = plan.held[i];
       const uint32_t full = static_cast<uint32_t>(p.map.lengths[src]) / p.page_size;
       const int32_t* from = p.map.table + static_cast<size_t>(src) * p.width;
@@ -379,10 +403,7 @@ __global__ void __launch_bounds__(256) move_kernel(const PagesParams p) {
         int32_t page = -1;
         if (j < full) {
           page = from[j];
-          if (static_cast<uint32_t>(page) < p.pages)
-            atomicAdd(&p.map.refs[page], 1);
-          else
-            atomicOr(p.err, RTA_DEVERR_PAGE);
+          atomicAdd(&p.map.refs[page], 1);
         } else if (j == full && rest) {
           page = static_cast<int32_t>(plan.dst[i]);
         }

@@ -75,3 +75,36 @@ def test_free_of_many(paged):
     model.free(which)
     cache.check()
     model.same(cache.map)
+
+
+@pytest.mark.parametrize("entry", [-1, 12, 10 ** 6, -2 ** 31])
+@pytest.mark.parametrize("where", [0, 1])
+def test_fork_of_a_bad_page_changes_nothing(paged, entry, where):
+    """A full page of the source that is no page of the pool."""
+    cache = small(paged)
+    cache.map.table[0, where] = entry
+    flagged(cache, 4, lambda out: cache.fork(ints(1, 0), ints(3, 4), out=out))
+
+
+@pytest.mark.parametrize("j", [0, 1, 2])
+def test_fork_of_a_free_page_changes_nothing(paged, j):
+    """A page of the source, full or the last, that nothing refers to: it could be handed out by the same call."""
+    cache = small(paged)
+    cache.map.refs[cache.map.table[0, j].item()] = 0
+    flagged(cache, 4, lambda out: cache.fork(ints(1, 0), ints(3, 4), out=out))
+
+
+def test_fork_of_long_tables(paged):
+    """More full pages than the plan reads at a time; one bad one far along."""
+    cache = paged.PagedCache.create(1, 5000, 1, 1, 64, 4, 4000, torch.float16)
+    cache.reserve(ints(3900, 1000))
+    cache.check()
+    was = cache.map.table[0, 3700].item()
+    cache.map.table[0, 3700] = -5
+    flagged(cache, 4, lambda out: cache.fork(ints(1, 0), ints(2, 3), out=out))
+    cache.map.table[0, 3700] = was
+    model = Model(cache)
+    cache.fork(ints(1, 0, ), ints(2, 3))
+    model.fork([1, 0], [2, 3])
+    cache.check()
+    model.same(cache.map)
