@@ -393,8 +393,9 @@ RTA_API rta_status rta_pages_free(const rta_page_pool* pool, const rta_page_map*
                                   void* stream);
 /* compact: with L pages in use, the k-th free page below L takes the data (of
  * every layer), references and table entries of the k-th page in use from L
- * on; afterwards pages 0 .. L - 1 are the ones in use.  live (device, may be
- * NULL) receives L. */
+ * on; afterwards pages 0 .. L - 1 are the ones in use.  A table entry that names
+ * a page outside the pool or one without references is flagged.  live (device,
+ * may be NULL) receives L, of a flagged call too. */
 RTA_API rta_status rta_pages_compact(const rta_page_pool* pool, const rta_page_map* map, const rta_page_map* out,
                                      uint32_t* live, void* workspace, size_t workspace_bytes, void* stream);
 /* copy: page dst[i] takes the data of page src[i] in every layer (device

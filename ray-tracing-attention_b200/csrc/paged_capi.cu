@@ -145,8 +145,9 @@ bool same_map(const rta_page_map* a, const rta_page_map* b) {
 }
 
 // Checks a bookkeeping call, fills its parameters, and has map copied to out when
-// they are two maps: by the call's plan where it can, else by a launch.
-rta_status pages_params(const char* fn, bool plan, const rta_page_pool* pool, const rta_page_map* map, const rta_page_map* out,
+// they are two maps: by a launch, by the call's plan where that can, or by the call.
+enum Copies { kByLaunch, kByPlan, kByCall };
+rta_status pages_params(const char* fn, Copies by, const rta_page_pool* pool, const rta_page_map* map, const rta_page_map* out,
                         uint32_t count, void* ws, size_t ws_bytes, cudaStream_t s, paged::PagesParams& p) {
   const char* why = bad_pool(pool);
   if (!why) why = bad_map(pool, map);
@@ -180,7 +181,7 @@ rta_status pages_params(const char* fn, bool plan, const rta_page_pool* pool, co
   p.err = w.err;
   p.plan = static_cast<uint32_t*>(w.body);
   if (same_map(map, out)) return RTA_OK;
-  if (plan && paged::plan_copies(pool->pages, map->slots, map->width)) {
+  if (by == kByCall || (by == kByPlan && paged::plan_copies(pool->pages, map->slots, map->width))) {
     p.from = {map->refs, map->table, map->lengths};
     return RTA_OK;
   }
@@ -262,7 +263,7 @@ rta_status rta_pages_reserve(const rta_page_pool* pool, const rta_page_map* map,
   if (!counts || !batch) return refuse("rta_pages_reserve", "null counts or an empty batch");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   paged::PagesParams p;
-  const rta_status st = pages_params("rta_pages_reserve", true, pool, map, out, batch, workspace, workspace_bytes, s, p);
+  const rta_status st = pages_params("rta_pages_reserve", kByPlan, pool, map, out, batch, workspace, workspace_bytes, s, p);
   if (st != RTA_OK) return st;
   p.a = slots;
   p.b = counts;
@@ -275,7 +276,7 @@ rta_status rta_pages_fork(const rta_page_pool* pool, const rta_page_map* map, co
   if (!src || !dst || !count) return refuse("rta_pages_fork", "null src or dst, or nothing to fork");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   paged::PagesParams p;
-  const rta_status st = pages_params("rta_pages_fork", true, pool, map, out, count, workspace, workspace_bytes, s, p);
+  const rta_status st = pages_params("rta_pages_fork", kByPlan, pool, map, out, count, workspace, workspace_bytes, s, p);
   if (st != RTA_OK) return st;
   p.a = src;
   p.b = dst;
@@ -288,7 +289,7 @@ rta_status rta_pages_free(const rta_page_pool* pool, const rta_page_map* map, co
   if (!slots || !count) return refuse("rta_pages_free", "null slots or nothing to free");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   paged::PagesParams p;
-  const rta_status st = pages_params("rta_pages_free", false, pool, map, out, count, workspace, workspace_bytes, s, p);
+  const rta_status st = pages_params("rta_pages_free", kByLaunch, pool, map, out, count, workspace, workspace_bytes, s, p);
   if (st != RTA_OK) return st;
   p.a = slots;
   return status(paged::launch_free(p, s), "rta_pages_free");
@@ -298,7 +299,7 @@ rta_status rta_pages_compact(const rta_page_pool* pool, const rta_page_map* map,
                              uint32_t* live, void* workspace, size_t workspace_bytes, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   paged::PagesParams p;
-  const rta_status st = pages_params("rta_pages_compact", true, pool, map, out, 0, workspace, workspace_bytes, s, p);
+  const rta_status st = pages_params("rta_pages_compact", kByCall, pool, map, out, 0, workspace, workspace_bytes, s, p);
   if (st != RTA_OK) return st;
   p.live = live;
   return status(paged::launch_compact(p, s), "rta_pages_compact");

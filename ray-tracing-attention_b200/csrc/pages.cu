@@ -103,15 +103,17 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
 }
 
 // ------------------------------------------------------------------ plans
-// Scratch words of a plan: [0] moves, then per move source page, destination
+// Scratch words of a plan: [0] moves, [1] live pages, [8 ..] what the blocks of a
+// compact's look over the map have found; then per move source page, destination
 // page and positions, then the free-page list, or for compact the map of moved
 // pages.
-constexpr uint32_t kPlanHead = 8;
+constexpr uint32_t kLookBlocks = 296, kPlanHead = 8 + kLookBlocks;
 struct Plan {
-  uint32_t *moves, *src, *dst, *held, *list;
+  uint32_t *moves, *found, *src, *dst, *held, *list;
   __device__ __forceinline__ Plan(uint32_t* w, uint32_t pages, uint32_t slots) {
     const uint32_t most = pages > slots ? pages : slots;
     moves = w;
+    found = w + 8;
     src = w + kPlanHead;
     dst = src + most;
     held = dst + most;
@@ -317,15 +319,49 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagesPara
   if (threadIdx.x == 0) *plan.moves = p.count;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagesParams p) {
+// Before a compact: whether every entry of the tables names a page of the pool
+// that is in use (each block notes what it has found), and the copy of the map
+// where the result goes into another one.
+__global__ void __launch_bounds__(256) compact_look_kernel(const PagesParams p) {
   pdl_wait();
   pdl_launch_dependents();
-  copy_map(p);
+  const Plan plan(p.plan, p.pages, p.slot_count);
+  const bool copy = p.from.refs != nullptr;
+  const MapArrays from = copy ? p.from : p.map;
+  const uint64_t stride = static_cast<uint64_t>(gridDim.x) * blockDim.x, cells = static_cast<uint64_t>(p.slot_count) * p.width;
+  const uint64_t t = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  bool bad = false;
+#pragma unroll 4
+  for (uint64_t i = t; i < cells; i += stride) {
+    const int32_t page = from.table[i];
+    if (copy) p.map.table[i] = page;
+    if (page >= 0) bad |= static_cast<uint32_t>(page) >= p.pages || from.refs[page] <= 0;
+  }
+  if (copy) {
+    for (uint64_t i = t; i < p.pages; i += stride) p.map.refs[i] = from.refs[i];
+    for (uint64_t i = t; i < p.slot_count; i += stride) p.map.lengths[i] = from.lengths[i];
+  }
+  const uint32_t any = __syncthreads_or(bad);
+  if (threadIdx.x == 0) plan.found[blockIdx.x] = any;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagesParams p, const uint32_t look_blocks) {
+  pdl_wait();
+  pdl_launch_dependents();
   __shared__ uint64_t part[32];
   const Plan plan(p.plan, p.pages, p.slot_count);
+  const bool wrong = __syncthreads_or(threadIdx.x < look_blocks && plan.found[threadIdx.x]);
   uint64_t mine = 0, live;
   for (uint32_t i = threadIdx.x; i < p.pages; i += kPlanThreads) mine += p.map.refs[i] > 0 ? 1u : 0u;
   block_scan(mine, part, live);
+  if (wrong) {
+    if (threadIdx.x == 0) {
+      *plan.moves = 0u;
+      if (p.live) *p.live = static_cast<uint32_t>(live);
+      atomicOr(p.err, RTA_DEVERR_PAGE);
+    }
+    return;
+  }
   uint64_t holes = 0, movers = 0;
   for (uint32_t p0 = 0; p0 < p.pages; p0 += kPlanThreads * 4u) {
     const uint32_t i = p0 + threadIdx.x * 4u;
@@ -336,7 +372,6 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagesP
         const bool used = p.map.refs[i + k] > 0;
         if (!used && i + k < live) hole |= 1u << k;
         if (used && i + k >= live) mover |= 1u << k;
-        if (!used && i + k >= live) plan.list[i + k] = 0xffffffffu;  // no table entry should name it
       }
     uint64_t sum;  // both ranks in one scan: holes in the low half, movers in the high half
     const uint64_t n = __popc(hole) | static_cast<uint64_t>(__popc(mover)) << 32;
@@ -411,18 +446,12 @@ __global__ void __launch_bounds__(256) move_kernel(const PagesParams p) {
       }
     }
   }
-  if (KIND == kMoveCompact) {
+  if (KIND == kMoveCompact && moves) {
     const uint32_t live = plan.moves[1];
     const uint64_t cells = static_cast<uint64_t>(p.slot_count) * p.width;
     for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < cells; i += warps * 32u) {
       const int32_t page = p.map.table[i];
-      if (page >= 0 && static_cast<uint32_t>(page) >= live) {
-        const uint32_t to = static_cast<uint32_t>(page) < p.pages ? plan.list[page] : 0xffffffffu;
-        if (to != 0xffffffffu)
-          p.map.table[i] = static_cast<int32_t>(to);
-        else
-          atomicOr(p.err, RTA_DEVERR_PAGE);
-      }
+      if (page >= 0 && static_cast<uint32_t>(page) >= live) p.map.table[i] = static_cast<int32_t>(plan.list[page]);  // a moved one
     }
   }
   // (move, layer, K or V, head, piece of the head's positions)
@@ -556,7 +585,11 @@ cudaError_t launch_free(const PagesParams& p, cudaStream_t s) {
   return launch_early(free_kernel, dim3(p.count < kFreeBlocks ? p.count : kFreeBlocks), dim3(256), 0, s, p);
 }
 cudaError_t launch_compact(const PagesParams& p, cudaStream_t s) {
-  const cudaError_t e = launch_early(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p);
+  const uint64_t blocks = (static_cast<uint64_t>(p.slot_count) * p.width + 1023u) / 1024u;  // four entries a thread
+  const uint32_t look = static_cast<uint32_t>(blocks < kLookBlocks ? blocks : kLookBlocks);
+  cudaError_t e = launch_early(compact_look_kernel, dim3(look), dim3(256), 0, s, p);
+  if (e != cudaSuccess) return e;
+  e = launch_early(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p, look);
   if (e != cudaSuccess) return e;
   return launch_early(move_kernel<kMoveCompact>, dim3(move_blocks(p, p.pages / 2u)), dim3(256), 0, s, p);
 }

@@ -108,3 +108,40 @@ def test_fork_of_long_tables(paged):
     model.fork([1, 0], [2, 3])
     cache.check()
     model.same(cache.map)
+
+
+def holes(paged, **kw):
+    """Slots 0 and 2 hold pages behind free ones: compact has something to move."""
+    cache = small(paged, **kw)
+    cache.free(ints(1))
+    cache.check()
+    return cache
+
+
+@pytest.mark.parametrize("entry,bits", [(99, 4), (12, 4), (3, 4), (7, 4), (11, 4)])
+@pytest.mark.parametrize("width", [8, 9000])
+def test_compact_of_a_bad_entry_changes_nothing(paged, entry, bits, width):
+    """Table entries past the pool, of the hole that another page would move to (3, 4 and the pages from 7 on are free
+    once slot 1 is gone), and of a free page behind the live ones; maps that one block copies and larger ones."""
+    cache = holes(paged, width=width)
+    assert cache.map.refs.tolist() == [1, 1, 1, 0, 0, 1, 1, 0, 0, 0, 0, 0]
+    cache.map.table[3, 1] = entry
+    flagged(cache, bits, lambda out: cache.compact(out=out))
+    cache.map.table[3, 1] = -1
+    model = Model(cache)
+    assert model.compact() == 5
+    cache.compact()
+    cache.check()
+    model.same(cache.map)
+    assert cache.k[0, :5, 0, 0, 0].tolist() == [0, 1, 2, 5, 6]
+
+
+def test_compact_flagged_tells_no_count(paged):
+    """The count of a call that changes nothing is the count of pages in use all the same."""
+    from rta_b200._lib import RtaError
+    cache, live = holes(paged), ints(-7)
+    cache.map.table[3, 1] = 4
+    cache.compact(live=live)
+    with pytest.raises(RtaError, match="word 4$"):
+        cache.check()
+    assert live.item() == 5
