@@ -399,7 +399,8 @@ RTA_API rta_status rta_pages_free(const rta_page_pool* pool, const rta_page_map*
 RTA_API rta_status rta_pages_compact(const rta_page_pool* pool, const rta_page_map* map, const rta_page_map* out,
                                      uint32_t* live, void* workspace, size_t workspace_bytes, void* stream);
 /* copy: page dst[i] takes the data of page src[i] in every layer (device
- * arrays, at most `pages` of them; no dst is a src, and dst are distinct). */
+ * arrays, at most `pages` of them; no dst is a src, and dst are distinct).  A
+ * page outside the pool is flagged, and none is copied. */
 RTA_API rta_status rta_pages_copy(const rta_page_pool* pool, const int32_t* src, const int32_t* dst, uint32_t count,
                                   void* workspace, size_t workspace_bytes, void* stream);
 

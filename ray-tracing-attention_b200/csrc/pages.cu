@@ -404,15 +404,19 @@ __global__ void __launch_bounds__(kPlanThreads) copy_plan_kernel(const PagesPara
   pdl_wait();
   pdl_launch_dependents();
   const Plan plan(p.plan, p.pages, p.slot_count);
+  bool bad = false;
   for (uint32_t i = threadIdx.x; i < p.count; i += kPlanThreads) {
     const uint32_t s = p.a[i], d = p.b[i];
-    const bool ok = s < p.pages && d < p.pages;
-    if (!ok) atomicOr(p.err, RTA_DEVERR_PAGE);
-    plan.src[i] = ok ? s : 0u;
-    plan.dst[i] = ok ? d : 0u;
-    plan.held[i] = ok ? p.page_size : 0u;
+    bad |= s >= p.pages || d >= p.pages;
+    plan.src[i] = s;
+    plan.dst[i] = d;
+    plan.held[i] = p.page_size;
   }
-  if (threadIdx.x == 0) *plan.moves = p.count;
+  bad = __syncthreads_or(bad);
+  if (threadIdx.x == 0) {
+    *plan.moves = bad ? 0u : p.count;
+    if (bad) atomicOr(p.err, RTA_DEVERR_PAGE);
+  }
 }
 
 // ------------------------------------------------------------------ moves

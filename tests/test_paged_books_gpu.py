@@ -145,3 +145,9 @@ def test_compact_flagged_tells_no_count(paged):
     with pytest.raises(RtaError, match="word 4$"):
         cache.check()
     assert live.item() == 5
+
+
+@pytest.mark.parametrize("src,dst", [((1, 12), (0, 3)), ((-1, 1), (0, 3)), ((1, 2), (12, 3)), ((1, 2), (3, -1))])
+def test_copy_with_a_bad_page_copies_none(paged, src, dst):
+    cache = small(paged)
+    flagged(cache, 4, lambda out: cache.copy_pages(ints(*src), ints(*dst)) or cache.map)
