@@ -1177,10 +1177,11 @@ __device__ __forceinline__ void join_cut(const AttendParams& p, const Cut& cut) 
   }
 }
 
-// (Two blocks per SM: 128 registers.  The compiler's own 64 or 80 spilled what is
-// on its way: 64 rows over 2048 positions 33 us instead of 20.)
+// (Registers for three or two blocks per SM: with the compiler's own choice what is
+// on its way was spilled, 64 rows over 2048 positions took 33 us instead of 20; for
+// two where three fit, ragged batches of 128-dimension heads 214 instead of 211.)
 template <typename T, int HD>
-__global__ void __launch_bounds__(256, 2) prefill_join_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(256, HD == 64 ? 2 : 3) prefill_join_kernel(const AttendParams p) {
   pdl_wait();
   pdl_launch_dependents();
   const Cut cut = cut_of(p, blockIdx.x);
