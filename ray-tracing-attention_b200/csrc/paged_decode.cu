@@ -20,8 +20,8 @@
 // 16-byte copies two tiles ahead, across the ends of units; the page of a tile is looked up
 // one tile before its copies; the next unit's queries are copied while this
 // one's tiles are read.  Measured: 64 sequences of 128 to 8192 positions, 16 / 4
-// heads x 256 fp16, 176 us (1.1 GB at 6.2 TB/s, 96 % of a copy's rate), 100
-// windowed ones, 32 / 8 x 128 bf16, 234 us (99 %); one of 32768 positions 32 us,
+// heads x 256 fp16, 178 us (1.1 GB at 6.2 TB/s, 94 % of a copy's rate), 100
+// windowed ones, 32 / 8 x 128 bf16, 234 us (99 %); one of 32768 positions 33 us,
 // of which about 10 are the way to the first tile and the joining launch.
 #include <atomic>
 #include <mutex>
@@ -222,8 +222,16 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, Q, HD, WARPS, STAGES, PAI
     while (at < end) {
       if (++next.u.pr == per_seq) {
         next.u.pr = 0;
-        do visible(p, sequence(p.c, ++next.u.b, nullptr), next.u);
-        while (next.u.tiles == 0u);
+        visible(p, sequence(p.c, ++next.u.b, nullptr), next.u);
+        if (next.u.tiles == 0u) {  // the next sequence with anything to see, a warp's 32 at a time
+          uint32_t b = next.u.b + 1u, some = 0;
+          for (; b < p.c.batch; b += 32u) {
+            some = __ballot_sync(0xffffffffu, b + lane < p.c.batch && sequence(p.c, b + lane, nullptr).length != 0u);
+            if (some) break;
+          }
+          next.u.b = b + __ffs(some) - 1u;
+          visible(p, sequence(p.c, next.u.b, nullptr), next.u);
+        }
       }
       if (take(next, 0u)) return true;
     }

@@ -39,9 +39,9 @@
 // head_dim 256: one lane, two S buffers, so that S of the next block is
 // computed under this block's softmax; 64 and 128: two lanes take turns.
 //
-// Measured: 8192 rows of 16 / 4 heads x 256 fp16 604 us sustained (0.91 PFLOP/s
+// Measured: 8192 rows of 16 / 4 heads x 256 fp16 605 us sustained (0.91 PFLOP/s
 // of visible pairs; K and V come out of L2 at 128 KB per block and SM, which
-// bounds it), seven ragged prompts of 32 / 8 x 128 bf16 234 us (0.71 PFLOP/s; a
+// bounds it), seven ragged prompts of 32 / 8 x 128 bf16 232 us (0.72 PFLOP/s; a
 // lane's chain of products and exponentials bounds it, the tensor pipe is 41 %
 // active), 64 rows over 2048 positions 20 us (latency).
 #include <atomic>
@@ -142,6 +142,7 @@ __device__ __forceinline__ void set_tile(const AttendParams& p, Unit& u, uint32_
   u.seen = seen_by(p, u, R1 - 1u);
   u.blocks = blocks_of(u.seen);
 }
+// By a whole warp; there is a next unit.
 template <int HD>
 __device__ __forceinline__ void next_unit(const AttendParams& p, Unit& u) {
   if (u.tile + 1u < u.tiles) {
@@ -150,8 +151,16 @@ __device__ __forceinline__ void next_unit(const AttendParams& p, Unit& u) {
   }
   if (++u.kv == p.c.kv_heads) {
     u.kv = 0;
-    do load_sequence<HD>(p, u.b + 1u, u, nullptr);
-    while (u.tiles == 0u);
+    load_sequence<HD>(p, u.b + 1u, u, nullptr);
+    if (u.tiles == 0u) {  // the next sequence with new rows, a warp's 32 at a time: other roles wait meanwhile
+      uint32_t b = u.b + 1u, some = 0, first;
+      for (; b < p.c.batch; b += 32u) {
+        const uint32_t l = b + (threadIdx.x & 31u);
+        some = __ballot_sync(0xffffffffu, l < p.c.batch && new_rows(p, l, first, nullptr) != 0u);
+        if (some) break;
+      }
+      load_sequence<HD>(p, b + __ffs(some) - 1u, u, nullptr);
+    }
   }
   set_tile<HD>(p, u, 0u);
 }
@@ -365,7 +374,8 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32
 //   common, and then those others are the result: with shift 0 and no `least` the
 //   values of 3000 positions 18 nats below it came out 15 percent off, 120 of them
 //   73, now 0.02 and 0.1.  Scores that spread by three nats take new references
-//   more often so (8192 rows of 256-dimension heads 580 -> 700 us; one nat: 520).
+//   more often so (8192 rows of 256-dimension heads 580 -> 700 us; one nat: 520 before and after;
+//   one input over and over).
 //   bf16 has fp32's exponents, and so have its values: 2^24 blocks (2^31
 //   positions) below 2^-24 add up to less than 1, so O stays below the largest
 //   value.  A later block may weigh 2^30 times the reference (2^20 made ragged
