@@ -332,10 +332,13 @@ RTA_API size_t rta_paged_workspace_bytes(const rta_page_pool* pool, const rta_pa
  *   out[b][h] = sum_p softmax_p(scale q[b][h] . k_p) v_p, K/V head
  *   h / (heads / kv_heads);  lse[b][h] = log sum_p exp(scale q . k_p)
  * q: element (b, h, d) at q + b * q_row_stride + h * q_head_stride + d, 16-byte
- * aligned rows, q_format the pool's format, or RTA_F32 with an RTA_F16 pool;
+ * aligned rows, q_format the pool's format, or RTA_F32 with an RTA_F16 pool (of
+ * any size: they are scaled before they are split into two fp16 halves);
  * out [batch][heads][head_dim] contiguous (16-byte aligned) in q's format; lse [batch][heads]
- * fp32 or NULL.  A sequence of length 0 gives zeros and lse -inf.  heads is a
- * multiple of kv_heads, at most 128 query heads per K/V head. */
+ * fp32 or NULL.  A sequence of length 0 gives zeros and lse -inf, and so does a
+ * bad slot, which is flagged.  heads is a multiple of kv_heads, at most 128 query
+ * heads per K/V head.  Where a visible K or V value is not finite, neither is the
+ * result (whether it is an infinity or NaN is not defined). */
 RTA_API rta_status rta_paged_decode(const rta_page_pool* pool, const rta_page_map* map, uint32_t layer,
                                     const int32_t* slots, uint32_t batch, const void* q, int q_format, uint32_t heads,
                                     uint64_t q_row_stride, uint64_t q_head_stride, float scale, uint32_t window,
@@ -346,9 +349,11 @@ RTA_API rta_status rta_paged_decode(const rta_page_pool* pool, const rta_page_ma
  * starts[b] .. starts[b + 1] - 1 (device, batch + 1 entries, ascending from 0
  * to rows), already written to the pages and counted in lengths; row i of m
  * sits at position t = lengths[slot] - m + i.  q_format is the pool's format;
- * out [rows][heads][head_dim] (32-byte aligned), lse [rows][heads].  A row before position 0
- * (more new rows than the sequence is long) gives zeros and lse -inf.  What a
- * row does not see never reaches it, non-finite values included. */
+ * out [rows][heads][head_dim] (32-byte aligned, not over q: rows that are looked
+ * at again read their queries once more), lse [rows][heads].  A row before position 0
+ * (more new rows than the sequence is long) gives zeros and lse -inf, and so do
+ * the rows of a bad slot.  Rows that belong to no sequence are flagged and not
+ * written.  What a row does not see never reaches it, non-finite values included. */
 RTA_API rta_status rta_paged_prefill(const rta_page_pool* pool, const rta_page_map* map, uint32_t layer,
                                      const int32_t* slots, uint32_t batch, const int32_t* starts, uint32_t rows,
                                      const void* q, int q_format, uint32_t heads, uint64_t q_row_stride,

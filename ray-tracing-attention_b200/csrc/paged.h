@@ -58,7 +58,7 @@ struct AttendParams {
   void* out;
   float* lse;
   uint32_t* err;
-  void* cuts;  // [kMaxCtas] units that are cut, of kCutBytes each
+  void* cuts;  // [kMaxDecodeCtas, the larger of the two] what the second launch has to know, kCutBytes each
   float* records;
 };
 constexpr uint32_t kCutBytes = 64;

@@ -4,15 +4,16 @@
 // Everything is decided on the device (no call waits for the host): one block
 // plans -- it ranks free pages, holes and movers with block-wide sums, so the
 // choice is the lowest page first, whatever the order of threads -- and a
-// launch over the whole device moves the data.  The moves of a plan have
-// disjoint sources and destinations, so they run in any order.
+// launch over the whole device moves the data.  What a call checks is checked
+// before anything is written.  The moves of a plan have disjoint sources and
+// destinations, so they run in any order.
 //
 // The moves are bound by HBM (freeing half of 64 sequences and compacting, 1.85 GB
-// of reads and writes, takes 310 us with its plan; pages of 64 to 128 positions are
+// of reads and writes, takes 319 us with its plan; pages of 64 to 128 positions are
 // copied at 6.3 TB/s; pieces of 4 KB per warp keep eight loads in flight per lane,
-// 2 and 8 KB were slower), the plans by the latency of one block (9 - 15 us over
-// some thousand pages), appended rows by HBM when they are many (17,000 rows of
-// 8 x 128 in 31 us with reserve).
+// 2 and 8 KB were slower), the plans by the latency of one block (8 - 15 us over
+// some thousand pages, more over larger pools), appended rows by HBM when they are
+// many (17,000 rows of 8 x 128 in 33 us with reserve).
 #include "paged_device.cuh"
 
 namespace rta {
@@ -531,9 +532,10 @@ __global__ void __launch_bounds__(256) free_kernel(const PagesParams p) {
 }
 
 // Blocks of a move: a warp per piece, at most eight rounds of the four blocks
-// that an SM holds.  Compacting 1.85 GB took 341 us with a round and a half, 326
-// with four, 310 with eight, 305 with sixteen, forking 0.21 GB 49, 44, 44, 45 us;
-// a block without work costs 0.8 ns, so a call that can move little launches few.
+// that each of the 148 SMs holds.  Compacting 1.85 GB took 341 us with a round and
+// a half, 326 with four, 310 with eight, 305 with sixteen, forking 0.21 GB 49, 44,
+// 44, 45 us (one input over and over; changing ones take 319 and 49 with eight); a
+// block without work costs 0.8 ns, so a call that can move little launches few.
 uint32_t move_blocks(const PagesParams& p, uint64_t most_moves) {
   const uint64_t pieces = (p.page_size * p.row_bytes + kPiece - 1u) / kPiece;
   const uint64_t blocks = (most_moves * p.layers * 2u * p.kv_heads * pieces + 7u) / 8u;
@@ -551,7 +553,7 @@ size_t plan_bytes(uint32_t pages, uint32_t slots) {
 cudaError_t launch_append(const AppendParams& in, int fmt, int in_fmt, cudaStream_t s) {
   if (in.rows == 0u) return cudaSuccess;
   AppendParams p = in;
-  // kAhead pieces per thread, fewer while that leaves SMs idle
+  // kAhead pieces per thread, fewer while that leaves SMs (148, two blocks each) idle
   const uint32_t per_row = p.c.kv_heads * p.c.head_dim / 4u;
   p.block_rows = per_row >= 256u * kAhead ? 1u : 256u * kAhead / per_row;
   if (p.block_rows > kBlockRows) p.block_rows = kBlockRows;

@@ -146,7 +146,8 @@ class PagedCache:
                 window: int = 0, sinks: int = 0, scale: float | None = None, out: torch.Tensor | None = None,
                 lse: bool = False, map: PageMap | None = None):
         """Attention of the newest tokens of each sequence (rta_paged_prefill): rows starts[b] .. starts[b + 1] - 1 of
-        q [rows, heads, head_dim] are sequence b's, its last ones.  The rest as in decode; q in the cache's type."""
+        q [rows, heads, head_dim] are sequence b's, its last ones.  The rest as in decode; q in the cache's type, out
+        not over q.  Rows that `starts` gives to no sequence are flagged and not written."""
         rows, heads, fmt, row, head = self._q(q)
         out, l = self._out(q, out, lse)
         window, sinks = self._reach(window, sinks)
