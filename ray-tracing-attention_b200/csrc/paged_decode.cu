@@ -20,8 +20,8 @@
 // 16-byte copies two tiles ahead, across the ends of units; the page of a tile is looked up
 // one tile before its copies; the next unit's queries are copied while this
 // one's tiles are read.  Measured: 64 sequences of 128 to 8192 positions, 16 / 4
-// heads x 256 fp16, 178 us (1.1 GB at 6.2 TB/s, 94 % of a copy's rate), 100
-// windowed ones, 32 / 8 x 128 bf16, 234 us (99 %); one of 32768 positions 33 us,
+// heads x 256 fp16, 177 us (1.1 GB at 6.2 TB/s, 95 % of a copy's rate), 100
+// windowed ones, 32 / 8 x 128 bf16, 233 us (99 %); one of 32768 positions 33 us,
 // of which about 10 are the way to the first tile and the joining launch.
 #include <atomic>
 #include <mutex>

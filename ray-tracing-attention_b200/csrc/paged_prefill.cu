@@ -39,10 +39,10 @@
 // head_dim 256: one lane, two S buffers, so that S of the next block is
 // computed under this block's softmax; 64 and 128: two lanes take turns.
 //
-// Measured: 8192 rows of 16 / 4 heads x 256 fp16 605 us sustained (0.91 PFLOP/s
+// Measured: 8192 rows of 16 / 4 heads x 256 fp16 595 us sustained (0.92 PFLOP/s
 // of visible pairs; K and V come out of L2 at 128 KB per block and SM, which
-// bounds it), seven ragged prompts of 32 / 8 x 128 bf16 232 us (0.72 PFLOP/s; a
-// lane's chain of products and exponentials bounds it, the tensor pipe is 41 %
+// bounds it), seven ragged prompts of 32 / 8 x 128 bf16 226 us (0.73 PFLOP/s; a
+// lane's chain of products and exponentials bounds it, the tensor pipe is 43 %
 // active), 64 rows over 2048 positions 20 us (latency).
 #include <atomic>
 #include <mutex>
@@ -374,8 +374,8 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32
 //   common, and then those others are the result: with shift 0 and no `least` the
 //   values of 3000 positions 18 nats below it came out 15 percent off, 120 of them
 //   73, now 0.02 and 0.1.  Scores that spread by three nats take new references
-//   more often so (8192 rows of 256-dimension heads 580 -> 700 us; one nat: 520 before and after;
-//   one input over and over).
+//   more often so (8192 rows of 256-dimension heads 580 -> 700 us; by one nat 520
+//   before and after; one input over and over).
 //   bf16 has fp32's exponents, and so have its values: 2^24 blocks (2^31
 //   positions) below 2^-24 add up to less than 1, so O stays below the largest
 //   value.  A later block may weigh 2^30 times the reference (2^20 made ragged

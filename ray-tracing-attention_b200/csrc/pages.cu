@@ -9,7 +9,7 @@
 // destinations, so they run in any order.
 //
 // The moves are bound by HBM (freeing half of 64 sequences and compacting, 1.85 GB
-// of reads and writes, takes 319 us with its plan; pages of 64 to 128 positions are
+// of reads and writes, takes 316 us with its plan; pages of 64 to 128 positions are
 // copied at 6.3 TB/s; pieces of 4 KB per warp keep eight loads in flight per lane,
 // 2 and 8 KB were slower), the plans by the latency of one block (8 - 15 us over
 // some thousand pages, more over larger pools), appended rows by HBM when they are
@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(256) free_kernel(const PagesParams p) {
 // Blocks of a move: a warp per piece, at most eight rounds of the four blocks
 // that each of the 148 SMs holds.  Compacting 1.85 GB took 341 us with a round and
 // a half, 326 with four, 310 with eight, 305 with sixteen, forking 0.21 GB 49, 44,
-// 44, 45 us (one input over and over; changing ones take 319 and 49 with eight); a
+// 44, 45 us (one input over and over; changing ones take 316 and 48 with eight); a
 // block without work costs 0.8 ns, so a call that can move little launches few.
 uint32_t move_blocks(const PagesParams& p, uint64_t most_moves) {
   const uint64_t pieces = (p.page_size * p.row_bytes + kPiece - 1u) / kPiece;

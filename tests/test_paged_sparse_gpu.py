@@ -42,3 +42,30 @@ def test_sequences_far_apart(batch, active):
         row += n
     one[list(active)] = 0
     assert not one.any()
+
+
+def test_a_bad_slot_gives_zeros():
+    """Sequences of a slot that is none are flagged and see nothing; the others are as they were."""
+    from rta_b200._lib import RtaError
+    from rta_b200.paged import PagedCache
+    cache = PagedCache.create(1, 8, 16, 2, 64, 3, 32, torch.float16)
+    cache.reserve(ints(20, 7, 0))
+    k = torch.randn(27, 2, 64, device="cuda").half()
+    cache.append(k, k * 2, ints(0, 20, 27, 27))
+    q = torch.randn(9, 4, 64, device="cuda").half()
+    starts, slots = ints(0, 3, 5, 9), ints(0, 3, 1)
+    good, good_lse = cache.prefill(q[[0, 1, 2, 5, 6, 7, 8]], ints(0, 3, 7), slots=ints(0, 1), lse=True)
+    one, one_lse = cache.decode(q[:2], slots=ints(0, 1), lse=True)
+    cache.check()
+    for bad in (3, -1):
+        slots[1] = bad
+        out, lse = cache.prefill(q, starts, slots=slots, out=torch.full_like(q, 7), lse=True)
+        with pytest.raises(RtaError, match="word 16$"):
+            cache.check()
+        assert torch.equal(out[[0, 1, 2, 5, 6, 7, 8]], good) and torch.equal(lse[[0, 1, 2, 5, 6, 7, 8]], good_lse)
+        assert not out[3:5].any() and (lse[3:5] == -torch.inf).all()
+        out, lse = cache.decode(q[[0, 4, 1]], slots=slots, out=torch.full_like(q[:3], 7), lse=True)
+        with pytest.raises(RtaError, match="word 16$"):
+            cache.check()
+        assert torch.equal(out[[0, 2]], one) and torch.equal(lse[[0, 2]], one_lse)
+        assert not out[1].any() and (lse[1] == -torch.inf).all()
