@@ -83,9 +83,9 @@ struct Num<__half> {
   // multiple of 2^-24 below, and ends at 2^16.  A tile whose largest score is more
   // than kFar below the reference takes its own as the new one, unless it is
   // kNothing below the largest of all (a part of 2^-56 or less, and o and z stay
-  // within fp32 for 2^31 positions).  Behind a first token of zeros that takes all
-  // but e^-18 of the weight, 120 positions came out 3.5e-4 off with shift 10 and
-  // no kFar (fp32 results), now 1e-5.
+  // within fp32 for 2^31 positions).  Behind a first token that scores 18 nats
+  // above 120 others and holds zeros, fp32 results were 3.5e-4 off with shift 10
+  // and no kFar, now 1e-5.
   static constexpr float kShift = 15.f, kFar = 12.f, kNothing = 56.f;
   static constexpr bool kBf16 = false;
   static __device__ __forceinline__ __half from(float x) { return __float2half_rn(x); }
